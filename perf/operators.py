@@ -190,7 +190,8 @@ def _quantize(x):
     M, K = x.shape
     kb = -(-K // BLOCK)
     xp = torch.nn.functional.pad(x, (0, kb * BLOCK - K)).view(M, kb, BLOCK)
-    scale = (xp.abs().amax(2) / FP8_MAX).clamp_min(TINY)
+    top = xp.abs().amax(2)
+    scale = (top / torch.full_like(top, FP8_MAX)).clamp_min(TINY)  # by a tensor: by a number it would be a product with 1 / 448
     codes = (xp / scale.unsqueeze(2)).to(torch.float8_e4m3fn)
     return codes.view(M, kb * BLOCK)[:, :K].contiguous(), scale
 
