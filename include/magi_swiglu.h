@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define MAGI_SWIGLU_ABI_VERSION 8
+#define MAGI_SWIGLU_ABI_VERSION 9
 
 /* variant selector of magi_swiglu_forward_bf16 */
 #define MAGI_SWIGLU_VARIANT_AUTO   0  /* M <= 128 -> STREAM, else MMA2           */
@@ -268,6 +268,49 @@ int magi_swiglu_backward_dh_bf16(const void* x, const void* w_gate_up, const voi
                                  int64_t M, int64_t N, int64_t K,
                                  int64_t ldx, int64_t ldw, int64_t lddy, int64_t lddh,
                                  int device, void* cuda_stream);
+
+/* ---- Routed (mixture-of-experts) rows.  T tokens choose k experts each: slot s = t * k + j, R = T * k slots.
+ * row_slot[r] = s says which slot sorted row r holds (-1: none), slot_row[s] = r is its inverse (-1: slot s has no
+ * expert).  Index arrays are int32 in device memory; entries are bounds-checked by the kernels (out of range = none).
+ * Outputs are contiguous; H is the row length.  T == 0 is a successful no-op (the sort still writes its offsets). */
+
+/* Stable counting sort of `slots` expert ids (int32, or int64 when ids_64bit) into num_experts (<= 1024) contiguous row
+ * ranges: rows [offsets[e], offsets[e+1]) hold expert e's slots in slot order; ids outside [0, num_experts) have no
+ * expert, rows from offsets[num_experts] on hold none.  offsets has num_experts + 1 entries.  One launch, no scratch.
+ * It has no counterpart in the reference, whose models have no routed block. */
+int magi_swiglu_expert_sort(const void* ids, int ids_64bit, int64_t slots, int num_experts, int32_t* row_slot,
+                            int32_t* slot_row, int32_t* offsets, int device, void* cuda_stream);
+
+/* xs[r] = x[row_slot[r] / k], zeros where row_slot[r] is none: x [T, H] bf16 (row stride ldx), xs [T * k, H].
+ * H % 8 == 0, ldx % 8 == 0, 16-byte aligned pointers.  It has no counterpart in the reference. */
+int magi_swiglu_expert_gather_bf16(const void* x, const int32_t* row_slot, const int32_t* slot_row, void* xs, int64_t T,
+                                   int64_t k, int64_t H, int64_t ldx, int device, void* cuda_stream);
+
+/* out[t] = sum over j of weights[t * k + j] * y[slot_row[t * k + j]]: y [T * k, H] bf16 (row stride ldy), weights fp32
+ * [T * k] or NULL (ones: the gradient of the gather), out [T, H]; fp32 sums in slot order, one rounding to bf16; slots
+ * without an expert add nothing.  H % 8 == 0.  It has no counterpart in the reference. */
+int magi_swiglu_expert_combine_bf16(const void* y, const float* weights, const int32_t* slot_row, void* out, int64_t T,
+                                    int64_t k, int64_t H, int64_t ldy, int device, void* cuda_stream);
+
+/* The combine's gradients: dy[slot_row[s]] = weights[s] * dout[t] (zero rows where row_slot is none) and
+ * dw[s] = <dout[t], y[slot_row[s]]> in fp32 (0 where slot s has no expert).  dy or dw may be NULL (not wanted); y is read
+ * for dw only, weights and row_slot for dy only.  It has no counterpart in the reference. */
+int magi_swiglu_expert_combine_backward_bf16(const void* dout, const void* y, const float* weights, const int32_t* row_slot,
+                                             const int32_t* slot_row, void* dy, float* dw, int64_t T, int64_t k, int64_t H,
+                                             int64_t lddout, int64_t ldy, int device, void* cuda_stream);
+
+/* Block quantiser: x [M, K] bf16 -> codes [M, K] e4m3 and scales [M, ceil(K / 128)] fp32, per row and 128 columns
+ * scale = max(max|x| / 448, 2^-126), code = e4m3(x / scale) (IEEE divisions, round to nearest even).  A block with a NaN
+ * is all NaN; one with an infinity has scale inf and codes 0 (finite) or NaN (infinite).  K % 16 == 0, ldx % 8 == 0.
+ * It has no counterpart in the reference. */
+int magi_swiglu_quantize_fp8_block(const void* x, void* codes, float* scales, int64_t M, int64_t K, int64_t ldx, int device,
+                                   void* cuda_stream);
+
+/* The same quantiser on the way to the experts: rows of the gather above, each token read and quantised once.  Rows
+ * without a slot get zero codes and scale 2^-126.  It has no counterpart in the reference. */
+int magi_swiglu_expert_gather_fp8_block(const void* x, const int32_t* row_slot, const int32_t* slot_row, void* codes,
+                                        float* scales, int64_t T, int64_t k, int64_t K, int64_t ldx, int device,
+                                        void* cuda_stream);
 
 /* Scratch bytes the preferred schedule of magi_swiglu_forward_bf16_ws wants for this problem (0 = none needed;
  * negative = argument error).  Needs no GPU when sm_count > 0.

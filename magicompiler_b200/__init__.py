@@ -11,6 +11,9 @@ from .ops import (OP_NAME, fold_rmsnorm_weight, gemm_bf16, gemm_nt, gemm_nt_out,
                   rmsnorm_gemm_swiglu, set_gradient_gemms, swiglu_backward_act, swiglu_backward_dh)
 from .passes import FuseSwiGLUPass, install_into_magi_compiler, pack_gate_up_cached  # noqa: F401
 from .register import COMPUTE_SENSITIVE_OPS, SPLITTING_OPS, magi_register_custom_op  # noqa: F401
+from .routed import (expert_combine, expert_combine_backward, expert_combine_out, expert_gather, expert_gather_fp8,  # noqa: F401
+                     expert_gather_fp8_out, expert_gather_out, expert_sort, expert_sort_out, quantize_fp8_block,
+                     quantize_fp8_block_out)
 from .sharding import (  # noqa: F401
     ColumnParallelSwiGLU,
     PeerScatterReducer,
@@ -25,5 +28,7 @@ __all__ = [
     "gemm_swiglu", "gemm_swiglu_auto", "gemm_swiglu_fp8", "gemm_swiglu_nvfp4", "nvfp4_scale_shape", "gemm_swiglu_preact", "gemm_swiglu_train", "gemm_swiglu_out", "gemm_bf16", "gemm_nt", "gemm_nt_out", "swiglu_backward_act", "swiglu_backward_dh", "set_gradient_gemms", "rmsnorm_gemm_swiglu", "fold_rmsnorm_weight", "OP_NAME", "pack_gate_up", "shard_gate_up", "shard_down", "shard_bounds",
     "ColumnParallelSwiGLU", "TensorParallelSwiGLUMLP", "PeerScatterReducer", "FuseSwiGLUPass", "install_into_magi_compiler",
     "pack_gate_up_cached", "magi_register_custom_op", "SPLITTING_OPS",
+    "expert_sort", "expert_sort_out", "expert_gather", "expert_gather_out", "expert_combine", "expert_combine_out",
+    "expert_combine_backward", "expert_gather_fp8", "expert_gather_fp8_out", "quantize_fp8_block", "quantize_fp8_block_out",
     "COMPUTE_SENSITIVE_OPS", "build_library", "load_library", "plan", "workspace_bytes", "device_status", "kernel_clock", "MagiSwigluLibraryError",
 ]

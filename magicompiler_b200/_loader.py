@@ -16,8 +16,9 @@ _PKG = Path(__file__).resolve().parent
 CSRC = _PKG / "csrc"
 INCLUDE = _PKG.parent / "include"
 LIB_PATH = _PKG / "_lib" / "libmagi_swiglu.so"
-SOURCES = [CSRC / "swiglu_sm100.cu"]
-HEADERS = [CSRC / "ptx_sm100.cuh", CSRC / "swiglu_kernels.cuh", CSRC / "swiglu_plan.hpp", INCLUDE / "magi_swiglu.h"]
+SOURCES = [CSRC / "swiglu_sm100.cu", CSRC / "routed_sm100.cu"]
+HEADERS = [CSRC / "ptx_sm100.cuh", CSRC / "swiglu_kernels.cuh", CSRC / "swiglu_plan.hpp", CSRC / "host_common.hpp",
+           CSRC / "routed_kernels.cuh", INCLUDE / "magi_swiglu.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -25,7 +26,7 @@ NVCC_FLAGS = [
     "-shared", "-Xcompiler", "-fPIC",
 ]
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 VARIANT_AUTO, VARIANT_MMA, VARIANT_STREAM, VARIANT_SIMT, VARIANT_MMA2 = 0, 1, 2, 3, 4
 VARIANTS = {"auto": VARIANT_AUTO, "mma": VARIANT_MMA, "stream": VARIANT_STREAM, "simt": VARIANT_SIMT,
             "mma2": VARIANT_MMA2}
@@ -109,6 +110,18 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.magi_swiglu_sum_slots_bf16.argtypes = [vp, vp, i32, i64, i64, i32, vp]
     lib.magi_swiglu_sum_slots_bf16_bcast.restype = i32
     lib.magi_swiglu_sum_slots_bf16_bcast.argtypes = [vp, ctypes.POINTER(vp), i32, i32, i64, i64, i32, vp]
+    lib.magi_swiglu_expert_sort.restype = i32
+    lib.magi_swiglu_expert_sort.argtypes = [vp, i32, i64, i32, vp, vp, vp, i32, vp]
+    lib.magi_swiglu_expert_gather_bf16.restype = i32
+    lib.magi_swiglu_expert_gather_bf16.argtypes = [vp, vp, vp, vp, i64, i64, i64, i64, i32, vp]
+    lib.magi_swiglu_expert_combine_bf16.restype = i32
+    lib.magi_swiglu_expert_combine_bf16.argtypes = [vp, vp, vp, vp, i64, i64, i64, i64, i32, vp]
+    lib.magi_swiglu_expert_combine_backward_bf16.restype = i32
+    lib.magi_swiglu_expert_combine_backward_bf16.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i32, vp]
+    lib.magi_swiglu_quantize_fp8_block.restype = i32
+    lib.magi_swiglu_quantize_fp8_block.argtypes = [vp, vp, vp, i64, i64, i64, i32, vp]
+    lib.magi_swiglu_expert_gather_fp8_block.restype = i32
+    lib.magi_swiglu_expert_gather_fp8_block.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, i32, vp]
     lib.magi_swiglu_backward_act_bf16.restype = i32
     lib.magi_swiglu_backward_act_bf16.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i32, vp]
     lib.magi_swiglu_workspace_bytes.restype = i64

@@ -1,0 +1,362 @@
+// Device code of the routed (mixture-of-experts) row movements: tokens sorted by expert, gathered into expert order (bf16,
+// or quantised to block-scaled fp8 on the way), added up again with the router's weights, and the gradients of both.
+//
+//   slot s = t * k + j        the j-th expert choice of token t
+//   row_slot[r] = s           which slot sorted row r holds (-1: none, a row behind the last expert's)
+//   slot_row[s] = r           where slot s went (-1: the slot has no expert)
+//
+// All of them are bound by HBM: the arithmetic is a few operations per byte.  What counts is that every token row is
+// read ONCE however many experts it goes to (the kernels walk tokens, not sorted rows), that accesses are 16 bytes wide
+// and contiguous per row, and that a call is one launch.  Indices read from memory are bounds-checked: one that is out of
+// range counts as "no expert", so a bad index array gives wrong rows but no access outside the operands.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "ptx_sm100.cuh"
+
+namespace magi {
+
+constexpr int kMaxExperts = 1024;   // one 32-warp histogram of 1025 counters is 131 KB of shared memory
+constexpr int kSlotBatch = 8;       // expert rows of one token in flight per thread
+constexpr float kFp8Max = 448.0f;   // largest e4m3 value
+constexpr float kScaleFloor = 1.17549435e-38f;  // 2^-126: a block of zeros (or of subnormals) keeps a normal scale
+
+// ---------------------------------------------------------------- sort
+// Stable counting sort of the slots by expert, slots without an expert last.  One thread-block cluster does it in one
+// launch: each warp owns a contiguous range of slots and a histogram row; __match_any_sync ranks equal keys inside a
+// warp step, so ties keep slot order and no atomic decides anything.  The CTAs of the cluster read each other's totals
+// through distributed shared memory.  hist: [warps][E + 1], total: [E + 1], start: [E + 1].
+__device__ __forceinline__ int ld_cluster_s32(uint32_t cluster_addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ int slot_key(const void* ids, int wide, int s, int end, int E) {
+  if (s >= end) return -1;  // no slot: matches only other absent lanes
+  const long long v = wide ? static_cast<const long long*>(ids)[s] : (long long)static_cast<const int*>(ids)[s];
+  return (v >= 0 && v < E) ? (int)v : E;
+}
+
+__global__ void __launch_bounds__(1024, 1)
+expert_sort_kernel(const void* ids, int wide, int R, int E, int* row_slot, int* slot_row, int* offsets, int ctas) {
+  extern __shared__ int sort_smem[];
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int buckets = E + 1;
+  int* hist = sort_smem + warp * buckets;
+  int* total = sort_smem + warps * buckets;
+  int* start = total + buckets;
+  const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
+
+  // a warp's share, a multiple of 32 slots
+  const int units = ctas * warps;
+  const long long share = (((long long)R + units - 1) / units + 31) / 32 * 32;
+  const long long first = share * (rank * warps + warp);
+  const int lo = (int)(first < R ? first : R), hi = (int)(first + share < R ? first + share : R);
+
+  for (int i = threadIdx.x; i < warps * buckets; i += blockDim.x) sort_smem[i] = 0;
+  __syncthreads();
+  for (int b = lo; b < hi; b += 128) {
+    int key[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) key[i] = slot_key(ids, wide, b + 32 * i + lane, hi, E);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned same = __match_any_sync(0xffffffffu, key[i]);
+      if (key[i] >= 0 && (same & ((1u << lane) - 1u)) == 0) hist[key[i]] += __popc(same);
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  // histogram column e -> exclusive prefix over this CTA's warps, and the CTA's total
+  for (int e = threadIdx.x; e < buckets; e += blockDim.x) {
+    int sum = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int n = sort_smem[w * buckets + e];
+      sort_smem[w * buckets + e] = sum;
+      sum += n;
+    }
+    total[e] = sum;
+  }
+  __syncthreads();
+  if (ctas > 1) cluster_sync_all();
+  // start[e] = slots of lower buckets (everywhere) + slots of this bucket in lower CTAs
+  if (warp == 0) {
+    int carry = 0;
+    for (int b = 0; b < buckets; b += 32) {
+      const int e = b + lane;
+      int all = 0, before = 0;
+      if (e < buckets) {
+        if (ctas == 1) {
+          all = total[e];
+        } else {
+          for (int c = 0; c < ctas; ++c) {
+            const int n = ld_cluster_s32(map_to_cta(smem_u32(total + e), c));
+            before += c < rank ? n : 0;
+            all += n;
+          }
+        }
+      }
+      int scan = all;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += up;
+      }
+      if (e < buckets) {
+        start[e] = carry + scan - all + before;
+        if (rank == 0) offsets[e] = carry + scan - all;  // offsets[E] = first slot without an expert
+      }
+      carry += __shfl_sync(0xffffffffu, scan, 31);
+    }
+  }
+  __syncthreads();
+  for (int b = lo; b < hi; b += 128) {
+    int key[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) key[i] = slot_key(ids, wide, b + 32 * i + lane, hi, E);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned same = __match_any_sync(0xffffffffu, key[i]);
+      const unsigned lower = same & ((1u << lane) - 1u);
+      const int base = key[i] >= 0 ? hist[key[i]] : 0;
+      __syncwarp();
+      if (key[i] >= 0) {
+        if (lower == 0) hist[key[i]] = base + __popc(same);
+        const int s = b + 32 * i + lane;
+        const int r = start[key[i]] + base + __popc(lower);
+        row_slot[r] = key[i] < E ? s : -1;
+        slot_row[s] = key[i] < E ? r : -1;
+      }
+      __syncwarp();
+    }
+  }
+  if (ctas > 1) cluster_sync_all();  // nobody leaves while its totals may still be read
+}
+
+// ---------------------------------------------------------------- row movement
+// Thread (x, y) of block b: token (b / col_chunks) * blockDim.y + y, 16-byte column piece (b % col_chunks) * blockDim.x + x.
+struct RowPiece {
+  long long t;
+  int c;
+};
+__device__ __forceinline__ RowPiece row_piece(int col_chunks) {
+  RowPiece p;
+  p.t = (long long)(blockIdx.x / col_chunks) * blockDim.y + threadIdx.y;
+  p.c = (blockIdx.x % col_chunks) * blockDim.x + threadIdx.x;
+  return p;
+}
+__device__ __forceinline__ uint4 ld_stream(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
+
+// xs[slot_row[t, j]] = x[t]; row t * k + j is zeroed when it holds no slot.
+__global__ void __launch_bounds__(256)
+expert_gather_kernel(const uint4* x, long long ldx, const int* row_slot, const int* slot_row, uint4* xs, long long T, int k,
+                     int vecs, int col_chunks) {
+  const RowPiece p = row_piece(col_chunks);
+  if (p.t >= T || p.c >= vecs) return;
+  const long long R = T * k;
+  const uint4 v = ld_stream(x + p.t * ldx + p.c);
+  for (int j = 0; j < k; ++j) {
+    const long long s = p.t * k + j;
+    const int r = slot_row[s];
+    if (r >= 0 && r < R) xs[(long long)r * vecs + p.c] = v;
+    if (row_slot[s] < 0) xs[s * vecs + p.c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ void bf16x8_to_f32(uint4 v, float (&f)[8]) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(u[i] << 16);
+    f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 f32_to_bf16x8(const float (&f)[8]) {
+  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+
+// out[t] = sum over j of w[t, j] * y[slot_row[t, j]] in fp32, j ascending, one rounding; w null: all ones (the gradient of
+// the gather).  Slots without an expert add nothing, whatever their weight.
+__global__ void __launch_bounds__(256)
+expert_combine_kernel(const uint4* y, long long ldy, const float* w, const int* slot_row, uint4* out, long long T, int k,
+                      int vecs, int col_chunks) {
+  const RowPiece p = row_piece(col_chunks);
+  if (p.t >= T || p.c >= vecs) return;
+  const long long R = T * k;
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int j0 = 0; j0 < k; j0 += kSlotBatch) {
+    uint4 v[kSlotBatch];
+    float wj[kSlotBatch];
+    int r[kSlotBatch];
+#pragma unroll
+    for (int i = 0; i < kSlotBatch; ++i) {
+      const long long s = p.t * k + j0 + i;
+      r[i] = j0 + i < k ? slot_row[s] : -1;
+      if (r[i] >= R) r[i] = -1;
+      wj[i] = (r[i] >= 0 && w) ? w[s] : 1.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kSlotBatch; ++i)
+      if (r[i] >= 0) v[i] = ld_stream(y + (long long)r[i] * ldy + p.c);
+#pragma unroll
+    for (int i = 0; i < kSlotBatch; ++i)
+      if (r[i] >= 0) {
+        float f[8];
+        bf16x8_to_f32(v[i], f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] = fmaf(wj[i], f[q], acc[q]);
+      }
+  }
+  out[p.t * vecs + p.c] = f32_to_bf16x8(acc);
+}
+
+// The combine's gradients in one pass: dy[slot_row[t, j]] = w[t, j] * dout[t] (rows without a slot are zeroed) and
+// dw[t, j] = <dout[t], y[slot_row[t, j]]> (0 for a slot without an expert), sums in fp32 in a fixed order.
+// token_warps warps (1, 2, 4 or 8) share a token.  dy or dw may be null (y is not read without dw).
+__global__ void __launch_bounds__(256)
+expert_combine_backward_kernel(const uint4* dout, long long lddout, const uint4* y, long long ldy, const float* w,
+                               const int* row_slot, const int* slot_row, uint4* dy, float* dw, long long T, int k, int vecs,
+                               int token_warps) {
+  __shared__ float red[8][kSlotBatch];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = warp % token_warps;
+  const long long t = (long long)blockIdx.x * (8 / token_warps) + warp / token_warps;
+  const bool here = t < T;
+  const long long R = T * k;
+  const int step = token_warps * 32;
+  for (int j0 = 0; j0 < k; j0 += kSlotBatch) {
+    float dot[kSlotBatch], wj[kSlotBatch];
+    int r[kSlotBatch];
+    unsigned empty = 0;  // bit i: row t * k + j0 + i holds no slot
+#pragma unroll
+    for (int i = 0; i < kSlotBatch; ++i) {
+      const long long s = t * k + j0 + i;
+      const bool on = here && j0 + i < k;
+      dot[i] = 0.0f;
+      r[i] = on ? slot_row[s] : -1;
+      if (r[i] >= R) r[i] = -1;
+      wj[i] = (r[i] >= 0 && dy) ? w[s] : 0.0f;
+      if (on && dy && row_slot[s] < 0) empty |= 1u << i;
+    }
+    if (here)
+      for (int c = part * 32 + lane; c < vecs; c += step) {
+        float d[8];
+        uint4 v[kSlotBatch];
+        const uint4 dv = dout[t * lddout + c];
+        if (dw) {
+#pragma unroll
+          for (int i = 0; i < kSlotBatch; ++i)
+            if (r[i] >= 0) v[i] = ld_stream(y + (long long)r[i] * ldy + c);
+        }
+        bf16x8_to_f32(dv, d);
+#pragma unroll
+        for (int i = 0; i < kSlotBatch; ++i) {
+          if (dw && r[i] >= 0) {
+            float f[8];
+            bf16x8_to_f32(v[i], f);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) dot[i] = fmaf(d[q], f[q], dot[i]);
+          }
+          if (dy && r[i] >= 0) {
+            float f[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) f[q] = wj[i] * d[q];
+            dy[(long long)r[i] * vecs + c] = f32_to_bf16x8(f);
+          }
+          if (empty >> i & 1u) dy[(t * k + j0 + i) * vecs + c] = make_uint4(0, 0, 0, 0);
+        }
+      }
+    if (dw) {
+#pragma unroll
+      for (int i = 0; i < kSlotBatch; ++i)
+#pragma unroll
+        for (int o = 16; o; o >>= 1) dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], o);
+      if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < kSlotBatch; ++i) red[warp][i] = dot[i];
+      __syncthreads();
+      if (here && part == 0 && lane < kSlotBatch && j0 + lane < k) {
+        float sum = 0.0f;
+        for (int q = 0; q < token_warps; ++q) sum += red[warp + q][lane];
+        dw[t * k + j0 + lane] = sum;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// ---------------------------------------------------------------- block quantiser
+// Per row and 128 columns: s = max(max|x| / 448, 2^-126), q = e4m3(x / s).  Eight lanes hold a block (16 columns each).
+// The maximum is taken on the bf16 bit patterns without their sign, which order like the values and put infinities and
+// NaN on top: a block with an infinity gets s = inf (its finite elements become 0, the infinity NaN), one with a NaN is
+// all NaN.  Both divisions are IEEE divisions, so codes and scales equal the formula evaluated in fp32 bit for bit.
+__device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+__device__ __forceinline__ float block_scale(float amax) {
+  const float s = __fdiv_rn(amax, kFp8Max);
+  return s < kScaleFloor ? kScaleFloor : s;  // a NaN stays
+}
+
+// slot_row null: codes[t], scales[t] from x[t].  Else the quantised gather: token t goes to rows slot_row[t, j] and row
+// t * k + j gets zero codes and the floor scale when it holds no slot.
+__global__ void __launch_bounds__(256)
+quantize_fp8_block_kernel(const uint4* x, long long ldx, const int* row_slot, const int* slot_row, uint4* codes,
+                          float* scales, long long T, int k, int pieces, int col_chunks, int kb) {
+  const RowPiece p = row_piece(col_chunks);
+  const bool on = p.t < T && p.c < pieces;
+  uint4 a = make_uint4(0, 0, 0, 0), b = a;
+  if (on) {
+    a = ld_stream(x + p.t * ldx + 2 * p.c);
+    b = ld_stream(x + p.t * ldx + 2 * p.c + 1);
+  }
+  const uint32_t m = 0x7fff7fffu;
+  uint32_t top = __vmaxu2(__vmaxu2(__vmaxu2(a.x & m, a.y & m), __vmaxu2(a.z & m, a.w & m)),
+                          __vmaxu2(__vmaxu2(b.x & m, b.y & m), __vmaxu2(b.z & m, b.w & m)));
+  top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float s = block_scale(__uint_as_float(top << 16));
+  if (!on) return;
+  float f[8], g[8];
+  bf16x8_to_f32(a, f);
+  bf16x8_to_f32(b, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    f[i] = __fdiv_rn(f[i], s);
+    g[i] = __fdiv_rn(g[i], s);
+  }
+  const uint4 q = make_uint4(pack4_e4m3(f[0], f[1], f[2], f[3]), pack4_e4m3(f[4], f[5], f[6], f[7]),
+                             pack4_e4m3(g[0], g[1], g[2], g[3]), pack4_e4m3(g[4], g[5], g[6], g[7]));
+  const bool writes_scale = (p.c & 7) == 0;
+  if (!slot_row) {
+    codes[p.t * pieces + p.c] = q;
+    if (writes_scale) scales[p.t * kb + (p.c >> 3)] = s;
+    return;
+  }
+  const long long R = T * k;
+  for (int j = 0; j < k; ++j) {
+    const long long sl = p.t * k + j;
+    const int r = slot_row[sl];
+    if (r >= 0 && r < R) {
+      codes[(long long)r * pieces + p.c] = q;
+      if (writes_scale) scales[(long long)r * kb + (p.c >> 3)] = s;
+    }
+    if (row_slot[sl] < 0) {
+      codes[sl * pieces + p.c] = make_uint4(0, 0, 0, 0);
+      if (writes_scale) scales[sl * kb + (p.c >> 3)] = kScaleFloor;
+    }
+  }
+}
+
+}  // namespace magi

@@ -1,0 +1,188 @@
+// C ABI of the routed row movements and the block quantiser (include/magi_swiglu.h): argument checks and launches.
+// Device code lives in routed_kernels.cuh.
+#include "host_common.hpp"
+#include "routed_kernels.cuh"
+
+namespace magi {
+
+// Threads of a block over one row's 16-byte pieces (x) and several rows (y), and how many blocks cover a row.
+struct RowGrid {
+  dim3 block;
+  unsigned grid;
+  int col_chunks;
+};
+static int row_grid(int64_t rows, int64_t pieces, RowGrid* g) {
+  const int64_t wide = (pieces + 31) / 32 * 32;
+  const unsigned bx = (unsigned)(wide < 256 ? wide : 256), by = 256 / bx;
+  const int64_t chunks = (pieces + bx - 1) / bx, blocks = (rows + by - 1) / by * chunks;
+  if (blocks > 0x7fffffffLL) return fail(MAGI_SWIGLU_ERR_SHAPE, "too many rows x columns for one launch");
+  g->block = dim3(bx, by);
+  g->grid = (unsigned)blocks;
+  g->col_chunks = (int)chunks;
+  return 0;
+}
+
+static int check_rows(int64_t T, int64_t k, int64_t H, int64_t ld, int multiple) {
+  if (T < 0 || k < 1 || H < 1 || T > 0x7fffffffLL / k)
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "T=%lld, k=%lld, H=%lld out of range (T * k < 2^31)", (long long)T, (long long)k,
+                (long long)H);
+  if (H % multiple) return fail(MAGI_SWIGLU_ERR_SHAPE, "the row length %lld must be a multiple of %d", (long long)H, multiple);
+  if (H > 0x7fffffffLL || ld < H) return fail(MAGI_SWIGLU_ERR_SHAPE, "row stride %lld too small for %lld columns", (long long)ld, (long long)H);
+  if (ld % 8) return fail(MAGI_SWIGLU_ERR_ALIGN, "row strides must be multiples of 8 elements");
+  return 0;
+}
+static bool unaligned(const void* a, const void* b = nullptr, const void* c = nullptr) {
+  return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15u) != 0;
+}
+
+static int quantize(const void* x, const int32_t* row_slot, const int32_t* slot_row, void* codes, float* scales, int64_t T,
+                    int64_t k, int64_t K, int64_t ldx, int device, void* stream) {
+  if (int rc = check_rows(T, k, K, ldx, 16)) return rc;
+  if (T == 0) return 0;
+  if (!x || !codes || !scales) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  if (unaligned(x, codes)) return fail(MAGI_SWIGLU_ERR_ALIGN, "x and codes must be 16-byte aligned");
+  const DeviceInfo* di = nullptr;
+  if (int rc = require_b200(device, &di)) return rc;
+  RowGrid g;
+  if (int rc = row_grid(T, K / 16, &g)) return rc;
+  DeviceGuard guard;
+  cudaError_t e = guard.set(device);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  quantize_fp8_block_kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint4*>(x), ldx / 8, row_slot, slot_row, static_cast<uint4*>(codes), scales, T, (int)k,
+      (int)(K / 16), g.col_chunks, (int)((K + 127) / 128));
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : fail_cuda(e, "launch of quantize_fp8_block_kernel");
+}
+
+}  // namespace magi
+
+using namespace magi;
+
+extern "C" {
+
+int magi_swiglu_expert_sort(const void* ids, int ids_64bit, int64_t slots, int num_experts, int32_t* row_slot,
+                            int32_t* slot_row, int32_t* offsets, int device, void* cuda_stream) {
+  g_err[0] = 0;
+  if (slots < 0 || slots > 0x3fffffffLL) return fail(MAGI_SWIGLU_ERR_SHAPE, "slots=%lld out of range [0, 2^30)", (long long)slots);
+  if (num_experts < 1 || num_experts > kMaxExperts)
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "num_experts=%d out of range [1, %d]", num_experts, kMaxExperts);
+  if (!offsets || (slots > 0 && (!ids || !row_slot || !slot_row))) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  if (((uintptr_t)ids & (ids_64bit ? 7u : 3u)) || (((uintptr_t)row_slot | (uintptr_t)slot_row | (uintptr_t)offsets) & 3u))
+    return fail(MAGI_SWIGLU_ERR_ALIGN, "index arrays must be aligned to their element size");
+  const DeviceInfo* di = nullptr;
+  if (int rc = require_b200(device, &di)) return rc;
+  DeviceGuard guard;
+  cudaError_t e = guard.set(device);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  // A warp step handles 32 slots; a warp gets at least 128 of them before another joins, and one CTA's 32 warps at least
+  // 256 each before the cluster grows: the cluster barrier and the remote totals cost about as much as that many steps.
+  int warps = (int)((slots + 127) / 128);
+  warps = warps < 4 ? 4 : (warps > 32 ? 32 : warps);
+  int ctas = 1;
+  while (ctas < 8 && slots > (int64_t)ctas * 32 * 256) ctas *= 2;
+  const size_t smem = (size_t)(warps + 2) * (num_experts + 1) * sizeof(int);
+  e = cudaFuncSetAttribute(expert_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)((32 + 2) * (kMaxExperts + 1) * sizeof(int)));
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)warps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(cuda_stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, expert_sort_kernel, ids, ids_64bit, (int)slots, num_experts, (int*)row_slot, (int*)slot_row,
+                         (int*)offsets, ctas);
+  return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_sort_kernel");
+}
+
+int magi_swiglu_expert_gather_bf16(const void* x, const int32_t* row_slot, const int32_t* slot_row, void* xs, int64_t T,
+                                   int64_t k, int64_t H, int64_t ldx, int device, void* cuda_stream) {
+  g_err[0] = 0;
+  if (int rc = check_rows(T, k, H, ldx, 8)) return rc;
+  if (T == 0) return 0;
+  if (!x || !row_slot || !slot_row || !xs) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  if (unaligned(x, xs)) return fail(MAGI_SWIGLU_ERR_ALIGN, "x and xs must be 16-byte aligned");
+  const DeviceInfo* di = nullptr;
+  if (int rc = require_b200(device, &di)) return rc;
+  RowGrid g;
+  if (int rc = row_grid(T, H / 8, &g)) return rc;
+  DeviceGuard guard;
+  cudaError_t e = guard.set(device);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  expert_gather_kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
+      static_cast<const uint4*>(x), ldx / 8, row_slot, slot_row, static_cast<uint4*>(xs), T, (int)k, (int)(H / 8),
+      g.col_chunks);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_gather_kernel");
+}
+
+int magi_swiglu_expert_combine_bf16(const void* y, const float* weights, const int32_t* slot_row, void* out, int64_t T,
+                                    int64_t k, int64_t H, int64_t ldy, int device, void* cuda_stream) {
+  g_err[0] = 0;
+  if (int rc = check_rows(T, k, H, ldy, 8)) return rc;
+  if (T == 0) return 0;
+  if (!y || !slot_row || !out) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  if (unaligned(y, out)) return fail(MAGI_SWIGLU_ERR_ALIGN, "y and out must be 16-byte aligned");
+  const DeviceInfo* di = nullptr;
+  if (int rc = require_b200(device, &di)) return rc;
+  RowGrid g;
+  if (int rc = row_grid(T, H / 8, &g)) return rc;
+  DeviceGuard guard;
+  cudaError_t e = guard.set(device);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  expert_combine_kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
+      static_cast<const uint4*>(y), ldy / 8, weights, slot_row, static_cast<uint4*>(out), T, (int)k, (int)(H / 8),
+      g.col_chunks);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_combine_kernel");
+}
+
+int magi_swiglu_expert_combine_backward_bf16(const void* dout, const void* y, const float* weights, const int32_t* row_slot,
+                                             const int32_t* slot_row, void* dy, float* dw, int64_t T, int64_t k, int64_t H,
+                                             int64_t lddout, int64_t ldy, int device, void* cuda_stream) {
+  g_err[0] = 0;
+  if (int rc = check_rows(T, k, H, lddout, 8)) return rc;
+  if (dw)
+    if (int rc = check_rows(T, k, H, ldy, 8)) return rc;
+  if (T == 0 || (!dy && !dw)) return 0;
+  if (!dout || !slot_row || (dy && (!weights || !row_slot)) || (dw && !y)) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  if (unaligned(dout, dw ? y : nullptr, dy)) return fail(MAGI_SWIGLU_ERR_ALIGN, "dout, y and dy must be 16-byte aligned");
+  const DeviceInfo* di = nullptr;
+  if (int rc = require_b200(device, &di)) return rc;
+  DeviceGuard guard;
+  cudaError_t e = guard.set(device);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  // One warp walks a whole token when there are enough tokens to fill the GPU (8 warps a block, 8 blocks an SM); few
+  // tokens get up to eight warps each, as far as the row has pieces for them.
+  int token_warps = 1;
+  while (token_warps < 8 && T * token_warps < (int64_t)di->sm_count * 32 && H / 8 > token_warps * 32) token_warps *= 2;
+  const int64_t blocks = (T + 8 / token_warps - 1) / (8 / token_warps);
+  expert_combine_backward_kernel<<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
+      static_cast<const uint4*>(dout), lddout / 8, static_cast<const uint4*>(y), ldy / 8, weights, row_slot, slot_row,
+      static_cast<uint4*>(dy), dw, T, (int)k, (int)(H / 8), token_warps);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_combine_backward_kernel");
+}
+
+int magi_swiglu_quantize_fp8_block(const void* x, void* codes, float* scales, int64_t M, int64_t K, int64_t ldx, int device,
+                                   void* cuda_stream) {
+  g_err[0] = 0;
+  return quantize(x, nullptr, nullptr, codes, scales, M, 1, K, ldx, device, cuda_stream);
+}
+
+int magi_swiglu_expert_gather_fp8_block(const void* x, const int32_t* row_slot, const int32_t* slot_row, void* codes,
+                                        float* scales, int64_t T, int64_t k, int64_t K, int64_t ldx, int device,
+                                        void* cuda_stream) {
+  g_err[0] = 0;
+  if (T > 0 && (!row_slot || !slot_row)) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  return quantize(x, row_slot, slot_row, codes, scales, T, k, K, ldx, device, cuda_stream);
+}
+
+}  // extern "C"

@@ -1,32 +1,17 @@
 // Host-side schedule selection for the SwiGLU kernels: which variant, tile width, ring depth, raster band, CTA
-// count and (for narrow small-M problems) how many CTAs split K, plus the error-text helpers of the C ABI.
+// count and (for narrow small-M problems) how many CTAs split K.
 // Pure host arithmetic: nothing here touches a GPU.
 #pragma once
-#include <cstdarg>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 
 #include "../../include/magi_swiglu.h"
+#include "host_common.hpp"
 #include "swiglu_kernels.cuh"
 
 namespace magi {
-
-thread_local char g_err[512] = "";
-
-static int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-static int fail_cuda(cudaError_t e, const char* what) {
-  snprintf(g_err, sizeof(g_err), "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
-  cudaGetLastError();  // the error has been reported here: do not leave it for the next, unrelated launch check
-  return e == cudaSuccess ? 1 : (int)e;
-}
 
 // Tuning aids.  Their initial values are read from the environment ONCE (first use), never on the launch path; tests
 // and sweeps change them afterwards through magi_swiglu_tuning():

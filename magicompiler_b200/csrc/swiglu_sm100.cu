@@ -2,63 +2,19 @@
 // kernel launches.  Device code lives in swiglu_kernels.cuh, schedule selection in swiglu_plan.hpp.
 #include <cuda_runtime.h>
 
-#include <mutex>
-
 #include "../../include/magi_swiglu.h"
+#include "host_common.hpp"
 #include "swiglu_kernels.cuh"
 #include "swiglu_plan.hpp"
 
 namespace magi {
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn tensor_map_encoder() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
-    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess) return (EncodeTiledFn) nullptr;
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
-
-constexpr int kMaxDevices = 64;
-struct DeviceInfo {
-  int queried = 0;  // 1 = ok, -1 = unusable
-  int sm_count = 0;
-  int cc_major = 0, cc_minor = 0;
-  int smem_optin_set = 0;
-  int pair_clusters = 0;  // co-resident 2-CTA clusters of the pair kernel (0 = not queried yet, -1 = none)
-};
-static DeviceInfo g_dev[kMaxDevices];
 struct ScatterSet {  // what magi_swiglu_scatter_setup last wrote into g_scatter_maps[set] of a device
   int world = 0;
   int64_t rows = 0, n = 0;
 };
 static ScatterSet g_scatter[kMaxDevices][2];
-static std::mutex g_dev_mutex;
 
-static const DeviceInfo* device_info(int device) {
-  if (device < 0 || device >= kMaxDevices) return nullptr;
-  std::lock_guard<std::mutex> lock(g_dev_mutex);
-  DeviceInfo& d = g_dev[device];
-  if (d.queried == 0) {
-    int n = 0;
-    if (cudaGetDeviceCount(&n) != cudaSuccess || device >= n) {
-      cudaGetLastError();
-      d.queried = -1;
-    } else {
-      cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, device);
-      cudaDeviceGetAttribute(&d.cc_major, cudaDevAttrComputeCapabilityMajor, device);
-      cudaDeviceGetAttribute(&d.cc_minor, cudaDevAttrComputeCapabilityMinor, device);
-      d.queried = 1;
-    }
-  }
-  return d.queried == 1 ? &d : nullptr;
-}
 // A 2-D map over a matrix stored with the reduction index as the row index ([K, cols], row stride ld elements):
 // boxes of 64 columns x 64 K rows, i.e. one 128-byte swizzled line per K index (the MN-major operand tile).
 static int encode_mn_major_map(EncodeTiledFn enc, const void* ptr, int64_t cols, int64_t K, int64_t ld, CUtensorMap* tm,
@@ -131,24 +87,6 @@ static int encode_y_map(const void* y, int64_t rows, int64_t cols, int64_t halve
   if (r != CUDA_SUCCESS) return fail(MAGI_SWIGLU_ERR_DRIVER, "tensor map for Y rejected by the driver (CUresult %d)", (int)r);
   return 0;
 }
-
-struct DeviceGuard {
-  int prev = -1;
-  bool changed = false;
-  cudaError_t set(int device) {
-    cudaError_t e = cudaGetDevice(&prev);
-    if (e != cudaSuccess) return e;
-    // Always set the device, even when it already is the current one: on a thread that has made no CUDA call yet
-    // (an autograd worker, say) this is what binds the device's primary context, which the driver-level
-    // tensor-map encoder needs.
-    e = cudaSetDevice(device);
-    changed = (e == cudaSuccess && prev != device);
-    return e;
-  }
-  ~DeviceGuard() {
-    if (changed) cudaSetDevice(prev);
-  }
-};
 
 static int forward_impl(const void* x, const void* w, void* y, int64_t M, int64_t N, int64_t K, int64_t ldx,
                         int64_t ldw, int64_t ldy, int device, void* stream_v, int variant, int block_n, int stages,
