@@ -312,6 +312,33 @@ int magi_swiglu_expert_gather_fp8_block(const void* x, const int32_t* row_slot, 
                                         float* scales, int64_t T, int64_t k, int64_t K, int64_t ldx, int device,
                                         void* cuda_stream);
 
+/* ---- Block-scaled fp8 products.  Codes are e4m3 bytes; a_scale holds one fp32 scale per row of A and 128 K elements
+ * ([M, ceil(K/128)], row stride ld_scale), b_scale one per 128 x 128 block of B.  With `offsets` (num_experts + 1 int32 in
+ * device memory, clamped to [0, M] by the kernel; they must not decrease) rows [offsets[e], offsets[e+1]) of A meet B[e];
+ * rows from offsets[num_experts] on are written as zeros when zero_tail is set and left as they are otherwise.  Without
+ * offsets num_experts is 1.  Sums are fp32.  K % 16 == 0, lda % 16 == 0, 16-byte aligned a, b, c, codes; B and the outputs
+ * are contiguous.  M == 0 is a successful no-op.  Rows of A with a NaN scale or code give NaN. */
+
+/* C[M, N] (bf16, one rounding) = sum over K blocks of a_scale * b_scale * (A codes . B codes^T): A [M, K], B
+ * [num_experts, N, K], b_scale [num_experts, ceil(N/128), ceil(K/128)].  N % 8 == 0.
+ * Replaces: the library GEMM behind self.down_proj(...) (tests/model_definition.py:339) when weights and activations are
+ * held in 8 bits; the reference itself has no 8-bit GEMM. */
+int magi_swiglu_gemm_fp8_block(const void* a, const float* a_scale, const void* b, const float* b_scale,
+                               const int32_t* offsets, int num_experts, void* c, int64_t M, int64_t N, int64_t K,
+                               int64_t lda, int64_t ld_scale, int zero_tail, int device, void* cuda_stream);
+
+/* The fused SwiGLU form: y = silu(A . Wg^T) * (A . Wu^T) on the scaled fp32 sums, quantised in the epilogue to codes [M, N]
+ * e4m3 and scales [M, ceil(N/128)] fp32 (scale = max(max|y| / 448, 2^-126) per row and 128 columns, code = e4m3(y / scale)):
+ * what magi_swiglu_gemm_fp8_block reads next.  w_gate_up [num_experts, 2N, K], gate rows first; w_scale [num_experts,
+ * 2 * ceil(N/128), ceil(K/128)], the blocks of the gate half, then those of the up half (each half is blocked from its own
+ * first row).  N % 16 == 0.
+ * Replaces: gate = F.silu(gate_proj(x)); up = up_proj(x); gate * up (tests/model_definition.py:337-339) in 8 bits, with
+ * the quantising activation of passes/piecewise_graph/fix_functionalization.py:110-112. */
+int magi_swiglu_gemm_swiglu_fp8_block(const void* a, const float* a_scale, const void* w_gate_up, const float* w_scale,
+                                      const int32_t* offsets, int num_experts, void* codes, float* scales, int64_t M,
+                                      int64_t N, int64_t K, int64_t lda, int64_t ld_scale, int zero_tail, int device,
+                                      void* cuda_stream);
+
 /* Scratch bytes the preferred schedule of magi_swiglu_forward_bf16_ws wants for this problem (0 = none needed;
  * negative = argument error).  Needs no GPU when sm_count > 0.
  * Replaces: nothing in the reference. */

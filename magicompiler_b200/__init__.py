@@ -6,6 +6,8 @@ before ahead-of-time artifacts that mention the op are deserialised.
 """
 from ._loader import (MagiSwigluLibraryError, build_library, device_status, kernel_clock, load_library,  # noqa: F401
                       plan, workspace_bytes)
+from .fp8_block import (gemm_fp8_block, gemm_fp8_block_out, gemm_swiglu_fp8_block, gemm_swiglu_fp8_block_out,  # noqa: F401
+                        quantize_fp8_gate_up, quantize_fp8_weight)
 from .ops import (OP_NAME, fold_rmsnorm_weight, gemm_bf16, gemm_nt, gemm_nt_out, gemm_swiglu, gemm_swiglu_fp8, gemm_swiglu_out,  # noqa: F401
                   gemm_swiglu_auto, gemm_swiglu_nvfp4, gemm_swiglu_preact, gemm_swiglu_train, nvfp4_scale_shape,
                   rmsnorm_gemm_swiglu, set_gradient_gemms, swiglu_backward_act, swiglu_backward_dh)
@@ -30,5 +32,7 @@ __all__ = [
     "pack_gate_up_cached", "magi_register_custom_op", "SPLITTING_OPS",
     "expert_sort", "expert_sort_out", "expert_gather", "expert_gather_out", "expert_combine", "expert_combine_out",
     "expert_combine_backward", "expert_gather_fp8", "expert_gather_fp8_out", "quantize_fp8_block", "quantize_fp8_block_out",
+    "gemm_fp8_block", "gemm_fp8_block_out", "gemm_swiglu_fp8_block", "gemm_swiglu_fp8_block_out", "quantize_fp8_weight",
+    "quantize_fp8_gate_up",
     "COMPUTE_SENSITIVE_OPS", "build_library", "load_library", "plan", "workspace_bytes", "device_status", "kernel_clock", "MagiSwigluLibraryError",
 ]

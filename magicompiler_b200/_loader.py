@@ -16,9 +16,9 @@ _PKG = Path(__file__).resolve().parent
 CSRC = _PKG / "csrc"
 INCLUDE = _PKG.parent / "include"
 LIB_PATH = _PKG / "_lib" / "libmagi_swiglu.so"
-SOURCES = [CSRC / "swiglu_sm100.cu", CSRC / "routed_sm100.cu"]
+SOURCES = [CSRC / "swiglu_sm100.cu", CSRC / "routed_sm100.cu", CSRC / "fp8_block_sm100.cu"]
 HEADERS = [CSRC / "ptx_sm100.cuh", CSRC / "swiglu_kernels.cuh", CSRC / "swiglu_plan.hpp", CSRC / "host_common.hpp",
-           CSRC / "routed_kernels.cuh", INCLUDE / "magi_swiglu.h"]
+           CSRC / "routed_kernels.cuh", CSRC / "fp8_block_kernels.cuh", INCLUDE / "magi_swiglu.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -122,6 +122,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.magi_swiglu_quantize_fp8_block.argtypes = [vp, vp, vp, i64, i64, i64, i32, vp]
     lib.magi_swiglu_expert_gather_fp8_block.restype = i32
     lib.magi_swiglu_expert_gather_fp8_block.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, i32, vp]
+    lib.magi_swiglu_gemm_fp8_block.restype = i32
+    lib.magi_swiglu_gemm_fp8_block.argtypes = [vp, vp, vp, vp, vp, i32, vp, i64, i64, i64, i64, i64, i32, i32, vp]
+    lib.magi_swiglu_gemm_swiglu_fp8_block.restype = i32
+    lib.magi_swiglu_gemm_swiglu_fp8_block.argtypes = [vp, vp, vp, vp, vp, i32, vp, vp, i64, i64, i64, i64, i64, i32, i32, vp]
     lib.magi_swiglu_backward_act_bf16.restype = i32
     lib.magi_swiglu_backward_act_bf16.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i32, vp]
     lib.magi_swiglu_workspace_bytes.restype = i64

@@ -1,0 +1,388 @@
+// Device code of the block-scaled fp8 products:
+//
+//   C[m, n] = sum over K blocks b of  as[m, b] * bs[n / 128, b] * ( sum over k in block b of  a[m, k] * w[n, k] )
+//
+// with e4m3 codes, one fp32 scale per row and 128 K elements of A and one per 128 x 128 block of W; and the fused SwiGLU
+// form, whose result silu(g) * u is quantised again in the same way (e4m3, one scale per row and 128 columns) without ever
+// being written in a wider type.  With `offsets`, rows [offsets[e], offsets[e+1]) of A meet expert e's W.
+//
+// The inner sums run on the tensor cores (tcgen05 kind::f8f6f4, fp32 in tensor memory); the scales are not powers of two,
+// so every K block of 128 is finished in tensor memory, read back, scaled and added to fp32 registers.  Two accumulator
+// buffers in tensor memory let the MMAs of the next block run meanwhile.
+//
+// fp8_block_stream_kernel: W's rows are the MMA's 128 rows ("M") and the tokens are its columns ("N", 16..128), so few
+// tokens cost few MMA columns and few additions, and the kernel is a stream over W.  A CTA owns 128 output columns (128
+// gate rows and 128 up rows of W in the SwiGLU form) of up to kTok rows of one expert.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "ptx_sm100.cuh"
+
+namespace magi {
+namespace fp8 {
+
+constexpr int kBlk = 128;                 // K elements (= bytes) per scale block and pipeline stage: one swizzle row
+constexpr int kRowsW = 128;               // rows of W per tile = tensor-memory lanes
+constexpr int kWTile = kRowsW * kBlk;     // bytes
+constexpr int kMaxStages = 8;
+constexpr long long kWaitLimit = 6000000000LL;  // three to four seconds of SM cycles
+constexpr float kCodeMax = 448.0f;
+constexpr float kScaleFloor = 1.17549435e-38f;  // 2^-126
+
+__device__ unsigned int g_fp8_watchdog[4];  // {role that gave up, block, stage/buffer, parity}
+
+// Bounded wait: after kWaitLimit the waiting role records itself, raises the CTA's abort flag and every role leaves.
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned role,
+                                             unsigned idx) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  unsigned spins = 0;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((++spins & 255u) == 0u) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > kWaitLimit) {
+        *abort_flag = 1;
+        if (atomicCAS(&g_fp8_watchdog[0], 0u, role) == 0u) {
+          g_fp8_watchdog[1] = blockIdx.x;
+          g_fp8_watchdog[2] = idx;
+          g_fp8_watchdog[3] = parity;
+        }
+        return false;
+      }
+    }
+  }
+}
+
+struct Args {
+  const float* a_scale;   // [R, kb] fp32, row stride ld_as
+  const float* b_scale;   // [E][halves * nb][kb]
+  const int* offsets;     // [E + 1], or null: one expert with all R rows
+  __nv_bfloat16* c;       // plain: [R, N]
+  uint8_t* codes;         // SwiGLU: [R, N]
+  float* scales;          // SwiGLU: [R, nb]
+  long long ld_as;
+  int R, N, E, kb, nb;    // nb = ceil(N / 128)
+  int splits;             // CTAs of a cluster that share a tile's K blocks
+  int stages;
+  int zero_tail;          // rows from offsets[E] on: 1 = written as zeros, 0 = left alone
+};
+
+struct Unit {  // rows [row0, row0 + rows) of expert e; e == E: rows behind the last expert's; rows == 0: nothing
+  int e, row0, rows;
+};
+
+// The unit-th group of at most kTok rows, counting every expert's groups in order (one whole warp calls this).  Offsets are
+// clamped to [0, R], so that a bad array cannot lead outside the operands.
+template <int kTok>
+__device__ __forceinline__ Unit find_unit(const Args& a, int unit) {
+  if (!a.offsets) {
+    const long long r0 = (long long)unit * kTok;
+    return r0 < a.R ? Unit{0, (int)r0, min(kTok, a.R - (int)r0)} : Unit{0, 0, 0};
+  }
+  const int lane = threadIdx.x & 31;
+  int seen = 0;
+  for (int b = 0; b <= a.E; b += 32) {
+    const int e = b + lane;
+    int lo = 0, len = 0, n = 0;
+    if (e <= a.E) {
+      lo = min(max(a.offsets[e], 0), a.R);
+      const int hi = e < a.E ? min(max(a.offsets[e + 1], lo), a.R) : a.R;
+      len = hi - lo;
+      n = (e == a.E && !a.zero_tail) ? 0 : (len + kTok - 1) / kTok;
+    }
+    int scan = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, scan, d);
+      if (lane >= d) scan += up;
+    }
+    const bool mine = n > 0 && unit >= seen + scan - n && unit < seen + scan;
+    const unsigned hit = __ballot_sync(0xffffffffu, mine);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int first = __shfl_sync(0xffffffffu, lo, src), all = __shfl_sync(0xffffffffu, len, src);
+      const int i = unit - seen - __shfl_sync(0xffffffffu, scan - n, src);
+      return Unit{b + src, first + i * kTok, min(kTok, all - i * kTok)};
+    }
+    seen += __shfl_sync(0xffffffffu, scan, 31);
+  }
+  return Unit{0, 0, 0};
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  return g * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * g)) * u;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {  // maximum of non-negative values and NaN, NaN wins
+  unsigned b = __float_as_uint(v);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+  return __uint_as_float(b);
+}
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void epilogue_sync(int threads) {  // named barrier of the epilogue warps
+  asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+}
+
+constexpr int kStreamThreads = 192;  // warps 0-3 epilogue (one tensor-memory lane quarter each), 4 TMA producer, 5 MMA issuer
+
+// Two CTAs share an SM where the sums of a thread leave the registers for it.
+template <int kHalves, int kTok>
+__global__ void __launch_bounds__(kStreamThreads, kHalves * kTok <= 64 ? 2 : 1)
+fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const Args a) {
+  constexpr int kATile = kTok * kBlk;
+  constexpr int kStage = kHalves * kWTile + kATile;
+  constexpr int kAccCols = kHalves * kTok;
+  constexpr int kTmem = 2 * kAccCols < 32 ? 32 : 2 * kAccCols;
+  constexpr int kPiece = kTok < 32 ? kTok : 32;  // columns per tensor-memory load
+  constexpr int kScaleRow = kTok + 4;            // token scales of one K block, then the weights' scales of the halves
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(16) float ring[2][4][kScaleRow];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ Unit unit_slot;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 2 + b); };
+  const int split = a.splits > 1 ? (int)cluster_ctarank() : 0;
+  const int n0 = (int)(blockIdx.x / a.splits) * kRowsW;
+
+  if (warp == 4) {
+    const Unit u = find_unit<kTok>(a, blockIdx.y);
+    if (lane == 0) unit_slot = u;
+  }
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 4);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc<1>(smem_u32(&tmem_slot), kTmem);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const Unit u = unit_slot;
+  const bool live = u.rows > 0 && u.e < a.E;  // the same for every CTA of a cluster
+  const int kb0 = (int)((long long)a.kb * split / a.splits), kb1 = (int)((long long)a.kb * (split + 1) / a.splits);
+
+  if (live && warp == 4 && lane == 0) {
+    // ------------------------------------------------------------ TMA producer
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_a);
+    const uint64_t keep = l2_policy_evict_last(), once = l2_policy_evict_first();
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!wait_bounded(empty_bar(stage), phase ^ 1u, &abort_flag, 1u, stage)) break;
+      mbar_arrive_expect_tx(full_bar(stage), kStage);
+      const uint32_t dst = tiles + stage * kStage;
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+        tma_load_3d_hint(dst + h * kWTile, &tm_w, full_bar(stage), kb * kBlk, n0, u.e * kHalves + h, once);
+      tma_load_2d_hint(dst + kHalves * kWTile, &tm_a, full_bar(stage), kb * kBlk, u.row0, keep);
+      if (++stage == a.stages) stage = 0, phase ^= 1u;
+    }
+  } else if (live && warp == 5 && lane == 0) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t idesc = umma_idesc_e4m3(kRowsW, kTok);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int buf = (kb - kb0) & 1;
+      const uint32_t buf_phase = ((kb - kb0) >> 1) & 1;
+      if (!wait_bounded(acc_empty(buf), buf_phase ^ 1u, &abort_flag, 2u, 16 + buf)) break;
+      if (!wait_bounded(full_bar(stage), phase, &abort_flag, 2u, stage)) break;
+      tc_fence_after_sync();
+      const uint32_t src = tiles + stage * kStage;
+      const uint64_t tok = umma_desc_k_sw128(src + kHalves * kWTile);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const uint64_t w = umma_desc_k_sw128(src + h * kWTile);
+#pragma unroll
+        for (int i = 0; i < kBlk / 32; ++i)
+          umma_fp8<1>(tmem + buf * kAccCols + h * kTok, w + 2 * i, tok + 2 * i, idesc, i > 0);
+      }
+      umma_commit<1>(empty_bar(stage));
+      umma_commit<1>(acc_full(buf));
+      if (++stage == a.stages) stage = 0, phase ^= 1u;
+    }
+  } else if (live && warp < 4) {
+    // ------------------------------------------------------------ scale and add (one row of W per thread)
+    float acc[kHalves][kTok];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int c = 0; c < kTok; ++c) acc[h][c] = 0.0f;
+    // Scales travel four K blocks at a time: a prefetch into registers, then into one half of a shared ring.
+    constexpr int kLoads = (4 * kTok + 127) / 128;
+    float next[kLoads], next_w = 0.0f;
+    const float* ws = a.b_scale + ((long long)u.e * kHalves * a.nb + n0 / kBlk) * a.kb;
+    auto fetch = [&](int kb) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int idx = threadIdx.x + 128 * i, c = idx >> 2, b = kb + (idx & 3);
+        next[i] = (c < u.rows && c < kTok && b < kb1) ? __ldg(a.a_scale + (long long)(u.row0 + c) * a.ld_as + b) : 0.0f;
+      }
+      if (threadIdx.x < 4 * kHalves) {
+        const int b = kb + (threadIdx.x & 3), h = threadIdx.x >> 2;
+        next_w = b < kb1 ? __ldg(ws + (long long)h * a.nb * a.kb + b) : 0.0f;
+      }
+    };
+    fetch(kb0);
+    const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int i = kb - kb0, half = (i >> 2) & 1, buf = i & 1;
+      if ((i & 3) == 0) {
+        // everyone is past the previous four blocks, so the other half of the ring is free
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+          const int idx = threadIdx.x + 128 * q;
+          if ((idx >> 2) < kTok) ring[half][idx & 3][idx >> 2] = next[q];
+        }
+        if (threadIdx.x < 4 * kHalves) ring[half][threadIdx.x & 3][kTok + (threadIdx.x >> 2)] = next_w;
+        epilogue_sync(128);
+        fetch(kb + 4);
+      }
+      const float* sc = ring[half][i & 3];
+      // a wait that gave up skips the work but not the barrier above, which the other warps are counting on
+      ok = __all_sync(0xffffffffu, ok && wait_bounded(acc_full(buf), (i >> 1) & 1, &abort_flag, 3u, buf));
+      if (!ok) continue;
+      tc_fence_after_sync();
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const float w = sc[kTok + h];
+#pragma unroll
+        for (int c0 = 0; c0 < kTok; c0 += kPiece) {
+          uint32_t p[32];
+          if constexpr (kPiece == 32)
+            tmem_ld_x32(lane_base + buf * kAccCols + h * kTok + c0, p);
+          else
+            tmem_ld_x16_into32(lane_base + buf * kAccCols + h * kTok + c0, p);
+          tmem_ld_wait();
+          tmem_regs_ready(p);
+#pragma unroll
+          for (int c = 0; c < kPiece; c += 4) {
+            const float4 t = *reinterpret_cast<const float4*>(sc + c0 + c);
+            acc[h][c0 + c] = fmaf(__uint_as_float(p[c]), w * t.x, acc[h][c0 + c]);
+            acc[h][c0 + c + 1] = fmaf(__uint_as_float(p[c + 1]), w * t.y, acc[h][c0 + c + 1]);
+            acc[h][c0 + c + 2] = fmaf(__uint_as_float(p[c + 2]), w * t.z, acc[h][c0 + c + 2]);
+            acc[h][c0 + c + 3] = fmaf(__uint_as_float(p[c + 3]), w * t.w, acc[h][c0 + c + 3]);
+          }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_relaxed(acc_empty(buf));
+    }
+    // Every MMA of this CTA is complete, so the stages are free: the sums go there as [token][half][128], which is
+    // conflict-free here and gives the writer below a token's 128 columns in a row.
+    const uint32_t mine = tiles + (warp * 32 + lane) * 4;
+#pragma unroll
+    for (int c = 0; c < kTok; ++c)
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) st_shared_f32(mine + (c * kHalves + h) * 512, acc[h][c]);
+  }
+  __syncwarp();
+  if (live) {
+    if (a.splits > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+  }
+
+  // ------------------------------------------------------------ output: one warp per token, four columns per lane
+  if (warp < 4 && u.rows > 0) {
+    const int n = n0 + 4 * lane;
+    for (int c = split + a.splits * warp; c < u.rows; c += a.splits * 4) {
+      float4 v[kHalves];
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        v[h] = make_float4(0, 0, 0, 0);
+        if (!live) continue;
+        const uint32_t at = tiles + (c * kHalves + h) * 512 + lane * 16;
+        if (a.splits == 1) {
+          v[h] = ld_shared_f4(at);
+        } else {
+          for (int z = 0; z < a.splits; ++z) {  // in split order: the same sum every time
+            const float4 q = ld_cluster_f4(map_to_cta(at, z));
+            v[h].x += q.x, v[h].y += q.y, v[h].z += q.z, v[h].w += q.w;
+          }
+        }
+      }
+      const long long row = u.row0 + c;
+      if constexpr (kHalves == 1) {
+        if (n < a.N) {
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0].x, v[0].y), hi = __floats2bfloat162_rn(v[0].z, v[0].w);
+          uint2 o;
+          o.x = *reinterpret_cast<const uint32_t*>(&lo);
+          o.y = *reinterpret_cast<const uint32_t*>(&hi);
+          *reinterpret_cast<uint2*>(a.c + row * a.N + n) = o;
+        }
+      } else {
+        // columns beyond N hold zeros (W's rows there are zero-filled), which no maximum notices
+        const float y0 = silu_mul(v[0].x, v[1].x), y1 = silu_mul(v[0].y, v[1].y), y2 = silu_mul(v[0].z, v[1].z),
+                    y3 = silu_mul(v[0].w, v[1].w);
+        unsigned top = max(max(__float_as_uint(fabsf(y0)), __float_as_uint(fabsf(y1))),
+                           max(__float_as_uint(fabsf(y2)), __float_as_uint(fabsf(y3))));
+        float s = __fdiv_rn(warp_max_nan(__uint_as_float(top)), kCodeMax);
+        s = s < kScaleFloor ? kScaleFloor : s;
+        // one reciprocal per row: a product with it is off by at most 2^-23 before the rounding to 4 bits
+        const float r = __frcp_rn(s);
+        if (n < a.N) *reinterpret_cast<uint32_t*>(a.codes + row * a.N + n) = pack4(y0 * r, y1 * r, y2 * r, y3 * r);
+        if (lane == 0) a.scales[row * a.nb + n0 / kBlk] = s;
+      }
+    }
+  }
+
+  // ------------------------------------------------------------ teardown (also the abort path)
+  __syncwarp();
+  if (*reinterpret_cast<volatile int*>(&abort_flag)) {
+    const long long t0 = clock64();  // copies and MMAs in flight land before tensor memory is freed
+    while (clock64() - t0 < 4000000LL) {
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (live && a.splits > 1) cluster_sync_all();  // nobody leaves while its sums may still be read
+  if (warp == 5) tmem_dealloc<1>(tmem, kTmem);
+}
+
+}  // namespace fp8
+}  // namespace magi

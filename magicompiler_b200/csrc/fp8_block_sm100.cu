@@ -1,0 +1,186 @@
+// C ABI of the block-scaled fp8 products (include/magi_swiglu.h): argument checks, tile choice, tensor maps, launches.
+// Device code lives in fp8_block_kernels.cuh.
+#include <cstring>
+
+#include "fp8_block_kernels.cuh"
+#include "host_common.hpp"
+
+namespace magi {
+
+// Read and clear this translation unit's watchdog word (the device is current and idle).
+cudaError_t fp8_block_watchdog(unsigned int out[4]) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, fp8::g_fp8_watchdog, 4 * sizeof(unsigned int));
+  if (e == cudaSuccess && out[0] != 0) {
+    const unsigned int zero[4] = {0, 0, 0, 0};
+    e = cudaMemcpyToSymbol(fp8::g_fp8_watchdog, zero, sizeof(zero));
+  }
+  return e;
+}
+
+namespace fp8 {
+
+static int encode_bytes_map(const void* ptr, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                            const cuuint32_t* box, CUtensorMap* tm, const char* what) {
+  EncodeTiledFn enc = tensor_map_encoder();
+  if (!enc) return fail(MAGI_SWIGLU_ERR_DRIVER, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, const_cast<void*>(ptr), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MAGI_SWIGLU_ERR_DRIVER, "tensor map for %s rejected by the driver (CUresult %d)", what, (int)r);
+  return 0;
+}
+
+struct Problem {
+  const void* a;
+  const void* b;
+  long long lda;
+  int64_t M, N, K;
+  int halves;
+  Args args;
+};
+
+template <int kHalves, int kTok>
+static int launch_stream(const Problem& p, int sm_count, cudaStream_t stream) {
+  constexpr int kStage = kHalves * kWTile + kTok * kBlk;
+  constexpr int kBudget = kHalves * kTok <= 64 ? 108 * 1024 : 216 * 1024;  // two CTAs an SM, or one
+  constexpr int kFit = (kBudget - 1024) / kStage;
+  constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+  static_assert(kStages >= 2 && kStages * kStage >= kTok * kHalves * 512, "stages hold the sums of a tile");
+  const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.args.E * kHalves};
+  const cuuint64_t wst[2] = {(cuuint64_t)p.K, (cuuint64_t)p.N * (cuuint64_t)p.K};
+  const cuuint32_t wb[3] = {kBlk, kRowsW, 1};
+  const cuuint64_t ad[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M};
+  const cuuint64_t ast[1] = {(cuuint64_t)p.lda};
+  const cuuint32_t ab[2] = {kBlk, kTok};
+  CUtensorMap tm_w, tm_a;
+  if (int rc = encode_bytes_map(p.b, 3, wd, wst, wb, &tm_w, "B")) return rc;
+  if (int rc = encode_bytes_map(p.a, 2, ad, ast, ab, &tm_a, "A")) return rc;
+  const int64_t n_tiles = (p.N + kRowsW - 1) / kRowsW;
+  // every expert adds at most one partial group of rows
+  const int64_t groups = p.args.offsets ? p.M / kTok + (p.M < p.args.E + 1 ? p.M : p.args.E + 1) : (p.M + kTok - 1) / kTok;
+  if (groups > 65535 || n_tiles > 0x7fffffffLL / 8)
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld rows are too many for one launch", (long long)p.M);
+  Args args = p.args;
+  args.splits = 1;
+  args.stages = kStages;
+  const int smem = kStages * kStage + 1024;
+  cudaError_t e = cudaFuncSetAttribute(fp8_block_stream_kernel<kHalves, kTok>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)args.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(n_tiles * args.splits), (unsigned)groups);
+  cfg.blockDim = dim3(kStreamThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, fp8_block_stream_kernel<kHalves, kTok>, tm_w, tm_a, args);
+  return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_stream_kernel");
+}
+
+static int run(const Problem& p, int device, void* cuda_stream) {
+  const DeviceInfo* di = nullptr;
+  if (int rc = require_b200(device, &di)) return rc;
+  DeviceGuard guard;
+  cudaError_t e = guard.set(device);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  // Tokens per tile: enough for an expert's average share of the rows, so that W is usually streamed once.
+  const int64_t share = p.args.offsets ? (p.M + p.args.E - 1) / p.args.E : p.M;
+  if (p.halves == 1) {
+    if (share <= 16) return launch_stream<1, 16>(p, di->sm_count, stream);
+    if (share <= 32) return launch_stream<1, 32>(p, di->sm_count, stream);
+    if (share <= 64) return launch_stream<1, 64>(p, di->sm_count, stream);
+    return launch_stream<1, 128>(p, di->sm_count, stream);
+  }
+  if (share <= 16) return launch_stream<2, 16>(p, di->sm_count, stream);
+  if (share <= 32) return launch_stream<2, 32>(p, di->sm_count, stream);
+  return launch_stream<2, 64>(p, di->sm_count, stream);
+}
+
+static int check(const void* a, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,
+                 int num_experts, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ld_scale, int n_multiple) {
+  if (M < 0 || N < 1 || K < 1 || M > 0x3fffffffLL || N > 0x3fffffffLL || K > 0x3fffffffLL)
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld, N=%lld, K=%lld out of range", (long long)M, (long long)N, (long long)K);
+  if (N % n_multiple || K % 16)
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "N=%lld must be a multiple of %d and K=%lld of 16", (long long)N, n_multiple, (long long)K);
+  if (num_experts < 1 || num_experts > 1024 || (!offsets && num_experts != 1))
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "num_experts=%d out of range [1, 1024], or more than one without offsets", num_experts);
+  if (lda < K || ld_scale < (K + 127) / 128)
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "row strides too small: lda=%lld (K=%lld), ld_scale=%lld", (long long)lda, (long long)K, (long long)ld_scale);
+  if (M == 0) return 0;
+  if (!a || !a_scale || !b || !b_scale) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  if (lda % 16 || (((uintptr_t)a | (uintptr_t)b) & 15u))
+    return fail(MAGI_SWIGLU_ERR_ALIGN, "a and b must be 16-byte aligned, and lda a multiple of 16");
+  if ((((uintptr_t)a_scale | (uintptr_t)b_scale | (uintptr_t)offsets) & 3u))
+    return fail(MAGI_SWIGLU_ERR_ALIGN, "scales and offsets must be 4-byte aligned");
+  return 0;
+}
+
+static Problem problem(const void* a, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,
+                       int num_experts, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ld_scale, int zero_tail,
+                       int halves) {
+  Problem p;
+  memset(&p, 0, sizeof(p));
+  p.a = a;
+  p.b = b;
+  p.lda = lda;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.halves = halves;
+  p.args.a_scale = a_scale;
+  p.args.b_scale = b_scale;
+  p.args.offsets = offsets;
+  p.args.ld_as = ld_scale;
+  p.args.R = (int)M;
+  p.args.N = (int)N;
+  p.args.E = num_experts;
+  p.args.kb = (int)((K + kBlk - 1) / kBlk);
+  p.args.nb = (int)((N + kBlk - 1) / kBlk);
+  p.args.zero_tail = zero_tail;
+  return p;
+}
+
+}  // namespace fp8
+}  // namespace magi
+
+using namespace magi;
+
+extern "C" {
+
+int magi_swiglu_gemm_fp8_block(const void* a, const float* a_scale, const void* b, const float* b_scale,
+                               const int32_t* offsets, int num_experts, void* c, int64_t M, int64_t N, int64_t K,
+                               int64_t lda, int64_t ld_scale, int zero_tail, int device, void* cuda_stream) {
+  g_err[0] = 0;
+  if (int rc = fp8::check(a, a_scale, b, b_scale, offsets, num_experts, M, N, K, lda, ld_scale, 8)) return rc;
+  if (M == 0) return 0;
+  if (!c) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  if ((uintptr_t)c & 15u) return fail(MAGI_SWIGLU_ERR_ALIGN, "c must be 16-byte aligned");
+  fp8::Problem p = fp8::problem(a, a_scale, b, b_scale, offsets, num_experts, M, N, K, lda, ld_scale, zero_tail, 1);
+  p.args.c = static_cast<__nv_bfloat16*>(c);
+  return fp8::run(p, device, cuda_stream);
+}
+
+int magi_swiglu_gemm_swiglu_fp8_block(const void* a, const float* a_scale, const void* w_gate_up, const float* w_scale,
+                                      const int32_t* offsets, int num_experts, void* codes, float* scales, int64_t M,
+                                      int64_t N, int64_t K, int64_t lda, int64_t ld_scale, int zero_tail, int device,
+                                      void* cuda_stream) {
+  g_err[0] = 0;
+  if (int rc = fp8::check(a, a_scale, w_gate_up, w_scale, offsets, num_experts, M, N, K, lda, ld_scale, 16)) return rc;
+  if (M == 0) return 0;
+  if (!codes || !scales) return fail(MAGI_SWIGLU_ERR_NULL, "null pointer argument");
+  if (((uintptr_t)codes & 15u) || ((uintptr_t)scales & 3u))
+    return fail(MAGI_SWIGLU_ERR_ALIGN, "codes must be 16-byte aligned and scales 4-byte aligned");
+  fp8::Problem p = fp8::problem(a, a_scale, w_gate_up, w_scale, offsets, num_experts, M, N, K, lda, ld_scale, zero_tail, 2);
+  p.args.codes = static_cast<uint8_t*>(codes);
+  p.args.scales = scales;
+  return fp8::run(p, device, cuda_stream);
+}
+
+}  // extern "C"

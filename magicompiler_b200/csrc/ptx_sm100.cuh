@@ -296,6 +296,29 @@ __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// The same for 8-bit floating-point operands (kind::f8f6f4): 32 K elements (32 bytes) per instruction.
+template <int kCtas>
+__device__ __forceinline__ void umma_fp8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  if constexpr (kCtas == 1)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // The mbarrier gets one arrival when every tcgen05 operation issued so far by this thread is done.
 // kCtas = 2: the barrier at the same shared-memory offset in BOTH CTAs of the pair gets the arrival.
 template <int kCtas>
@@ -393,6 +416,12 @@ __host__ __device__ __forceinline__ uint32_t umma_idesc_bf16(uint32_t m, uint32_
          | (1u << 7)      // A format bf16
          | (1u << 10)     // B format bf16
          | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// Instruction descriptor: e4m3 x e4m3 -> fp32, dense, MMA shape m x n (x32), both operand tiles K-major.
+__host__ __device__ __forceinline__ uint32_t umma_idesc_e4m3(uint32_t m, uint32_t n) {
+  return (1u << 4)  // D format fp32; A and B format fields 0 = e4m3
+         | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
 }  // namespace magi

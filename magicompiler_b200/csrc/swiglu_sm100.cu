@@ -9,6 +9,8 @@
 
 namespace magi {
 
+cudaError_t fp8_block_watchdog(unsigned int out[4]);  // fp8_block_sm100.cu
+
 struct ScatterSet {  // what magi_swiglu_scatter_setup last wrote into g_scatter_maps[set] of a device
   int world = 0;
   int64_t rows = 0, n = 0;
@@ -739,12 +741,16 @@ int magi_swiglu_device_status(int device, int32_t out[4]) {
   unsigned int host[4] = {0, 0, 0, 0};
   e = cudaMemcpyFromSymbol(host, magi::g_watchdog, sizeof(host));
   if (e != cudaSuccess) return magi::fail_cuda(e, "cudaMemcpyFromSymbol(g_watchdog)");
-  for (int i = 0; i < 4; ++i) out[i] = (int32_t)host[i];
   if (host[0] != 0) {
     const unsigned int zero[4] = {0, 0, 0, 0};
     e = cudaMemcpyToSymbol(magi::g_watchdog, zero, sizeof(zero));
     if (e != cudaSuccess) return magi::fail_cuda(e, "cudaMemcpyToSymbol(g_watchdog)");
   }
+  unsigned int fp8[4] = {0, 0, 0, 0};  // the block-scaled products keep a word of their own
+  e = magi::fp8_block_watchdog(fp8);
+  if (e != cudaSuccess) return magi::fail_cuda(e, "reading the watchdog of the fp8 products");
+  if (host[0] == 0) memcpy(host, fp8, sizeof(host));
+  for (int i = 0; i < 4; ++i) out[i] = (int32_t)host[i];
   return 0;
 }
 

@@ -1,0 +1,118 @@
+"""Block-scaled fp8 products without a GPU: refusals, fake implementations, the load-time weight quantisers and the host
+checks of the C entry points."""
+import ctypes
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import magicompiler_b200 as mb
+from magicompiler_b200 import _loader
+
+F8, F32, I32 = torch.float8_e4m3fn, torch.float32, torch.int32
+
+
+def operands(m=4, n=256, k=272, experts=0, halves=1):
+    lead = (experts,) if experts else ()
+    nb, kb = -(-n // 128), -(-k // 128)
+    t = dict(a=torch.zeros(m, k).to(F8), a_scale=torch.zeros(m, kb), b=torch.zeros(*lead, halves * n, k).to(F8),
+             b_scale=torch.zeros(*lead, halves * nb, kb))
+    if experts:
+        t["offsets"] = torch.zeros(experts + 1, dtype=I32)
+    return t
+
+
+FORMS = [(mb.gemm_fp8_block, 1), (mb.gemm_fp8_block_out, 1), (mb.gemm_swiglu_fp8_block, 2), (mb.gemm_swiglu_fp8_block_out, 2)]
+
+
+@pytest.mark.parametrize("form,halves", FORMS)
+def test_refusals(form, halves):
+    def call(error, match, experts=0, **changes):
+        t = operands(experts=experts, halves=halves)
+        t.update(changes)
+        with pytest.raises(error, match=match):
+            form(t["a"], t["a_scale"], t["b"], t["b_scale"], t.get("offsets"))
+
+    t = operands(halves=halves)
+    call(TypeError, "CUDA tensors only")
+    call(TypeError, "CUDA tensors only", experts=3)
+    call(TypeError, "a must be", a=t["a"].to(torch.float8_e5m2))
+    call(TypeError, "a must be", a=t["a"].to(torch.bfloat16))
+    call(TypeError, "b must be", b=t["b"].view(torch.uint8))
+    call(TypeError, "a_scale must be", a_scale=t["a_scale"].double())
+    call(TypeError, "b_scale must be", b_scale=t["b_scale"].to(torch.bfloat16))
+    call(TypeError, "offsets must be", experts=3, offsets=torch.zeros(4, dtype=torch.int64))
+    call(ValueError, "2-D", a=t["a"][None])
+    call(ValueError, "without offsets", b=t["b"][None])
+    call(ValueError, "with offsets", experts=3, b=t["b"])
+    call(ValueError, "offsets must be a contiguous", experts=3, offsets=torch.zeros(5, dtype=I32))
+    call(ValueError, "inner dimensions", a=torch.zeros(4, 256).to(F8))
+    call(ValueError, "a_scale must be", a_scale=torch.zeros(4, 2))
+    call(ValueError, "scales must be", b_scale=torch.zeros(1, 3))
+    call(ValueError, "must be contiguous", b=torch.zeros(halves * 256, 288).to(F8)[:, :272])
+    call(ValueError, "multiple of", **{k: v for k, v in operands(n=256, k=264, halves=halves).items()})
+    call(ValueError, "multiple of", **{k: v for k, v in operands(n=252, k=272, halves=halves).items()})
+    call(ValueError, "multiple of", a=torch.zeros(4, 0).to(F8), b=torch.zeros(halves * 256, 0).to(F8))
+
+
+def test_an_odd_number_of_packed_rows_is_refused():
+    t = operands(n=256, halves=1)
+    with pytest.raises(ValueError, match="N gate rows"):
+        mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"][:255], t["b_scale"])
+    with pytest.raises(ValueError, match="N gate rows"):
+        mb.quantize_fp8_gate_up(torch.zeros(255, 64))
+    with pytest.raises(ValueError, match="a weight is"):
+        mb.quantize_fp8_weight(torch.zeros(64))
+
+
+def test_fake_implementations():
+    with FakeTensorMode():
+        for experts in (0, 3):
+            t = {k: torch.empty(v.shape, dtype=v.dtype, device="cuda") for k, v in operands(experts=experts).items()}
+            c = torch.ops.magi_swiglu.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t.get("offsets"))
+            assert tuple(c.shape) == (4, 256) and c.dtype == torch.bfloat16
+            t = {k: torch.empty(v.shape, dtype=v.dtype, device="cuda") for k, v in operands(n=272, experts=experts, halves=2).items()}
+            q, s = torch.ops.magi_swiglu.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t.get("offsets"))
+            assert tuple(q.shape) == (4, 272) and q.dtype == F8 and tuple(s.shape) == (4, 3) and s.dtype == F32
+
+
+@pytest.mark.parametrize("n,k", [(128, 128), (130, 144), (1, 16), (300, 500)])
+def test_weight_quantiser(n, k):
+    """Each code times its scale is within half an e4m3 step of the weight: 2^-4 of its size, or half the smallest code
+    (2^-10) of the scale."""
+    w = torch.randn(n, k, generator=torch.Generator().manual_seed(n))
+    codes, scales = mb.quantize_fp8_weight(w)
+    assert codes.dtype == F8 and tuple(scales.shape) == (-(-n // 128), -(-k // 128))
+    full = scales.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+    err = (codes.float() * full - w).abs()
+    assert (err <= w.abs() * 2.0 ** -4 * (1 + 1e-6) + full * 2.0 ** -10).all()
+    two = torch.stack([w, -2 * w])
+    c2, s2 = mb.quantize_fp8_weight(two)
+    assert torch.equal(c2[0].float(), codes.float()) and torch.equal(s2[1], 2 * scales)
+
+
+def test_gate_up_halves_are_blocked_from_their_own_first_row():
+    w = torch.randn(2 * 200, 136, generator=torch.Generator().manual_seed(1))
+    codes, scales = mb.quantize_fp8_gate_up(w)
+    g, gs = mb.quantize_fp8_weight(w[:200])
+    u, us = mb.quantize_fp8_weight(w[200:])
+    assert torch.equal(codes.float(), torch.cat([g.float(), u.float()])) and torch.equal(scales, torch.cat([gs, us]))
+    assert tuple(mb.quantize_fp8_gate_up(torch.zeros(3, 400, 136))[1].shape) == (3, 4, 2)
+    assert (mb.quantize_fp8_weight(torch.zeros(8, 16))[1] == 2.0 ** -126).all()
+
+
+def test_c_entry_points_reject_on_the_host():
+    lib = mb.load_library()
+    buf = (ctypes.c_char * 4096)()
+    p = ctypes.addressof(buf)
+    p += -p % 16
+    base = dict(a=p, asc=p, b=p, bsc=p, off=None, e=1, c=p, M=4, N=16, K=32, lda=32, lds=1, zt=1, dev=0, st=None)
+    gemm = lambda **o: lib.magi_swiglu_gemm_fp8_block(*{**base, **o}.values())  # noqa: E731
+    assert gemm(M=-1) == -2 and gemm(N=12) == -2 and gemm(K=24) == -2 and gemm(e=2) == -2 and gemm(e=0) == -2
+    assert gemm(off=p, e=1025) == -2 and gemm(lda=16) == -2 and gemm(lds=0) == -2
+    assert gemm(lda=40) == -3 and gemm(a=p + 8) == -3 and gemm(c=p + 2) == -3 and gemm(bsc=p + 2) == -3
+    assert gemm(b=None) == -1 and gemm(c=None) == -1 and gemm(M=0, a=None) == 0
+    assert gemm(dev=1000) == -5 and "not available" in _loader.last_error()
+    base = dict(a=p, asc=p, b=p, bsc=p, off=None, e=1, c=p, s=p, M=4, N=16, K=32, lda=32, lds=1, zt=1, dev=0, st=None)
+    fused = lambda **o: lib.magi_swiglu_gemm_swiglu_fp8_block(*{**base, **o}.values())  # noqa: E731
+    assert fused(N=8) == -2 and fused(s=None) == -1 and fused(c=p + 4) == -3 and fused(M=0) == 0

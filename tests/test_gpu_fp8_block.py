@@ -1,0 +1,282 @@
+"""Block-scaled fp8 products against the formula in 64 bits.
+
+Tolerance of a sum.  The products of e4m3 codes are exact in fp32.  Let A = sum |terms|, scaled.  The tensor cores add the
+128 products of a block in fp32 steps that may truncate (one unit, 2^-23, a step; at most 128 steps), the two scales'
+product and the multiply-add round once each (2^-24), and the additions over the K blocks at most ceil(K/128) + 8 times:
+|error| <= A * (128 + ceil(K/128) + 10) * 2^-23.  A bf16 result adds half a bf16 step of its own value, 2^-8.
+SwiGLU: |d(silu(g) u)| <= 1.1 |u| dg + |silu(g)| du (|silu'| < 1.1) plus 2^-20 of the value for the exponential, the
+reciprocal and the products.  A scale is 1/448 of the largest of 128 such values, a code is within half an e4m3 step
+(2^-4 of the value, or 2^-10 of the scale below the smallest normal code) of value / scale."""
+import pytest
+import torch
+
+import magicompiler_b200 as mb
+
+pytestmark = pytest.mark.gpu
+F8, BF = torch.float8_e4m3fn, torch.bfloat16
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def codes_of(shape, seed, spread=1.0):
+    return (spread * torch.randn(*shape, generator=gen(seed), device="cuda")).clamp(-448, 448).to(F8)
+
+
+def scales_of(shape, seed):
+    return torch.exp2(4 * torch.rand(*shape, generator=gen(seed), device="cuda") - 6)
+
+
+def wide(codes, scales, rows_per_scale):
+    s = scales.double()
+    s = s.repeat_interleave(rows_per_scale, -2)[..., :codes.shape[-2], :] if rows_per_scale > 1 else s
+    return codes.double() * s.repeat_interleave(128, -1)[..., :codes.shape[-1]]
+
+
+def case(M, N, K, E=0, halves=1, seed=0, counts=None):
+    lead = (E,) if E else ()
+    kb, nb = -(-K // 128), -(-N // 128)
+    t = dict(a=codes_of((M, K), seed, 2.0), a_scale=scales_of((M, kb), seed + 1))
+    t["b"], t["b_scale"] = codes_of((*lead, halves * N, K), seed + 2), scales_of((*lead, halves * nb, kb), seed + 3)
+    t["offsets"] = None
+    if E:
+        t["offsets"] = torch.tensor([0] + list(torch.tensor(counts).cumsum(0)), dtype=torch.int32, device="cuda")
+    return t
+
+
+def sums(t, halves=1):
+    """(sum, sum of magnitudes) [M, halves * N] in 64 bits; rows behind the last expert are zero."""
+    a = wide(t["a"], t["a_scale"], 1)
+    outs = []
+    for x, mag in ((a, False), (a.abs(), True)):
+        def product(rows, b, bs):
+            n, nb = b.shape[0] // halves, bs.shape[0] // halves
+            w = torch.cat([wide(b[h * n:(h + 1) * n], bs[h * nb:(h + 1) * nb], 128) for h in range(halves)])
+            return rows @ (w.abs() if mag else w).t()
+        if t["offsets"] is None:
+            outs.append(product(x, t["b"], t["b_scale"]))
+            continue
+        out = torch.zeros(a.shape[0], t["b"].shape[1], dtype=torch.float64, device="cuda")
+        off = t["offsets"].tolist()
+        for e in range(len(off) - 1):
+            out[off[e]:off[e + 1]] = product(x[off[e]:off[e + 1]], t["b"][e], t["b_scale"][e])
+        outs.append(out)
+    return outs
+
+
+def slack(mag, K):
+    return mag * (128 + -(-K // 128) + 10) * 2.0 ** -23
+
+
+def check_plain(t, got):
+    K = t["a"].shape[1]
+    want, mag = sums(t)
+    lim = want.abs() * 2.0 ** -8 + slack(mag, K) * (1 + 2.0 ** -8) + 2.0 ** -133
+    err = (got.double() - want).abs()
+    assert got.dtype == BF and got.shape == want.shape
+    assert (err <= lim).all(), (err - lim).max().item()
+
+
+def check_fused(t, codes, scales):
+    K, N = t["a"].shape[1], codes.shape[1]
+    h, mag = sums(t, 2)
+    g, u, dg, du = h[:, :N], h[:, N:], slack(mag[:, :N], K), slack(mag[:, N:], K)
+    silu = g * torch.sigmoid(g)
+    y = silu * u
+    dy = 1.1 * (u.abs() + du) * dg + silu.abs() * du + y.abs() * 2.0 ** -20
+    nb = -(-N // 128)
+    pad = lambda v: torch.nn.functional.pad(v, (0, nb * 128 - N)).view(-1, nb, 128)  # noqa: E731
+    top, slop = pad(y.abs()).amax(2), pad(dy).amax(2)
+    floor = torch.full_like(top, 2.0 ** -126)
+    s = scales.double()
+    assert codes.dtype == F8 and scales.dtype == torch.float32 and tuple(scales.shape) == tuple(top.shape)
+    assert (s <= torch.maximum((top + slop) / 448, floor) * (1 + 2.0 ** -23)).all()
+    assert (s >= torch.maximum((top - slop) / 448, floor) * (1 - 2.0 ** -23)).all()
+    full = s.repeat_interleave(128, 1)[:, :N]
+    err = (codes.double() * full - y).abs()
+    lim = (y.abs() + dy) * 2.0 ** -4 + full * 2.0 ** -10 + dy * 1.001 + y.abs() * 2.0 ** -21
+    assert (err <= lim).all(), (err - lim).max().item()
+
+
+DENSE = [(1, 8, 16), (1, 128, 128), (1, 264, 144), (3, 136, 400), (16, 256, 512), (17, 384, 256), (31, 1000, 1040), (33, 128, 2048),
+         (64, 520, 384), (65, 256, 640), (127, 136, 272), (128, 256, 256), (129, 264, 1152), (200, 2048, 512), (257, 776, 912),
+         (300, 256, 4096), (513, 512, 384), (1000, 392, 1296), (2049, 1024, 256), (5, 4096, 8192)]
+
+
+@pytest.mark.parametrize("M,N,K", DENSE)
+def test_dense(M, N, K):
+    t = case(M, N, K, seed=M + N)
+    check_plain(t, mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"]))
+
+
+@pytest.mark.parametrize("M,N,K", [(m, -(-n // 16) * 16, k) for m, n, k in DENSE])
+def test_dense_swiglu(M, N, K):
+    t = case(M, N, K, halves=2, seed=M + N)
+    check_fused(t, *mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"]))
+
+
+GROUPED = [(1, [1], 0), (2, [0, 1], 0), (8, [0, 3, 0, 1, 17, 0, 2, 0], 5), (4, [130, 1, 64, 33], 0), (3, [0, 0, 0], 40),
+           (2, [300, 257], 7), (5, [256, 512, 1, 255, 600], 300), (40, [i % 7 for i in range(40)], 1), (1, [700], 20),
+           (70, [0] * 69 + [20], 0), (64, [9] * 64, 70)]
+
+
+@pytest.mark.parametrize("E,counts,tail", GROUPED)
+@pytest.mark.parametrize("N,K", [(136, 272), (256, 512)])
+def test_experts(E, counts, tail, N, K):
+    t = case(sum(counts) + tail, N, K, E=E, counts=counts, seed=E)
+    got = mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    check_plain(t, got)
+    assert (got[sum(counts):] == 0).all()
+
+
+@pytest.mark.parametrize("E,counts,tail", GROUPED)
+@pytest.mark.parametrize("N,K", [(144, 272), (256, 512)])
+def test_experts_swiglu(E, counts, tail, N, K):
+    t = case(sum(counts) + tail, N, K, E=E, counts=counts, halves=2, seed=E)
+    codes, scales = mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    check_fused(t, codes, scales)
+    assert (codes[sum(counts):].float() == 0).all() and (scales[sum(counts):] == 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("M,E,counts", [(20, 3, [4, 0, 7]), (700, 3, [300, 0, 257])])
+def test_rows_behind_the_last_expert_stay_with_out(M, E, counts):
+    n = sum(counts)
+    t = case(M, 256, 272, E=E, counts=counts)
+    out = torch.full((M, 256), 7.0, dtype=BF, device="cuda")
+    assert mb.gemm_fp8_block_out(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"], out=out) is out
+    assert torch.equal(out[:n], mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])[:n])
+    assert (out[n:] == 7).all()
+    t = case(M, 256, 272, E=E, counts=counts, halves=2)
+    codes, scales = torch.full((M, 256), 3.0, device="cuda").to(F8), torch.full((M, 2), 9.0, device="cuda")
+    mb.gemm_swiglu_fp8_block_out(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"], out=(codes, scales))
+    wc, ws = mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    assert torch.equal(codes[:n].float(), wc[:n].float()) and torch.equal(scales[:n], ws[:n])
+    assert (codes[n:].float() == 3).all() and (scales[n:] == 9).all()
+
+
+@pytest.mark.parametrize("M", [7, 300])
+def test_guard_rows_and_strides(M):
+    """Operands inside larger ones, the output between guard rows; what lies around A is NaN."""
+    N, K = 264, 400
+    t = case(M, N, K)
+    want = mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"])
+    big = torch.full((M + 2, 512), 127, dtype=torch.uint8, device="cuda")  # 127 is NaN in e4m3
+    big[1:-1, 64:64 + K] = t["a"].view(torch.uint8)
+    scales = torch.full((M + 2, 9), float("nan"), device="cuda")
+    scales[1:-1, 3:7] = t["a_scale"]
+    guard = torch.full((M + 2, N), 5.0, dtype=BF, device="cuda")
+    mb.gemm_fp8_block_out(big.view(F8)[1:-1, 64:64 + K], scales[1:-1, 3:7], t["b"], t["b_scale"], out=guard[1:-1])
+    assert torch.equal(guard[1:-1], want) and (guard[0] == 5).all() and (guard[-1] == 5).all()
+    odd = torch.zeros(M, 512, dtype=torch.uint8, device="cuda")[:, 1:1 + K]  # unaligned: copied
+    odd.copy_(t["a"].view(torch.uint8))
+    assert torch.equal(mb.gemm_fp8_block(odd.view(F8), t["a_scale"].t().contiguous().t(), t["b"], t["b_scale"]), want)
+    flat = torch.zeros(M * K + 8, dtype=torch.uint8, device="cuda")[8:].view(M, K)  # contiguous, 8-byte aligned
+    flat.copy_(t["a"].view(torch.uint8))
+    assert torch.equal(mb.gemm_fp8_block(flat.view(F8), t["a_scale"], t["b"], t["b_scale"]), want)
+
+
+@pytest.mark.parametrize("M", [9, 260])
+def test_nan_and_infinite_rows_stay_by_themselves(M):
+    N, K, E, counts = 256, 272, 2, [M // 2, M - M // 2]
+    t = case(M, N, K, E=E, counts=counts)
+    clean = mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    t["a"].view(torch.uint8)[2, 100] = 127
+    t["a_scale"][5, 1] = float("inf")
+    got = mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    assert got[2].isnan().all() and not got[5].isfinite().any()
+    keep = [i for i in range(M) if i not in (2, 5)]
+    assert torch.equal(got[keep], clean[keep])
+    t = case(M, N, K, E=E, counts=counts, halves=2)
+    t["a"].view(torch.uint8)[2, 100] = 127
+    codes, scales = mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    assert scales[2].isnan().all() and codes[2].float().isnan().all()
+    assert scales[keep].isfinite().all() and not codes[keep].float().isnan().any()
+
+
+@pytest.mark.parametrize("M,counts", [(12, [5, 7]), (600, [280, 320])])
+def test_bad_offsets_touch_nothing_outside(M, counts):
+    t = case(M, 256, 256, E=2, counts=counts)
+    guard = torch.full((M + 2, 256), 5.0, dtype=BF, device="cuda")
+    for bad in ([-9, counts[0], 2 ** 31 - 1], [0, 10 ** 6, M], [M, M, M]):
+        off = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        mb.gemm_fp8_block_out(t["a"], t["a_scale"], t["b"], t["b_scale"], off, out=guard[1:-1])
+        torch.cuda.synchronize()
+        assert (guard[0] == 5).all() and (guard[-1] == 5).all()
+    assert mb.device_status(0)["code"] == 0
+
+
+@pytest.mark.parametrize("M,N,K,E", [(3, 512, 2048, 0), (40, 256, 512, 8), (700, 512, 384, 0), (900, 264, 512, 3)])
+def test_the_same_bits_every_time(M, N, K, E):
+    counts = [M // E] * E if E else None
+    for halves, form in ((1, mb.gemm_fp8_block), (2, mb.gemm_swiglu_fp8_block)):
+        t = case(M, -(-N // 16) * 16, K, E=E, counts=counts, halves=halves)
+        runs = [form(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"]) for _ in range(3)]
+        for r in runs[1:]:
+            for x, y in zip(r if halves == 2 else (r,), runs[0] if halves == 2 else (runs[0],)):
+                assert torch.equal(x.float(), y.float())
+
+
+def routed_block(s):
+    row_slot, slot_row, offsets = mb.expert_sort_out(s["ids"], s["w2"].shape[0])
+    a, sc = mb.expert_gather_fp8_out(s["x"], row_slot, slot_row)
+    h, hs = mb.gemm_swiglu_fp8_block_out(a, sc, s["w13"], s["w13_scale"], offsets)
+    y = mb.gemm_fp8_block_out(h, hs, s["w2"], s["w2_scale"], offsets)
+    return mb.expert_combine_out(y, s["w"], row_slot, slot_row)
+
+
+def routed_state(T, k, E, H, N, seed, drop=0.0):
+    g = gen(seed)
+    w13 = (0.05 * torch.randn(E, 2 * N, H, generator=g, device="cuda")).to(BF)
+    w2 = (0.05 * torch.randn(E, H, N, generator=g, device="cuda")).to(BF)
+    s = dict(x=torch.randn(T, H, generator=g, device="cuda").to(BF), w13_bf16=w13, w2_bf16=w2)
+    s["w13"], s["w13_scale"] = mb.quantize_fp8_gate_up(w13)
+    s["w2"], s["w2_scale"] = mb.quantize_fp8_weight(w2)
+    s["ids"] = torch.randint(0, E, (T, k), generator=g, device="cuda")
+    s["ids"][torch.rand(T, k, generator=g, device="cuda") < drop] = -1
+    s["w"] = torch.softmax(torch.randn(T, k, generator=g, device="cuda"), 1)
+    return s
+
+
+@pytest.mark.parametrize("T,k,E,H,N,drop", [(1, 2, 8, 256, 272, 0), (37, 2, 4, 272, 256, 0.2), (500, 4, 6, 512, 384, 0.05)])
+def test_the_operators_together(T, k, E, H, N, drop):
+    """A routed block in 8 bits against the bf16 weights in 64 bits.  Each of the three quantisations (rows, weights, the
+    activation) is a relative error of at most 2^-4 an element with random signs; over sums of hundreds of elements the
+    result's 2-norm error stays under 3 * 2^-4 / sqrt(3) (uniform in a step) ~ 0.11 of its norm."""
+    s = routed_state(T, k, E, H, N, seed=T, drop=drop)
+    got = routed_block(s).double()
+    want = torch.zeros(T, H, dtype=torch.float64, device="cuda")
+    x = s["x"].double()
+    for t in range(T):
+        for j in range(k):
+            e = int(s["ids"][t, j])
+            if e >= 0:
+                h = s["w13_bf16"][e].double() @ x[t]
+                y = s["w2_bf16"][e].double() @ (h[:N] * torch.sigmoid(h[:N]) * h[N:])
+                want[t] += s["w"][t, j].double() * y
+    assert (got - want).norm() <= 0.11 * want.norm()
+
+
+def test_the_operators_together_in_a_graph():
+    """Captured once, replayed on new tokens and routings (decode and prompt sizes), two graphs in turn."""
+    built = []
+    for T in (3, 300):
+        s = routed_state(T, 2, 4, 256, 256, seed=T)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            routed_block(s)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = routed_block(s)
+        built.append((s, graph, out))
+    for turn in range(3):
+        for s, graph, _ in built:
+            new = routed_state(s["x"].shape[0], 2, 4, 256, 256, seed=90 + turn, drop=0.3)
+            for key in ("x", "ids", "w"):
+                s[key].copy_(new[key])
+            graph.replay()
+        for s, _, out in built:
+            assert torch.equal(out, routed_block(s))
+    assert mb.device_status(0)["code"] == 0
