@@ -384,5 +384,327 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
   if (warp == 5) tmem_dealloc<1>(tmem, kTmem);
 }
 
+// ---------------------------------------------------------------- many rows an expert: CTA pairs
+// fp8_block_tile_kernel: tokens are the MMA's rows.  A pair (tcgen05 cta_group::2) owns 256 rows of one expert and 256
+// rows of W (256 output columns, or 128 gate and the matching 128 up columns); each CTA loads its own 128 rows of A and
+// half of W's, 32 KB per K block for 512 cycles of MMA.  A thread of the epilogue owns one row, so its scale is one number
+// per 128 columns and an addition is one fused multiply-add; with 128 of them per thread and block, two epilogue warps a
+// scheduler keep up with the MMA (half of the issue slots) and the registers for them come from the other warpgroup.
+// Persistent: tiles go round-robin to the pairs in bands of kBand row groups, column tile by column tile, so that the
+// pairs that run together share A rows and W rows in L2.
+constexpr int kTileThreads = 384;  // warps 0 TMA, 1 MMA, 2 tensor-memory allocator, 3 expert map; 4-11 epilogue
+constexpr int kTileRegs = 168;     // a thread's registers at launch: 384 * 168 = 64512 = 128 * 40 + 256 * 232
+constexpr int kTileRows = 256;     // rows of a pair
+constexpr int kTileStage = 2 * kWTile;
+constexpr int kTileStages = 6;
+constexpr int kBand = 8;
+constexpr int kMapExperts = 1024;
+
+struct TileAt {
+  int e, row0, end, n0;  // rows [row0, min(row0 + 256, end)), first output column
+};
+
+template <int kHalves>
+__global__ void __launch_bounds__(kTileThreads, 1)
+fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const Args a,
+                      const int wide_store) {
+  constexpr int kOutCols = 256 / kHalves;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int row_start[kMapExperts + 1], unit_first[kMapExperts + 1];
+  __shared__ unsigned top_half[2][128];
+  __shared__ __align__(8) uint64_t bars[2 * kTileStages + 4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();  // rank 0 issues the pair's MMAs
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (kTileStages + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * kTileStages + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kTileStages + 2 + b); };
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kTileStages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 16);  // the epilogue warps of both CTAs
+    }
+    fence_barrier_init();
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_a);
+  }
+  if (warp == 2) {
+    tmem_alloc<2>(smem_u32(&tmem_slot), 512);
+    tmem_relinquish<2>();
+  }
+  if (warp == 3) {  // where each expert's rows and row groups begin; clamped, see find_unit
+    int seen = 0;
+    for (int b = 0; b <= a.E; b += 32) {
+      const int e = b + lane;
+      int lo = 0, n = 0;
+      if (e <= a.E) {
+        lo = a.offsets ? min(max(a.offsets[e], 0), a.R) : (e == 0 ? 0 : a.R);
+        if (e < a.E) {
+          const int hi = a.offsets ? min(max(a.offsets[e + 1], lo), a.R) : a.R;
+          n = (hi - lo + kTileRows - 1) / kTileRows;
+        }
+        row_start[e] = lo;
+      }
+      int scan = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += up;
+      }
+      if (e <= a.E) unit_first[e] = seen + scan - n;
+      seen += __shfl_sync(0xffffffffu, scan, 31);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers exist before anything signals them
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const int n_tiles = (a.N + kOutCols - 1) / kOutCols;
+  const int units = unit_first[a.E], total = units * n_tiles;
+
+  auto locate = [&](int t) {
+    TileAt at;
+    const int band = t / (kBand * n_tiles), rem = t - band * kBand * n_tiles;
+    const int high = min(kBand, units - band * kBand);
+    const int unit = band * kBand + rem % high;
+    at.n0 = rem / high * kOutCols;
+    int lo = 0, hi = a.E;  // unit_first[lo] <= unit < unit_first[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (unit_first[mid] <= unit) lo = mid; else hi = mid;
+    }
+    at.e = lo;
+    at.row0 = row_start[lo] + (unit - unit_first[lo]) * kTileRows;
+    at.end = max(row_start[lo], row_start[lo + 1]);
+    return at;
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------- TMA producer (each CTA its own halves)
+      const uint64_t keep = l2_policy_evict_last(), normal = l2_policy_evict_normal();
+      const uint32_t full0 = map_to_cta(full_bar(0), 0);  // the bytes of both CTAs are counted on rank 0's barrier
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += pairs) {
+        const TileAt at = locate(t);
+        const int row = at.row0 + 128 * rank;
+        const int wrow = kHalves == 1 ? at.n0 + 128 * rank : at.n0, whalf = kHalves == 1 ? at.e : at.e * 2 + rank;
+        for (int kb = 0; kb < a.kb; ++kb) {
+          if (!(ok = wait_bounded(empty_bar(stage), phase ^ 1u, &abort_flag, 1u, stage))) break;
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kTileStage);
+          const uint32_t dst = tiles + stage * kTileStage;
+          tma_load_2d_pair_hint(dst, &tm_a, full0 + 8u * stage, kb * kBlk, row, keep);
+          tma_load_3d_pair_hint(dst + kWTile, &tm_w, full0 + 8u * stage, kb * kBlk, wrow, whalf, normal);
+          if (++stage == kTileStages) stage = 0, phase ^= 1u;
+        }
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      const uint32_t idesc = umma_idesc_e4m3(256, 256);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += pairs)
+        for (int kb = 0; kb < a.kb; ++kb, ++it) {
+          const int buf = it & 1;
+          ok = wait_bounded(acc_empty(buf), ((it >> 1) & 1) ^ 1u, &abort_flag, 2u, 16 + buf) &&
+               wait_bounded(full_bar(stage), phase, &abort_flag, 2u, stage);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint64_t da = umma_desc_k_sw128(tiles + stage * kTileStage);
+          const uint64_t dw = umma_desc_k_sw128(tiles + stage * kTileStage + kWTile);
+#pragma unroll
+          for (int i = 0; i < kBlk / 32; ++i) umma_fp8<2>(tmem + buf * 256, da + 2 * i, dw + 2 * i, idesc, i > 0);
+          umma_commit<2>(empty_bar(stage));
+          umma_commit<2>(acc_full(buf));
+          if (++stage == kTileStages) stage = 0, phase ^= 1u;
+        }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    // ------------------------------------------------------------ scale, add, write: one row per thread
+    const int q = warp & 3, part = (warp - 4) >> 2;  // lane quarter; which half of the columns
+    const int my_row = 128 * rank + 32 * q + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+    const uint32_t acc_empty0 = map_to_cta(acc_empty(0), 0);
+    // plain: 128 columns of one block of W; SwiGLU: 64 gate columns, then the 64 up columns that meet them
+    const int col[4] = {kHalves == 1 ? 128 * part : 64 * part, kHalves == 1 ? 128 * part + 32 : 64 * part + 32,
+                        kHalves == 1 ? 128 * part + 64 : 128 + 64 * part, kHalves == 1 ? 128 * part + 96 : 160 + 64 * part};
+    struct Scales {
+      const float *row, *w0, *w1;
+    };
+    auto scales_at = [&](const TileAt& at) {
+      Scales p;
+      const int row = min(at.row0 + my_row, at.end - 1);
+      p.row = a.a_scale + (long long)row * a.ld_as;
+      const int block = min(at.n0 / kBlk + (kHalves == 1 ? part : 0), a.nb - 1);
+      p.w0 = a.b_scale + ((long long)at.e * kHalves * a.nb + block) * a.kb;
+      p.w1 = p.w0 + (kHalves == 1 ? 0 : (long long)a.nb * a.kb);
+      return p;
+    };
+    float row_s[4], w0_s[4], w1_s[4], row_n[4], w0_n[4], w1_n[4];  // four K blocks, and the next four
+    auto fetch = [&](const Scales& p, int kb) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int b = min(kb + i, a.kb - 1);
+        row_n[i] = __ldg(p.row + b);
+        w0_n[i] = __ldg(p.w0 + b);
+        if (kHalves == 2) w1_n[i] = __ldg(p.w1 + b);
+      }
+    };
+    int it = 0;
+    bool ok = true;
+    TileAt at{0, 0, 0, 0}, next_at{0, 0, 0, 0};
+    Scales sp{nullptr, nullptr, nullptr}, next_sp{nullptr, nullptr, nullptr};
+    if (pair < total) {
+      next_at = locate(pair);
+      next_sp = scales_at(next_at);
+      fetch(next_sp, 0);
+    }
+    for (int t = pair; t < total; t += pairs) {
+      at = next_at;
+      sp = next_sp;
+      float acc[128];
+#pragma unroll
+      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+      for (int kb = 0; kb < a.kb; kb += 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) row_s[i] = row_n[i], w0_s[i] = w0_n[i], w1_s[i] = w1_n[i];
+        if (kb + 4 < a.kb) {
+          fetch(sp, kb + 4);
+        } else if (t + pairs < total) {  // the next tile's first scales travel while this tile ends
+          next_at = locate(t + pairs);
+          next_sp = scales_at(next_at);
+          fetch(next_sp, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (kb + i >= a.kb) break;
+          const int buf = it & 1;
+          ok = __all_sync(0xffffffffu, ok && wait_bounded(acc_full(buf), (it >> 1) & 1, &abort_flag, 3u, buf));
+          ++it;
+          if (!ok) continue;
+          tc_fence_after_sync();
+          const float s0 = row_s[i] * w0_s[i], s1 = kHalves == 1 ? s0 : row_s[i] * w1_s[i];
+          uint32_t p[2][32];
+          tmem_ld_x32(lanes + buf * 256 + col[0], p[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait();
+            tmem_regs_ready(p[c & 1]);
+            if (c < 3) {
+              tmem_ld_x32(lanes + buf * 256 + col[c + 1], p[(c + 1) & 1]);
+            } else {  // the last read has landed: hand the buffer back before the arithmetic
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + 8u * buf);
+            }
+            const float s = c < 2 ? s0 : s1;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(p[c & 1][j]), s, acc[32 * c + j]);
+          }
+        }
+      }
+      const long long row = at.row0 + my_row;
+      const bool here = ok && row < at.end;
+      if constexpr (kHalves == 1) {
+        const int n = at.n0 + 128 * part;
+        __nv_bfloat16* dst = a.c + row * a.N + n;
+        if (here) {
+#pragma unroll
+          for (int j = 0; j < 128; j += 16) {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(acc[j + 2 * i], acc[j + 2 * i + 1]);
+              o[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+            if (wide_store) {  // 32-byte rows: N is a multiple of 16
+              if (n + j < a.N) st_global_v8_hint(dst + j, lo, hi, l2_policy_evict_first());
+            } else {
+              if (n + j < a.N) *reinterpret_cast<uint4*>(dst + j) = lo;
+              if (n + j + 8 < a.N) *reinterpret_cast<uint4*>(dst + j + 8) = hi;
+            }
+          }
+        }
+      } else {
+        unsigned top = 0;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+          acc[j] = silu_mul(acc[j], acc[64 + j]);  // columns beyond N are zeros
+          top = max(top, __float_as_uint(fabsf(acc[j])));
+        }
+        // the other 64 columns of this row's block belong to the other warp of the lane quarter
+        top_half[part][32 * q + lane] = top;
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+        top = max(top, top_half[part ^ 1][32 * q + lane]);
+        float s = __fdiv_rn(__uint_as_float(top), kCodeMax);
+        s = s < kScaleFloor ? kScaleFloor : s;
+        const float r = __frcp_rn(s);  // see the stream kernel
+        const int n = at.n0 + 64 * part;
+        if (here) {
+          uint8_t* dst = a.codes + row * a.N + n;
+#pragma unroll
+          for (int j = 0; j < 64; j += 16) {
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[i] = pack4(acc[j + 4 * i] * r, acc[j + 4 * i + 1] * r, acc[j + 4 * i + 2] * r, acc[j + 4 * i + 3] * r);
+            if (n + j < a.N) *reinterpret_cast<uint4*>(dst + j) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+          if (part == 0) a.scales[row * a.nb + at.n0 / kBlk] = s;
+        }
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");  // both have read before the next tile writes
+      }
+    }
+    // rows behind the last expert's: one contiguous piece of each output
+    if (a.zero_tail && a.offsets) {
+      const long long from = max(0, min(row_start[a.E], a.R)), rows = a.R - from;
+      const long long me = (long long)blockIdx.x * 256 + threadIdx.x - 128, all = (long long)gridDim.x * 256;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      if constexpr (kHalves == 1) {
+        uint4* dst = reinterpret_cast<uint4*>(a.c + from * a.N);
+        for (long long i = me; i < rows * a.N / 8; i += all) dst[i] = zero;
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(a.codes + from * a.N);
+        for (long long i = me; i < rows * a.N / 16; i += all) dst[i] = zero;
+        for (long long i = me; i < rows * a.nb; i += all) a.scales[from * a.nb + i] = kScaleFloor;
+      }
+    }
+  }
+
+  // ------------------------------------------------------------ teardown (also the abort path)
+  __syncwarp();
+  if (*reinterpret_cast<volatile int*>(&abort_flag)) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000LL) {
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // the pair leaves together: MMAs read both CTAs' shared memory, both share barriers
+  if (warp == 2) {
+    tc_fence_after_sync();
+    tmem_dealloc<2>(tmem, 512);
+  }
+}
+
 }  // namespace fp8
 }  // namespace magi

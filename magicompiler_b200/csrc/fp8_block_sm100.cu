@@ -83,6 +83,66 @@ static int launch_stream(const Problem& p, int sm_count, cudaStream_t stream) {
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_stream_kernel");
 }
 
+// CTA pairs that the GPU holds at once, per device and form (0: not queried yet).
+static int g_tile_pairs[kMaxDevices][2];
+
+template <int kHalves>
+static int launch_tiles(const Problem& p, int device, int sm_count, cudaStream_t stream) {
+  const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.args.E * kHalves};
+  const cuuint64_t wst[2] = {(cuuint64_t)p.K, (cuuint64_t)p.N * (cuuint64_t)p.K};
+  const cuuint64_t ad[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M};
+  const cuuint64_t ast[1] = {(cuuint64_t)p.lda};
+  const cuuint32_t wb[3] = {kBlk, 128, 1}, ab[2] = {kBlk, 128};
+  CUtensorMap tm_w, tm_a;
+  if (int rc = encode_bytes_map(p.b, 3, wd, wst, wb, &tm_w, "B")) return rc;
+  if (int rc = encode_bytes_map(p.a, 2, ad, ast, ab, &tm_a, "A")) return rc;
+  const int64_t n_tiles = (p.N + 256 / kHalves - 1) / (256 / kHalves);
+  const int64_t units = p.M / kTileRows + (p.args.offsets ? p.args.E : 1);  // at most one partial group an expert
+  if (units * n_tiles > 0x7fffffffLL / 2) return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld x N=%lld is too large for one launch", (long long)p.M, (long long)p.N);
+  constexpr int kSmem = kTileStages * kTileStage + 1024;
+  auto kernel = fp8_block_tile_kernel<kHalves>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaSuccess;
+  int pairs = 0;
+  {
+    std::lock_guard<std::mutex> lock(g_dev_mutex);
+    int& known = g_tile_pairs[device][kHalves - 1];
+    if (known == 0) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+      cudaFuncAttributes fa;
+      e = cudaFuncGetAttributes(&fa, kernel);
+      if (e != cudaSuccess) return fail_cuda(e, "cudaFuncGetAttributes");
+      // the warpgroups' register shares add up to the launch's total: fewer at launch and the larger share would wait for good
+      if (fa.numRegs != kTileRegs)
+        return fail(MAGI_SWIGLU_ERR_DEVICE, "fp8_block_tile_kernel was built with %d registers a thread, not %d", fa.numRegs, kTileRegs);
+      cfg.gridDim = dim3((unsigned)(sm_count / 2 * 2));
+      int n = 0;
+      e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+      if (e != cudaSuccess) return fail_cuda(e, "cudaOccupancyMaxActiveClusters");
+      if (n < 1) return fail(MAGI_SWIGLU_ERR_DEVICE, "this device cannot hold a CTA pair of fp8_block_tile_kernel");
+      known = n;
+    }
+    pairs = known;
+  }
+  const int64_t most = units * n_tiles;
+  if (pairs > most) pairs = (int)most;
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  const int wide = ((uintptr_t)p.args.c & 31u) == 0 && p.N % 16 == 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_a, p.args, wide);
+  return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_tile_kernel");
+}
+
 static int run(const Problem& p, int device, void* cuda_stream) {
   const DeviceInfo* di = nullptr;
   if (int rc = require_b200(device, &di)) return rc;
@@ -96,11 +156,13 @@ static int run(const Problem& p, int device, void* cuda_stream) {
     if (share <= 16) return launch_stream<1, 16>(p, di->sm_count, stream);
     if (share <= 32) return launch_stream<1, 32>(p, di->sm_count, stream);
     if (share <= 64) return launch_stream<1, 64>(p, di->sm_count, stream);
-    return launch_stream<1, 128>(p, di->sm_count, stream);
+    if (share <= 128) return launch_stream<1, 128>(p, di->sm_count, stream);
+    return launch_tiles<1>(p, device, di->sm_count, stream);
   }
   if (share <= 16) return launch_stream<2, 16>(p, di->sm_count, stream);
   if (share <= 32) return launch_stream<2, 32>(p, di->sm_count, stream);
-  return launch_stream<2, 64>(p, di->sm_count, stream);
+  if (share <= 64) return launch_stream<2, 64>(p, di->sm_count, stream);
+  return launch_tiles<2>(p, device, di->sm_count, stream);
 }
 
 static int check(const void* a, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,
