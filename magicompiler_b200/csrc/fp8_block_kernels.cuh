@@ -68,6 +68,7 @@ struct Args {
   int splits;             // CTAs of a cluster that share a tile's K blocks
   int stages;
   int zero_tail;          // rows from offsets[E] on: 1 = written as zeros, 0 = left alone
+  int never;              // 0; a condition that the compiler cannot fold
 };
 
 struct Unit {  // rows [row0, row0 + rows) of expert e; e == E: rows behind the last expert's; rows == 0: nothing
@@ -392,17 +393,19 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
 // scheduler keep up with the MMA (half of the issue slots) and the registers for them come from the other warpgroup.
 // Persistent: tiles go round-robin to the pairs in bands of kBand row groups, column tile by column tile, so that the
 // pairs that run together share A rows and W rows in L2.
-constexpr int kTileThreads = 384;  // warps 0 TMA, 1 MMA, 2 tensor-memory allocator, 3 expert map; 4-11 epilogue
-constexpr int kTileRegs = 168;     // a thread's registers at launch: 384 * 168 = 64512 = 128 * 40 + 256 * 232
+constexpr int kTileThreads = 384;  // warps 0 TMA, 1 and 3 MMA, 2 tensor-memory allocator and scales; 4-11 epilogue
+constexpr int kTileRegs = 168;     // a thread's registers at launch: 384 * 168 = 64512 = 128 * 56 + 256 * 224
 constexpr int kTileRows = 256;     // rows of a pair
 constexpr int kTileStage = 2 * kWTile;
 constexpr int kTileStages = 6;
 constexpr int kBand = 8;
 constexpr int kMapExperts = 1024;
+constexpr int kScaleSlots = 4;     // ring of scale products, four K blocks a slot
 
 struct TileAt {
   int e, row0, end, n0;  // rows [row0, min(row0 + 256, end)), first output column
 };
+constexpr int kTileInfos = 2 * kScaleSlots;  // the scale warp is at most kScaleSlots tiles ahead
 
 template <int kHalves>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -412,7 +415,9 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   extern __shared__ uint8_t smem_raw[];
   __shared__ int row_start[kMapExperts + 1], unit_first[kMapExperts + 1];
   __shared__ unsigned top_half[2][128];
-  __shared__ __align__(8) uint64_t bars[2 * kTileStages + 4];
+  __shared__ TileAt tile_info[kTileInfos];
+  __shared__ float scale_ring[kScaleSlots][4][2][128];  // as * bs of each row with both 128-column blocks of the tile
+  __shared__ __align__(8) uint64_t bars[2 * kTileStages + 4 + 2 * kScaleSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
 
@@ -425,6 +430,8 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   auto empty_bar = [&](int s) { return bar0 + 8u * (kTileStages + s); };
   auto acc_full = [&](int b) { return bar0 + 8u * (2 * kTileStages + b); };
   auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kTileStages + 2 + b); };
+  auto scale_full = [&](int s) { return bar0 + 8u * (2 * kTileStages + 4 + s); };
+  auto scale_empty = [&](int s) { return bar0 + 8u * (2 * kTileStages + 4 + kScaleSlots + s); };
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -435,6 +442,10 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
       mbar_init(acc_empty(b), 16);  // the epilogue warps of both CTAs
+    }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(scale_full(s), 1);
+      mbar_init(scale_empty(s), 8);
     }
     fence_barrier_init();
     prefetch_tensormap(&tm_w);
@@ -493,7 +504,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- TMA producer (each CTA its own halves)
       const uint64_t keep = l2_policy_evict_last(), normal = l2_policy_evict_normal();
@@ -514,30 +525,77 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
           if (++stage == kTileStages) stage = 0, phase ^= 1u;
         }
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-      // ---------------------------------------------------------- MMA issuer
+    } else if ((warp == 1 || warp == 3) && rank == 0) {
+      // ---------------------------------------------------------- MMA issuers: warp 1 the even K blocks, warp 3 the odd
+      // ones, each with a buffer of its own.  A wait costs about a hundred cycles even when it is over, and issuing four
+      // MMAs holds a thread until the tensor pipe has taken them; two issuers do their waits in each other's shadow, and
+      // lanes 0 and 1 of each wait for operands and buffer at the same time.
       const uint32_t idesc = umma_idesc_e4m3(256, 256);
-      int stage = 0, it = 0;
+      const int buf = warp >> 1;
+      int it = 0, stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; t < total && ok; t += pairs)
         for (int kb = 0; kb < a.kb; ++kb, ++it) {
-          const int buf = it & 1;
-          ok = wait_bounded(acc_empty(buf), ((it >> 1) & 1) ^ 1u, &abort_flag, 2u, 16 + buf) &&
-               wait_bounded(full_bar(stage), phase, &abort_flag, 2u, stage);
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint64_t da = umma_desc_k_sw128(tiles + stage * kTileStage);
-          const uint64_t dw = umma_desc_k_sw128(tiles + stage * kTileStage + kWTile);
+          if ((it & 1) == buf) {
+            if (lane == 0) ok = wait_bounded(full_bar(stage), phase, &abort_flag, 2u, stage);
+            if (lane == 1) ok = wait_bounded(acc_empty(buf), ((it >> 1) & 1) ^ 1u, &abort_flag, 2u, 16 + buf);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            tc_fence_after_sync();
+            if (lane == 0) {
+              const uint64_t da = umma_desc_k_sw128(tiles + stage * kTileStage);
+              const uint64_t dw = umma_desc_k_sw128(tiles + stage * kTileStage + kWTile);
 #pragma unroll
-          for (int i = 0; i < kBlk / 32; ++i) umma_fp8<2>(tmem + buf * 256, da + 2 * i, dw + 2 * i, idesc, i > 0);
-          umma_commit<2>(empty_bar(stage));
-          umma_commit<2>(acc_full(buf));
+              for (int i = 0; i < kBlk / 32; ++i) umma_fp8<2>(tmem + buf * 256, da + 2 * i, dw + 2 * i, idesc, i > 0);
+              umma_commit<2>(acc_full(buf));
+              umma_commit<2>(empty_bar(stage));
+            }
+            __syncwarp();
+          }
           if (++stage == kTileStages) stage = 0, phase ^= 1u;
         }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------- scales: the epilogue has no registers to spare for them
+      int slot = 0, nth = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += pairs, ++nth) {
+        const TileAt at = locate(t);
+        const float* w0 = a.b_scale + ((long long)at.e * kHalves * a.nb + at.n0 / kBlk) * a.kb;
+        // the tile's second block: the next 128 columns (none: any valid one), or the up half's
+        const float* w1 = w0 + (kHalves == 2 ? (long long)a.nb * a.kb : (at.n0 / kBlk + 1 < a.nb ? a.kb : 0));
+        const float* rows[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          rows[i] = a.a_scale + (long long)min(at.row0 + 128 * rank + 32 * i + lane, at.end - 1) * a.ld_as;
+        for (int kb = 0; kb < a.kb; kb += 4) {
+          if (!(ok = __all_sync(0xffffffffu, wait_bounded(scale_empty(slot), phase ^ 1u, &abort_flag, 4u, slot)))) break;
+#pragma unroll
+          for (int b = 0; b < 4; b += 2) {
+            const int k0 = min(kb + b, a.kb - 1), k1 = min(kb + b + 1, a.kb - 1);
+            float r0[4], r1[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r0[i] = __ldg(rows[i] + k0), r1[i] = __ldg(rows[i] + k1);
+            const float g0 = __ldg(w0 + k0), g1 = __ldg(w0 + k1), u0 = __ldg(w1 + k0), u1 = __ldg(w1 + k1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              scale_ring[slot][b][0][32 * i + lane] = r0[i] * g0;
+              scale_ring[slot][b][1][32 * i + lane] = r0[i] * u0;
+              scale_ring[slot][b + 1][0][32 * i + lane] = r1[i] * g1;
+              scale_ring[slot][b + 1][1][32 * i + lane] = r1[i] * u1;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) {
+            if (kb == 0) tile_info[nth % kTileInfos] = at;
+            mbar_arrive(scale_full(slot));
+          }
+          if (++slot == kScaleSlots) slot = 0, phase ^= 1u;
+        }
+      }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ------------------------------------------------------------ scale, add, write: one row per thread
     const int q = warp & 3, part = (warp - 4) >> 2;  // lane quarter; which half of the columns
     const int my_row = 128 * rank + 32 * q + lane;
@@ -546,81 +604,65 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     // plain: 128 columns of one block of W; SwiGLU: 64 gate columns, then the 64 up columns that meet them
     const int col[4] = {kHalves == 1 ? 128 * part : 64 * part, kHalves == 1 ? 128 * part + 32 : 64 * part + 32,
                         kHalves == 1 ? 128 * part + 64 : 128 + 64 * part, kHalves == 1 ? 128 * part + 96 : 160 + 64 * part};
-    struct Scales {
-      const float *row, *w0, *w1;
-    };
-    auto scales_at = [&](const TileAt& at) {
-      Scales p;
-      const int row = min(at.row0 + my_row, at.end - 1);
-      p.row = a.a_scale + (long long)row * a.ld_as;
-      const int block = min(at.n0 / kBlk + (kHalves == 1 ? part : 0), a.nb - 1);
-      p.w0 = a.b_scale + ((long long)at.e * kHalves * a.nb + block) * a.kb;
-      p.w1 = p.w0 + (kHalves == 1 ? 0 : (long long)a.nb * a.kb);
-      return p;
-    };
-    float row_s[4], w0_s[4], w1_s[4], row_n[4], w0_n[4], w1_n[4];  // four K blocks, and the next four
-    auto fetch = [&](const Scales& p, int kb) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int b = min(kb + i, a.kb - 1);
-        row_n[i] = __ldg(p.row + b);
-        w0_n[i] = __ldg(p.w0 + b);
-        if (kHalves == 2) w1_n[i] = __ldg(p.w1 + b);
-      }
-    };
-    int it = 0;
+    const uint64_t c_policy = l2_policy_evict_first();
+    int it = 0, slot = 0, never = a.never, nth = 0;
+    uint32_t slot_phase = 0;
     bool ok = true;
-    TileAt at{0, 0, 0, 0}, next_at{0, 0, 0, 0};
-    Scales sp{nullptr, nullptr, nullptr}, next_sp{nullptr, nullptr, nullptr};
-    if (pair < total) {
-      next_at = locate(pair);
-      next_sp = scales_at(next_at);
-      fetch(next_sp, 0);
-    }
-    for (int t = pair; t < total; t += pairs) {
-      at = next_at;
-      sp = next_sp;
-      float acc[128];
+    for (int t = pair; t < total; t += pairs, ++nth) {
+      uint64_t sum[64];  // pairs of neighbouring columns
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+      for (int i = 0; i < 64; ++i) sum[i] = 0;
       for (int kb = 0; kb < a.kb; kb += 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) row_s[i] = row_n[i], w0_s[i] = w0_n[i], w1_s[i] = w1_n[i];
-        if (kb + 4 < a.kb) {
-          fetch(sp, kb + 4);
-        } else if (t + pairs < total) {  // the next tile's first scales travel while this tile ends
-          next_at = locate(t + pairs);
-          next_sp = scales_at(next_at);
-          fetch(next_sp, 0);
-        }
+        ok = __all_sync(0xffffffffu, ok && wait_bounded(scale_full(slot), slot_phase, &abort_flag, 3u, 32 + slot));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (kb + i >= a.kb) break;
+          const float f0 = scale_ring[slot][i][kHalves == 1 ? part : 0][32 * q + lane];
+          const float f1 = kHalves == 1 ? f0 : scale_ring[slot][i][1][32 * q + lane];
           const int buf = it & 1;
           ok = __all_sync(0xffffffffu, ok && wait_bounded(acc_full(buf), (it >> 1) & 1, &abort_flag, 3u, buf));
           ++it;
           if (!ok) continue;
           tc_fence_after_sync();
-          const float s0 = row_s[i] * w0_s[i], s1 = kHalves == 1 ? s0 : row_s[i] * w1_s[i];
-          uint32_t p[2][32];
-          tmem_ld_x32(lanes + buf * 256 + col[0], p[0]);
+          const uint64_t s0 = pack_f32x2(f0, f0), s1 = pack_f32x2(f1, f1);
+          const uint32_t from = lanes + buf * 256;
+          // The buffer goes back as soon as the last columns have been read: everything before that is on the MMA's
+          // critical path, so two loads are in flight and the arithmetic that can wait comes after the arrival.
+          uint32_t p[32], q2[32];
+          tmem_ld_x32(from + col[0], p);
+          tmem_ld_x32(from + col[1], q2);
+          tmem_ld_wait();
+          tmem_regs_ready(p);
+          tmem_regs_ready(q2);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_ld_wait();
-            tmem_regs_ready(p[c & 1]);
-            if (c < 3) {
-              tmem_ld_x32(lanes + buf * 256 + col[c + 1], p[(c + 1) & 1]);
-            } else {  // the last read has landed: hand the buffer back before the arithmetic
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + 8u * buf);
-            }
-            const float s = c < 2 ? s0 : s1;
+          for (int j = 0; j < 16; ++j) fma_f32x2(sum[j], p[2 * j], p[2 * j + 1], s0);
+          tmem_ld_x32(from + col[2], p);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(p[c & 1][j]), s, acc[32 * c + j]);
-          }
+          for (int j = 0; j < 16; ++j) fma_f32x2(sum[16 + j], q2[2 * j], q2[2 * j + 1], s0);
+          tmem_ld_x32(from + col[3], q2);
+          tmem_ld_wait();
+          tmem_regs_ready(p);
+          tmem_regs_ready(q2);
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + 8u * buf);
+          // A branch that is never taken: instructions do not move across it, and without it the assembler puts the
+          // arithmetic below in front of the arrival (957 instead of 813 cycles a K block, K = 14336).
+          asm volatile("" : "+r"(never));
+          if (never) break;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) fma_f32x2(sum[32 + j], p[2 * j], p[2 * j + 1], s1);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) fma_f32x2(sum[48 + j], q2[2 * j], q2[2 * j + 1], s1);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scale_empty(slot));
+        if (++slot == kScaleSlots) slot = 0, slot_phase ^= 1u;
       }
+      const TileAt at = tile_info[nth % kTileInfos];
+      float acc[128];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) unpack_f32x2(sum[i], acc[2 * i], acc[2 * i + 1]);
       const long long row = at.row0 + my_row;
       const bool here = ok && row < at.end;
       if constexpr (kHalves == 1) {
@@ -637,7 +679,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
             }
             const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
             if (wide_store) {  // 32-byte rows: N is a multiple of 16
-              if (n + j < a.N) st_global_v8_hint(dst + j, lo, hi, l2_policy_evict_first());
+              if (n + j < a.N) st_global_v8_hint(dst + j, lo, hi, c_policy);
             } else {
               if (n + j < a.N) *reinterpret_cast<uint4*>(dst + j) = lo;
               if (n + j + 8 < a.N) *reinterpret_cast<uint4*>(dst + j + 8) = hi;

@@ -180,6 +180,27 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
+// Two fp32 values in one 64-bit register, and the fused multiply-add of two such pairs in one instruction.
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+// acc += {lo, hi} * s.  Volatile: keeps its place among tensor-memory loads, waits and barrier arrivals.
+__device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s) {
+  asm volatile(
+      "{\n\t"
+      ".reg .b64 t;\n\t"
+      "mov.b64 t, {%1, %2};\n\t"
+      "fma.rn.f32x2 %0, t, %3, %0;\n\t"
+      "}"
+      : "+l"(acc)
+      : "r"(lo), "r"(hi), "l"(s));
+}
+
 __device__ __forceinline__ uint64_t l2_policy_evict_first() {
   uint64_t p;
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
