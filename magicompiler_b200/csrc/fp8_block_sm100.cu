@@ -41,7 +41,7 @@ struct Problem {
 };
 
 template <int kHalves, int kTok>
-static int launch_stream(const Problem& p, int sm_count, cudaStream_t stream) {
+static int launch_stream(const Problem& p, int device, int sm_count, cudaStream_t stream) {
   constexpr int kStage = kHalves * kWTile + kTok * kBlk;
   constexpr int kBudget = kHalves * kTok <= 64 ? 108 * 1024 : 216 * 1024;  // two CTAs an SM, or one
   constexpr int kFit = (kBudget - 1024) / kStage;
@@ -62,10 +62,15 @@ static int launch_stream(const Problem& p, int sm_count, cudaStream_t stream) {
   if (groups > 65535 || n_tiles > 0x7fffffffLL / 8)
     return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld rows are too many for one launch", (long long)p.M);
   Args args = p.args;
+  // Few tiles leave SMs idle: then up to eight CTAs of a cluster share a tile's K blocks (at least four each) and add
+  // their sums through distributed shared memory, until there are about two CTAs an SM.
+  const int64_t busy = n_tiles * (p.args.offsets ? (p.M < p.args.E ? p.M : p.args.E) : groups);
   args.splits = 1;
+  while (args.splits < 8 && busy * args.splits * 2 <= 2 * sm_count && args.kb >= args.splits * 8) args.splits *= 2;
   args.stages = kStages;
   const int smem = kStages * kStage + 1024;
-  cudaError_t e = cudaFuncSetAttribute(fp8_block_stream_kernel<kHalves, kTok>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static int smem_set[kMaxDevices];
+  cudaError_t e = allow_smem_once(fp8_block_stream_kernel<kHalves, kTok>, smem, device, smem_set);
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -78,7 +83,7 @@ static int launch_stream(const Problem& p, int sm_count, cudaStream_t stream) {
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = args.splits > 1 ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, fp8_block_stream_kernel<kHalves, kTok>, tm_w, tm_a, args);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_stream_kernel");
 }
@@ -153,15 +158,15 @@ static int run(const Problem& p, int device, void* cuda_stream) {
   // Tokens per tile: enough for an expert's average share of the rows, so that W is usually streamed once.
   const int64_t share = p.args.offsets ? (p.M + p.args.E - 1) / p.args.E : p.M;
   if (p.halves == 1) {
-    if (share <= 16) return launch_stream<1, 16>(p, di->sm_count, stream);
-    if (share <= 32) return launch_stream<1, 32>(p, di->sm_count, stream);
-    if (share <= 64) return launch_stream<1, 64>(p, di->sm_count, stream);
-    if (share <= 128) return launch_stream<1, 128>(p, di->sm_count, stream);
+    if (share <= 16) return launch_stream<1, 16>(p, device, di->sm_count, stream);
+    if (share <= 32) return launch_stream<1, 32>(p, device, di->sm_count, stream);
+    if (share <= 64) return launch_stream<1, 64>(p, device, di->sm_count, stream);
+    if (share <= 128) return launch_stream<1, 128>(p, device, di->sm_count, stream);
     return launch_tiles<1>(p, device, di->sm_count, stream);
   }
-  if (share <= 16) return launch_stream<2, 16>(p, di->sm_count, stream);
-  if (share <= 32) return launch_stream<2, 32>(p, di->sm_count, stream);
-  if (share <= 64) return launch_stream<2, 64>(p, di->sm_count, stream);
+  if (share <= 16) return launch_stream<2, 16>(p, device, di->sm_count, stream);
+  if (share <= 32) return launch_stream<2, 32>(p, device, di->sm_count, stream);
+  if (share <= 64) return launch_stream<2, 64>(p, device, di->sm_count, stream);
   return launch_tiles<2>(p, device, di->sm_count, stream);
 }
 

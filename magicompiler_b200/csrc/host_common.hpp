@@ -84,6 +84,16 @@ inline int require_b200(int device, const DeviceInfo** out) {
   return 0;
 }
 
+// Raises a kernel's dynamic shared memory limit once per device; `done` is the caller's flag array for that kernel.
+template <typename Kernel>
+inline cudaError_t allow_smem_once(Kernel kernel, int bytes, int device, int* done) {
+  std::lock_guard<std::mutex> lock(g_dev_mutex);
+  if (done[device]) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done[device] = 1;
+  return e;
+}
+
 struct DeviceGuard {
   int prev = -1;
   bool changed = false;

@@ -82,8 +82,8 @@ int magi_swiglu_expert_sort(const void* ids, int ids_64bit, int64_t slots, int n
   int ctas = 1;
   while (ctas < 8 && slots > (int64_t)ctas * 32 * 256) ctas *= 2;
   const size_t smem = (size_t)(warps + 2) * (num_experts + 1) * sizeof(int);
-  e = cudaFuncSetAttribute(expert_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)((32 + 2) * (kMaxExperts + 1) * sizeof(int)));
+  static int smem_set[kMaxDevices];
+  e = allow_smem_once(expert_sort_kernel, (int)((32 + 2) * (kMaxExperts + 1) * sizeof(int)), device, smem_set);
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -96,7 +96,7 @@ int magi_swiglu_expert_sort(const void* ids, int ids_64bit, int64_t slots, int n
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(cuda_stream);
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, expert_sort_kernel, ids, ids_64bit, (int)slots, num_experts, (int*)row_slot, (int*)slot_row,
                          (int*)offsets, ctas);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_sort_kernel");

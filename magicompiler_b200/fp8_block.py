@@ -25,8 +25,9 @@ from typing import Optional
 import torch
 
 from . import _loader
+from .ops import _raw_stream
 from .register import magi_register_custom_op
-from .routed import BLOCK, FP8_MAX, SCALE_FLOOR, _device_stream, _raise, _result
+from .routed import BLOCK, FP8_MAX, SCALE_FLOOR, _check_device, _raise, _result
 
 GEMM_OP_NAME = "magi_swiglu::gemm_fp8_block"
 SWIGLU_OP_NAME = "magi_swiglu::gemm_swiglu_fp8_block"
@@ -74,10 +75,10 @@ def quantize_fp8_gate_up(w_gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.T
 
 
 def _check(name: str, a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
-           offsets: torch.Tensor | None, halves: int) -> tuple[int, int, int, int]:
+           offsets: torch.Tensor | None, halves: int) -> tuple[int, int, int, int, int]:
     for what, t, dtype in (("a", a, torch.float8_e4m3fn), ("a_scale", a_scale, torch.float32),
                            ("b", b, torch.float8_e4m3fn), ("b_scale", b_scale, torch.float32)):
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
             raise TypeError(f"{name}: {what} must be a {dtype} tensor; got {getattr(t, 'dtype', type(t))}")
     if a.dim() != 2 or a_scale.dim() != 2:
         raise ValueError(f"{name}: a and a_scale must be 2-D; got {tuple(a.shape)} and {tuple(a_scale.shape)}")
@@ -93,39 +94,39 @@ def _check(name: str, a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b
     elif b.dim() != 2:
         raise ValueError(f"{name}: without offsets the weight must be [rows, K]; got {tuple(b.shape)}")
     m, k = a.shape
-    if b.shape[-2] % halves:
-        raise ValueError(f"{name}: the weight has {b.shape[-2]} rows; it must hold N gate rows followed by N up rows")
-    n = b.shape[-2] // halves
-    if b.shape[-1] != k:
+    rows, kw = b.shape[-2:]
+    if rows % halves:
+        raise ValueError(f"{name}: the weight has {rows} rows; it must hold N gate rows followed by N up rows")
+    n = rows // halves
+    if kw != k:
         raise ValueError(f"{name}: inner dimensions differ: a {tuple(a.shape)}, weight {tuple(b.shape)}")
     if k == 0 or n == 0 or k % 16 or n % (8 * halves):
         raise ValueError(f"{name}: K ({k}) must be a positive multiple of 16 and N ({n}) of {8 * halves}")
-    kb, nb = -(-k // BLOCK), -(-n // BLOCK)
-    if tuple(a_scale.shape) != (m, kb):
+    kb, nb = (k + BLOCK - 1) // BLOCK, (n + BLOCK - 1) // BLOCK
+    if a_scale.shape != (m, kb):
         raise ValueError(f"{name}: a_scale must be [{m}, {kb}]; got {tuple(a_scale.shape)}")
-    want = (*((experts,) if offsets is not None else ()), halves * nb, kb)
-    if tuple(b_scale.shape) != want:
-        raise ValueError(f"{name}: the weight's scales must be {list(want)}; got {tuple(b_scale.shape)}")
+    if b_scale.shape != ((halves * nb, kb) if offsets is None else (experts, halves * nb, kb)):
+        raise ValueError(f"{name}: the weight's scales must be {[] if offsets is None else [experts]}{[halves * nb, kb]}; got {tuple(b_scale.shape)}")
     if not b.is_contiguous() or not b_scale.is_contiguous():
         raise ValueError(f"{name}: the weight and its scales must be contiguous (a copy on every call would double their traffic)")
-    tensors = [a, a_scale, b, b_scale] + ([offsets] if offsets is not None else [])
-    if not all(t.is_cuda for t in tensors):
-        raise TypeError(f"{name} runs on CUDA tensors only (there is no CPU implementation)")
-    if any(t.device != a.device for t in tensors):
-        raise ValueError(f"{name}: all operands must be on {a.device}")
+    if offsets is None:
+        dev = _check_device(name, a, a_scale, b, b_scale)
+    else:
+        dev = _check_device(name, a, a_scale, b, b_scale, offsets)
     if b.data_ptr() % 16:
         raise ValueError(f"{name}: the weight must be 16-byte aligned")
-    return m, n, k, experts
+    return m, n, k, experts, dev
 
 
 def _operand(a: torch.Tensor, a_scale: torch.Tensor) -> tuple[torch.Tensor, int, torch.Tensor, int]:
     """``a`` and its scales as the kernels read them (a copy if they cannot), with their row strides."""
     m, k = a.shape
-    if not (a.stride(1) == 1 and (m <= 1 or (a.stride(0) >= k and a.stride(0) % 16 == 0)) and a.data_ptr() % 16 == 0):
-        a = a.contiguous()
-        if a.data_ptr() % 16:  # contiguous() hands a contiguous view back as it is
+    if a.is_contiguous():
+        if a.data_ptr() % 16:
             a = a.clone()
-    if not (a_scale.stride(1) == 1 and (m <= 1 or a_scale.stride(0) >= a_scale.shape[1])):
+    elif not (a.stride(1) == 1 and a.stride(0) >= k and a.stride(0) % 16 == 0 and a.data_ptr() % 16 == 0):
+        a = a.contiguous()
+    if not (a_scale.is_contiguous() or (a_scale.stride(1) == 1 and a_scale.stride(0) >= a_scale.shape[1])):
         a_scale = a_scale.contiguous()
     return a, a.stride(0) if m > 1 else k, a_scale, a_scale.stride(0) if m > 1 else a_scale.shape[1]
 
@@ -133,15 +134,14 @@ def _operand(a: torch.Tensor, a_scale: torch.Tensor) -> tuple[torch.Tensor, int,
 def gemm_fp8_block_out(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
                        offsets: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """The body of ``gemm_fp8_block``.  With ``out`` the rows from ``offsets[E]`` on are left as they were."""
-    m, n, k, experts = _check("gemm_fp8_block", a, a_scale, b, b_scale, offsets, 1)
+    m, n, k, experts, dev = _check("gemm_fp8_block", a, a_scale, b, b_scale, offsets, 1)
     c = _result("gemm_fp8_block", out, (m, n), torch.bfloat16, a.device)
     if m == 0:
         return c
     a2, lda, s2, lds = _operand(a, a_scale)
-    dev, stream = _device_stream(a)
     rc = _loader.load_library().magi_swiglu_gemm_fp8_block(
         a2.data_ptr(), s2.data_ptr(), b.data_ptr(), b_scale.data_ptr(), offsets.data_ptr() if offsets is not None else None,
-        experts, c.data_ptr(), m, n, k, lda, lds, 0 if out is not None else 1, dev, stream)
+        experts, c.data_ptr(), m, n, k, lda, lds, 0 if out is not None else 1, dev, _raw_stream(dev))
     if rc != 0:
         _raise("gemm_fp8_block", rc)
     return c
@@ -164,18 +164,17 @@ def gemm_swiglu_fp8_block_out(a: torch.Tensor, a_scale: torch.Tensor, w_gate_up:
     """The body of ``gemm_swiglu_fp8_block``; ``out`` = (codes, scales), whose rows from ``offsets[E]`` on are left as they
     were."""
     name = "gemm_swiglu_fp8_block"
-    m, n, k, experts = _check(name, a, a_scale, w_gate_up, w_scale, offsets, 2)
+    m, n, k, experts, dev = _check(name, a, a_scale, w_gate_up, w_scale, offsets, 2)
     codes, scales = out if out is not None else (None, None)
     codes = _result(name, codes, (m, n), torch.float8_e4m3fn, a.device)
     scales = _result(name, scales, (m, -(-n // BLOCK)), torch.float32, a.device)
     if m == 0:
         return codes, scales
     a2, lda, s2, lds = _operand(a, a_scale)
-    dev, stream = _device_stream(a)
     rc = _loader.load_library().magi_swiglu_gemm_swiglu_fp8_block(
         a2.data_ptr(), s2.data_ptr(), w_gate_up.data_ptr(), w_scale.data_ptr(),
         offsets.data_ptr() if offsets is not None else None, experts, codes.data_ptr(), scales.data_ptr(), m, n, k, lda, lds,
-        0 if out is not None else 1, dev, stream)
+        0 if out is not None else 1, dev, _raw_stream(dev))
     if rc != 0:
         _raise(name, rc)
     return codes, scales

@@ -36,9 +36,9 @@ def _raise(name: str, rc: int) -> None:
     raise (ValueError(msg) if rc < 0 else RuntimeError(msg))
 
 
-def _device_stream(t: torch.Tensor) -> tuple[int, int]:
-    dev = t.device.index if t.device.index is not None else torch.cuda.current_device()
-    return dev, _raw_stream(dev)
+def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``t`` itself when the kernels can read it as it is (no view is made: a call's host time counts), else ``_rows_view``."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else _rows_view(t, cols)
 
 
 def _result(name: str, out: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype,
@@ -72,8 +72,7 @@ def expert_sort_out(expert_ids: torch.Tensor, num_experts: int,
         raise ValueError(f"expert_ids must be [tokens, choices]; got shape {tuple(expert_ids.shape)}")
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"num_experts must be in [1, {MAX_EXPERTS}]; got {num_experts}")
-    if not expert_ids.is_cuda:
-        raise TypeError("expert_sort runs on CUDA tensors only (there is no CPU implementation)")
+    dev = _check_device("expert_sort", expert_ids)
     ids = expert_ids.contiguous()
     slots, device = ids.numel(), ids.device
     if out is None:
@@ -84,10 +83,9 @@ def expert_sort_out(expert_ids: torch.Tensor, num_experts: int,
         row_slot = _result("expert_sort", out[0], (slots,), torch.int32, device)
         slot_row = _result("expert_sort", out[1], tuple(ids.shape), torch.int32, device)
         offsets = _result("expert_sort", out[2], (num_experts + 1,), torch.int32, device)
-    dev, stream = _device_stream(ids)
     rc = _loader.load_library().magi_swiglu_expert_sort(
         ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, slots, num_experts, row_slot.data_ptr(),
-        slot_row.data_ptr(), offsets.data_ptr(), dev, stream)
+        slot_row.data_ptr(), offsets.data_ptr(), dev, _raw_stream(dev))
     if rc != 0:
         _raise("expert_sort", rc)
     return row_slot, slot_row, offsets
@@ -104,7 +102,7 @@ def expert_sort(expert_ids: torch.Tensor, num_experts: int) -> tuple[torch.Tenso
 # ------------------------------------------------------------------------------------------------ checks shared below
 def _check_maps(name: str, row_slot: torch.Tensor, slot_row: torch.Tensor) -> tuple[int, int]:
     for what, t, dim in (("row_slot", row_slot, 1), ("slot_row", slot_row, 2)):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
             raise TypeError(f"{name}: {what} must be an int32 tensor (expert_sort returns it)")
         if t.dim() != dim or not t.is_contiguous():
             raise ValueError(f"{name}: {what} must be a contiguous {dim}-D tensor; got shape {tuple(t.shape)}")
@@ -124,12 +122,18 @@ def _check_rows(name: str, what: str, t: torch.Tensor, rows: int, multiple: int)
     return t.shape[1]
 
 
-def _check_device(name: str, first: torch.Tensor, *others: torch.Tensor) -> None:
-    if not all(t.is_cuda for t in (first, *others)):
-        raise TypeError(f"{name} runs on CUDA tensors only (there is no CPU implementation)")
+def _check_device(name: str, first: torch.Tensor, *others: torch.Tensor) -> int:
+    """The index of the one CUDA device that all operands are on."""
+    dev = first.get_device()  # -1 for a CPU tensor
     for t in others:
-        if t.device != first.device:
+        if t.get_device() != dev or dev < 0:
+            if dev < 0 or t.get_device() < 0:
+                break
             raise ValueError(f"{name}: operands are on {first.device} and {t.device}")
+    else:
+        if dev >= 0:
+            return dev
+    raise TypeError(f"{name} runs on CUDA tensors only (there is no CPU implementation)")
 
 
 def _check_weights(name: str, weights: torch.Tensor, tokens: int, k: int) -> None:
@@ -152,12 +156,11 @@ def expert_gather_out(x: torch.Tensor, row_slot: torch.Tensor, slot_row: torch.T
     """The body of ``expert_gather`` (no autograd)."""
     tokens, k = _check_maps("expert_gather", row_slot, slot_row)
     h = _check_rows("expert_gather", "x", x, tokens, 8)
-    _check_device("expert_gather", x, row_slot, slot_row)
-    x2 = _rows_view(x, h)
+    dev = _check_device("expert_gather", x, row_slot, slot_row)
+    x2 = _rows(x, h)
     xs = _result("expert_gather", out, (tokens * k, h), torch.bfloat16, x.device)
-    dev, stream = _device_stream(x)
     rc = _loader.load_library().magi_swiglu_expert_gather_bf16(
-        x2.data_ptr(), row_slot.data_ptr(), slot_row.data_ptr(), xs.data_ptr(), tokens, k, h, _ld(x2), dev, stream)
+        x2.data_ptr(), row_slot.data_ptr(), slot_row.data_ptr(), xs.data_ptr(), tokens, k, h, _ld(x2), dev, _raw_stream(dev))
     if rc != 0:
         _raise("expert_gather", rc)
     return xs
@@ -195,16 +198,15 @@ def expert_combine_out(y: torch.Tensor, weights: torch.Tensor | None, row_slot: 
     h = _check_rows("expert_combine", "y", y, tokens * k, 8)
     if weights is not None:
         _check_weights("expert_combine", weights, tokens, k)
-        _check_device("expert_combine", y, weights, row_slot, slot_row)
+        dev = _check_device("expert_combine", y, weights, row_slot, slot_row)
         weights = weights.contiguous()
     else:
-        _check_device("expert_combine", y, row_slot, slot_row)
-    y2 = _rows_view(y, h)
+        dev = _check_device("expert_combine", y, row_slot, slot_row)
+    y2 = _rows(y, h)
     res = _result("expert_combine", out, (tokens, h), torch.bfloat16, y.device)
-    dev, stream = _device_stream(y)
     rc = _loader.load_library().magi_swiglu_expert_combine_bf16(
         y2.data_ptr(), weights.data_ptr() if weights is not None else None, slot_row.data_ptr(), res.data_ptr(), tokens, k,
-        h, _ld(y2), dev, stream)
+        h, _ld(y2), dev, _raw_stream(dev))
     if rc != 0:
         _raise("expert_combine", rc)
     return res
@@ -227,14 +229,13 @@ def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor, weights: torch.
     if _check_rows(name, "y", y, tokens * k, 8) != h:
         raise ValueError(f"{name}: y {tuple(y.shape)} and dout {tuple(dout.shape)} differ in row length")
     _check_weights(name, weights, tokens, k)
-    _check_device(name, dout, y, weights, row_slot, slot_row)
-    d2, y2, w = _rows_view(dout, h), _rows_view(y, h), weights.contiguous()
+    dev = _check_device(name, dout, y, weights, row_slot, slot_row)
+    d2, y2, w = _rows(dout, h), _rows(y, h), weights.contiguous()
     dy = torch.empty((tokens * k, h) if need_dy else (0,), dtype=torch.bfloat16, device=y.device)
     dw = torch.empty((tokens, k) if need_dw else (0,), dtype=torch.float32, device=y.device)
-    dev, stream = _device_stream(dout)
     rc = _loader.load_library().magi_swiglu_expert_combine_backward_bf16(
         d2.data_ptr(), y2.data_ptr(), w.data_ptr(), row_slot.data_ptr(), slot_row.data_ptr(),
-        dy.data_ptr() if need_dy else None, dw.data_ptr() if need_dw else None, tokens, k, h, _ld(d2), _ld(y2), dev, stream)
+        dy.data_ptr() if need_dy else None, dw.data_ptr() if need_dw else None, tokens, k, h, _ld(d2), _ld(y2), dev, _raw_stream(dev))
     if rc != 0:
         _raise(name, rc)
     return dy, dw
@@ -284,12 +285,11 @@ def quantize_fp8_block_out(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tenso
                            ) -> tuple[torch.Tensor, torch.Tensor]:
     """The body of ``quantize_fp8_block``; ``out`` = (codes, scales) to write into."""
     cols = _check_rows("quantize_fp8_block", "x", x, x.shape[0] if isinstance(x, torch.Tensor) and x.dim() else 0, 16)
-    _check_device("quantize_fp8_block", x)
-    x2 = _rows_view(x, cols)
+    dev = _check_device("quantize_fp8_block", x)
+    x2 = _rows(x, cols)
     codes, scales = _fp8_block_outputs("quantize_fp8_block", out, x.shape[0], cols, x.device)
-    dev, stream = _device_stream(x)
     rc = _loader.load_library().magi_swiglu_quantize_fp8_block(
-        x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.shape[0], cols, _ld(x2), dev, stream)
+        x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.shape[0], cols, _ld(x2), dev, _raw_stream(dev))
     if rc != 0:
         _raise("quantize_fp8_block", rc)
     return codes, scales
@@ -311,13 +311,12 @@ def expert_gather_fp8_out(x: torch.Tensor, row_slot: torch.Tensor, slot_row: tor
     """The body of ``expert_gather_fp8``; ``out`` = (codes, scales) to write into."""
     tokens, k = _check_maps("expert_gather_fp8", row_slot, slot_row)
     cols = _check_rows("expert_gather_fp8", "x", x, tokens, 16)
-    _check_device("expert_gather_fp8", x, row_slot, slot_row)
-    x2 = _rows_view(x, cols)
+    dev = _check_device("expert_gather_fp8", x, row_slot, slot_row)
+    x2 = _rows(x, cols)
     codes, scales = _fp8_block_outputs("expert_gather_fp8", out, tokens * k, cols, x.device)
-    dev, stream = _device_stream(x)
     rc = _loader.load_library().magi_swiglu_expert_gather_fp8_block(
         x2.data_ptr(), row_slot.data_ptr(), slot_row.data_ptr(), codes.data_ptr(), scales.data_ptr(), tokens, k, cols,
-        _ld(x2), dev, stream)
+        _ld(x2), dev, _raw_stream(dev))
     if rc != 0:
         _raise("expert_gather_fp8", rc)
     return codes, scales
