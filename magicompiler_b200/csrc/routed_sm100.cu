@@ -80,10 +80,10 @@ int magi_swiglu_expert_sort(const void* ids, int ids_64bit, int64_t slots, int n
   int warps = (int)((slots + 127) / 128);
   warps = warps < 4 ? 4 : (warps > 32 ? 32 : warps);
   int ctas = 1;
-  while (ctas < 8 && slots > (int64_t)ctas * 32 * 256) ctas *= 2;
-  const size_t smem = (size_t)(warps + 2) * (num_experts + 1) * sizeof(int);
+  while (ctas < kSortCtas && slots > (int64_t)ctas * 32 * 256) ctas *= 2;
+  const size_t smem = (size_t)(warps + 3) * (num_experts + 1) * sizeof(int);
   static int smem_set[kMaxDevices];
-  e = allow_smem_once(expert_sort_kernel, (int)((32 + 2) * (kMaxExperts + 1) * sizeof(int)), device, smem_set);
+  e = allow_smem_once(expert_sort_kernel, (int)((32 + 3) * (kMaxExperts + 1) * sizeof(int)), device, smem_set);
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -132,14 +132,18 @@ int magi_swiglu_expert_combine_bf16(const void* y, const float* weights, const i
   if (unaligned(y, out)) return fail(MAGI_SWIGLU_ERR_ALIGN, "y and out must be 16-byte aligned");
   const DeviceInfo* di = nullptr;
   if (int rc = require_b200(device, &di)) return rc;
+  // eight loads in flight per thread, split between the token's rows and column pieces
+  const int pieces = k <= 1 ? 8 : (k <= 2 ? 4 : (k <= 4 ? 2 : 1));
   RowGrid g;
-  if (int rc = row_grid(T, H / 8, &g)) return rc;
+  if (int rc = row_grid(T, (H / 8 + pieces - 1) / pieces, &g)) return rc;
   DeviceGuard guard;
   cudaError_t e = guard.set(device);
   if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
-  expert_combine_kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
-      static_cast<const uint4*>(y), ldy / 8, weights, slot_row, static_cast<uint4*>(out), T, (int)k, (int)(H / 8),
-      g.col_chunks);
+  auto kernel = pieces == 8 ? expert_combine_kernel<1, 8> : pieces == 4 ? expert_combine_kernel<2, 4>
+                : pieces == 2 ? expert_combine_kernel<4, 2> : expert_combine_kernel<8, 1>;
+  kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(cuda_stream)>>>(static_cast<const uint4*>(y), ldy / 8, weights,
+                                                                         slot_row, static_cast<uint4*>(out), T, (int)k,
+                                                                         (int)(H / 8), g.col_chunks);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_combine_kernel");
 }

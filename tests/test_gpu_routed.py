@@ -256,6 +256,22 @@ def test_quantiser_of_every_bf16_value():
         assert torch.equal(scales, ws) and torch.equal(codes.float(), wc.float())
 
 
+def test_quantiser_of_every_pair_of_mantissas():
+    """The quotient x / s takes one correction step instead of a division: each of the 128 bf16 mantissas of x against each
+    of the 128 of the block's maximum, at every distance of exponents that gives a code other than zero, at scales near
+    both ends of the corrected range, in the middle and outside."""
+    mant = (1.0 + torch.arange(128) / 128.0).cuda()
+    for power in (-118, -100, -92, -91, 0, 100, 119, 126):
+        for down in range(1, 20):
+            x = torch.zeros(128, 256, device="cuda")
+            x[:, 0] = x[:, 128] = mant * 2.0 ** power
+            x[:, 1:128], x[:, 129] = mant[:127] * 2.0 ** (power - down), mant[127] * 2.0 ** (power - down)
+            x = x.to(BF)
+            codes, scales = mb.quantize_fp8_block(x)
+            wc, ws = plain_quantise(x)
+            assert torch.equal(scales, ws) and torch.equal(codes.float(), wc.float()), (power, down)
+
+
 def test_quantiser_of_special_values():
     x = rows_of(8, 256, 1)
     x[0, 3], x[1, 200], x[2, 5], x[3], x[4, :128] = float("nan"), float("inf"), float("-inf"), 0, 1e-40
