@@ -156,7 +156,7 @@ static int run(const Problem& p, int device, void* cuda_stream) {
   if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   // Tokens per tile of the stream kernel: enough for twice an expert's average share of the rows (shares are uneven), so
-  // that W is usually streamed once.  8 experts, 74 rows, N = 4096, K = 14336: 16 tokens a tile 86 us, 32 tokens XX us.
+  // that W is usually streamed once.  8 experts, 74 rows, N = 4096, K = 14336: 16 tokens a tile 86 us, 32 tokens 79 us.
   const int64_t share = p.args.offsets ? (2 * p.M + p.args.E - 1) / p.args.E : p.M;
   if (p.halves == 1) {
     if (share <= 16) return launch_stream<1, 16>(p, device, di->sm_count, stream);

@@ -25,10 +25,11 @@ constexpr float kScaleFloor = 1.17549435e-38f;  // 2^-126: a block of zeros (or 
 
 // ---------------------------------------------------------------- sort
 // Stable counting sort of the slots by expert, slots without an expert last.  One thread-block cluster does it in one
-// launch: each warp owns a contiguous range of slots and a histogram row; __match_any_sync ranks equal keys inside a
-// warp step, so ties keep slot order and no atomic decides anything.  The CTAs of the cluster read each other's totals
+// launch: each warp owns a contiguous range of slots and a histogram row; equal keys inside a warp step are ranked by lane,
+// so ties keep slot order and no atomic decides anything.  The CTAs of the cluster read each other's totals
 // through distributed shared memory.  hist: [warps][E + 1], total: [E + 1], start: [E + 1].
-constexpr int kSortCtas = 8;
+constexpr int kSortCtas = 16;  // more than the 8 every GPU has to offer: asked for, with 8 to fall back on
+constexpr int kSortKeep = 4;  // steps of 32 slots whose keys and matches a warp keeps between its two passes
 
 __device__ __forceinline__ int ld_cluster_s32(uint32_t cluster_addr) {
   int v;
@@ -37,15 +38,31 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t cluster_addr) {
 }
 
 __device__ __forceinline__ int slot_key(const void* ids, int wide, int s, int end, int E) {
-  if (s >= end) return -1;  // no slot: matches only other absent lanes
+  if (s >= end) return E + 1;  // no slot: equal to other absent lanes only
   const long long v = wide ? static_cast<const long long*>(ids)[s] : (long long)static_cast<const int*>(ids)[s];
   return (v >= 0 && v < E) ? (int)v : E;
+}
+
+// Lanes whose key (below 2^bits) equals mine: one vote per bit of the key.  (__match_any_sync walks the distinct keys one
+// by one: with 128 experts a step took about 500 cycles.)
+__device__ __forceinline__ unsigned equal_lanes(int key, int bits) {
+  unsigned m = 0xffffffffu;
+#pragma unroll
+  for (int b = 0; b < 11; ++b) {  // kMaxExperts + 1 has 11 bits
+    if (b >= bits) break;
+    const bool one = (key >> b) & 1;
+    const unsigned votes = __ballot_sync(0xffffffffu, one);
+    m &= one ? votes : ~votes;
+  }
+  return m;
 }
 
 __global__ void __launch_bounds__(1024, 1)
 expert_sort_kernel(const void* ids, int wide, int R, int E, int* row_slot, int* slot_row, int* offsets, int ctas) {
   extern __shared__ int sort_smem[];
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned lower = (1u << lane) - 1u;
+  const int bits = 32 - __clz(E + 1);
   const int buckets = E + 1;
   int* hist = sort_smem + warp * buckets;
   int* total = sort_smem + warps * buckets;
@@ -60,17 +77,27 @@ expert_sort_kernel(const void* ids, int wide, int R, int E, int* row_slot, int* 
   const int lo = (int)(first < R ? first : R), hi = (int)(first + share < R ? first + share : R);
 
   for (int i = threadIdx.x; i < warps * buckets; i += blockDim.x) sort_smem[i] = 0;
+  // the first steps' keys and matches stay in registers for the second pass
+  int key[kSortKeep];
+  unsigned same[kSortKeep];
+#pragma unroll
+  for (int i = 0; i < kSortKeep; ++i) key[i] = slot_key(ids, wide, lo + 32 * i + lane, hi, E);
   __syncthreads();
-  for (int b = lo; b < hi; b += 128) {
-    int key[4];
+  auto count = [&](int k, unsigned m) {  // the lowest lane of each group of equal keys
+    if (k <= E && (m & lower) == 0) hist[k] += __popc(m);
+    __syncwarp();
+  };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) key[i] = slot_key(ids, wide, b + 32 * i + lane, hi, E);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned same = __match_any_sync(0xffffffffu, key[i]);
-      if (key[i] >= 0 && (same & ((1u << lane) - 1u)) == 0) hist[key[i]] += __popc(same);
-      __syncwarp();
+  for (int i = 0; i < kSortKeep; ++i) {
+    same[i] = 0;
+    if (lo + 32 * i < hi) {
+      same[i] = equal_lanes(key[i], bits);
+      count(key[i], same[i]);
     }
+  }
+  for (int s = lo + 32 * kSortKeep; s < hi; s += 32) {
+    const int k = slot_key(ids, wide, s + lane, hi, E);
+    count(k, equal_lanes(k, bits));
   }
   __syncthreads();
   // histogram column e -> exclusive prefix over this CTA's warps, and the CTA's total
@@ -123,25 +150,23 @@ expert_sort_kernel(const void* ids, int wide, int R, int E, int* row_slot, int* 
     }
   }
   __syncthreads();
-  for (int b = lo; b < hi; b += 128) {
-    int key[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) key[i] = slot_key(ids, wide, b + 32 * i + lane, hi, E);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned same = __match_any_sync(0xffffffffu, key[i]);
-      const unsigned lower = same & ((1u << lane) - 1u);
-      const int base = key[i] >= 0 ? hist[key[i]] : 0;
-      __syncwarp();
-      if (key[i] >= 0) {
-        if (lower == 0) hist[key[i]] = base + __popc(same);
-        const int s = b + 32 * i + lane;
-        const int r = all[key[i]] + base + __popc(lower);
-        row_slot[r] = key[i] < E ? s : -1;
-        slot_row[s] = key[i] < E ? r : -1;
-      }
-      __syncwarp();
+  auto place = [&](int s, int k, unsigned m) {
+    const int base = k <= E ? hist[k] : 0;
+    __syncwarp();
+    if (k <= E) {
+      if ((m & lower) == 0) hist[k] = base + __popc(m);
+      const int r = all[k] + base + __popc(m & lower);
+      row_slot[r] = k < E ? s : -1;
+      slot_row[s] = k < E ? r : -1;
     }
+    __syncwarp();
+  };
+#pragma unroll
+  for (int i = 0; i < kSortKeep; ++i)
+    if (lo + 32 * i < hi) place(lo + 32 * i + lane, key[i], same[i]);
+  for (int s = lo + 32 * kSortKeep; s < hi; s += 32) {
+    const int k = slot_key(ids, wide, s + lane, hi, E);
+    place(s + lane, k, equal_lanes(k, bits));
   }
   if (ctas > 1) cluster_sync_all();  // nobody leaves while its totals may still be read
 }

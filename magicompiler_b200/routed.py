@@ -143,6 +143,12 @@ def _check_weights(name: str, weights: torch.Tensor, tokens: int, k: int) -> Non
         raise ValueError(f"{name}: weights must be [{tokens}, {k}]; got shape {tuple(weights.shape)}")
 
 
+def _eager(grad: torch.Tensor) -> bool:
+    """A plain backward step: nothing traces it and no graph of it is wanted, so the op's body may be called without the
+    dispatcher (which costs about as much host time as the rest of a call)."""
+    return type(grad) is torch.Tensor and not torch.is_grad_enabled() and not torch.compiler.is_compiling()
+
+
 def _ld(t2: torch.Tensor) -> int:
     return t2.stride(0) if t2.shape[0] > 1 else t2.shape[1]
 
@@ -172,7 +178,8 @@ def _gather_setup_context(ctx, inputs, output):
 
 def _gather_backward(ctx, grad):
     row_slot, slot_row = ctx.saved_tensors
-    return torch.ops.magi_swiglu.expert_combine(grad, None, row_slot, slot_row), None, None
+    combine = expert_combine_out if _eager(grad) else torch.ops.magi_swiglu.expert_combine
+    return combine(grad, None, row_slot, slot_row), None, None
 
 
 @magi_register_custom_op(
@@ -217,12 +224,8 @@ def _combine_backward_meta(dout, y, weights, row_slot, slot_row, need_dy, need_d
             y.new_empty(slot_row.shape if need_dw else (0,), dtype=torch.float32))
 
 
-@magi_register_custom_op(name=COMBINE_BWD_OP_NAME, mutates_args=(), infer_output_meta_fn=_combine_backward_meta)
-def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor, weights: torch.Tensor, row_slot: torch.Tensor,
-                            slot_row: torch.Tensor, need_dy: bool, need_dw: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """``dy[slot_row[t, j]] = weights[t, j] * dout[t]`` (zeros in rows without a slot) and
-    ``dw[t, j] = <dout[t], y[slot_row[t, j]]>`` in one pass (``magi_swiglu_expert_combine_backward_bf16``); the one that is
-    not needed comes back empty."""
+def _combine_backward_body(dout: torch.Tensor, y: torch.Tensor, weights: torch.Tensor, row_slot: torch.Tensor,
+                           slot_row: torch.Tensor, need_dy: bool, need_dw: bool) -> tuple[torch.Tensor, torch.Tensor]:
     name = "expert_combine_backward"
     tokens, k = _check_maps(name, row_slot, slot_row)
     h = _check_rows(name, "dout", dout, tokens, 8)
@@ -241,6 +244,15 @@ def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor, weights: torch.
     return dy, dw
 
 
+@magi_register_custom_op(name=COMBINE_BWD_OP_NAME, mutates_args=(), infer_output_meta_fn=_combine_backward_meta)
+def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor, weights: torch.Tensor, row_slot: torch.Tensor,
+                            slot_row: torch.Tensor, need_dy: bool, need_dw: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """``dy[slot_row[t, j]] = weights[t, j] * dout[t]`` (zeros in rows without a slot) and
+    ``dw[t, j] = <dout[t], y[slot_row[t, j]]>`` in one pass (``magi_swiglu_expert_combine_backward_bf16``); the one that is
+    not needed comes back empty."""
+    return _combine_backward_body(dout, y, weights, row_slot, slot_row, need_dy, need_dw)
+
+
 def _combine_setup_context(ctx, inputs, output):
     y, weights, row_slot, slot_row = inputs
     ctx.weighted = weights is not None
@@ -252,9 +264,11 @@ def _combine_setup_context(ctx, inputs, output):
 
 def _combine_backward(ctx, grad):
     if not ctx.weighted:
-        return torch.ops.magi_swiglu.expert_gather(grad, *ctx.saved_tensors), None, None, None
+        gather = expert_gather_out if _eager(grad) else torch.ops.magi_swiglu.expert_gather
+        return gather(grad, *ctx.saved_tensors), None, None, None
     need_dy, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    dy, dw = torch.ops.magi_swiglu.expert_combine_backward(grad, *ctx.saved_tensors, need_dy, need_dw)
+    backward = _combine_backward_body if _eager(grad) else torch.ops.magi_swiglu.expert_combine_backward
+    dy, dw = backward(grad, *ctx.saved_tensors, need_dy, need_dw)
     return dy if need_dy else None, dw if need_dw else None, None, None
 
 
