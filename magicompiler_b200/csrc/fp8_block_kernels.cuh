@@ -68,6 +68,7 @@ struct Args {
   int splits;             // CTAs of a cluster that share a tile's K blocks
   int stages;
   int zero_tail;          // rows from offsets[E] on: 1 = written as zeros, 0 = left alone
+  int band;               // row groups a raster band of the tile kernel
   int never;              // 0; a condition that the compiler cannot fold
 };
 
@@ -391,14 +392,13 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
 // half of W's, 32 KB per K block for 512 cycles of MMA.  A thread of the epilogue owns one row, so its scale is one number
 // per 128 columns and an addition is one fused multiply-add; with 128 of them per thread and block, two epilogue warps a
 // scheduler keep up with the MMA (half of the issue slots) and the registers for them come from the other warpgroup.
-// Persistent: tiles go round-robin to the pairs in bands of kBand row groups, column tile by column tile, so that the
+// Persistent: tiles go round-robin to the pairs in bands of row groups, column tile by column tile, so that the
 // pairs that run together share A rows and W rows in L2.
 constexpr int kTileThreads = 384;  // warps 0 TMA, 1 and 3 MMA, 2 tensor-memory allocator and scales; 4-11 epilogue
 constexpr int kTileRegs = 168;     // a thread's registers at launch: 384 * 168 = 64512 = 128 * 56 + 256 * 224
 constexpr int kTileRows = 256;     // rows of a pair
 constexpr int kTileStage = 2 * kWTile;
 constexpr int kTileStages = 6;
-constexpr int kBand = 8;
 constexpr int kMapExperts = 1024;
 constexpr int kScaleSlots = 4;     // ring of scale products, four K blocks a slot
 
@@ -488,9 +488,9 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 
   auto locate = [&](int t) {
     TileAt at;
-    const int band = t / (kBand * n_tiles), rem = t - band * kBand * n_tiles;
-    const int high = min(kBand, units - band * kBand);
-    const int unit = band * kBand + rem % high;
+    const int band = t / (a.band * n_tiles), rem = t - band * a.band * n_tiles;
+    const int high = min(a.band, units - band * a.band);
+    const int unit = band * a.band + rem % high;
     at.n0 = rem / high * kOutCols;
     int lo = 0, hi = a.E;  // unit_first[lo] <= unit < unit_first[hi]
     while (hi - lo > 1) {
@@ -515,12 +515,14 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       for (int t = pair; t < total && ok; t += pairs) {
         const TileAt at = locate(t);
         const int row = at.row0 + 128 * rank;
+        // a CTA whose rows all lie behind the expert's end brings no A rows; what the MMA reads instead is never used
+        const bool empty = row >= at.end, peer_empty = at.row0 + 128 >= at.end;
         const int wrow = kHalves == 1 ? at.n0 + 128 * rank : at.n0, whalf = kHalves == 1 ? at.e : at.e * 2 + rank;
         for (int kb = 0; kb < a.kb; ++kb) {
           if (!(ok = wait_bounded(empty_bar(stage), phase ^ 1u, &abort_flag, 1u, stage))) break;
-          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kTileStage);
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kTileStage - (peer_empty ? kWTile : 0));
           const uint32_t dst = tiles + stage * kTileStage;
-          tma_load_2d_pair_hint(dst, &tm_a, full0 + 8u * stage, kb * kBlk, row, keep);
+          if (!empty) tma_load_2d_pair_hint(dst, &tm_a, full0 + 8u * stage, kb * kBlk, row, keep);
           tma_load_3d_pair_hint(dst + kWTile, &tm_w, full0 + 8u * stage, kb * kBlk, wrow, whalf, normal);
           if (++stage == kTileStages) stage = 0, phase ^= 1u;
         }
@@ -614,6 +616,8 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       for (int i = 0; i < 64; ++i) sum[i] = 0;
       for (int kb = 0; kb < a.kb; kb += 4) {
         ok = __all_sync(0xffffffffu, ok && wait_bounded(scale_full(slot), slot_phase, &abort_flag, 3u, 32 + slot));
+        // a warp without rows only keeps the barriers going
+        const bool idle = tile_info[nth % kTileInfos].row0 + 128 * rank + 32 * q >= tile_info[nth % kTileInfos].end;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (kb + i >= a.kb) break;
@@ -623,6 +627,10 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
           ok = __all_sync(0xffffffffu, ok && wait_bounded(acc_full(buf), (it >> 1) & 1, &abort_flag, 3u, buf));
           ++it;
           if (!ok) continue;
+          if (idle) {
+            if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + 8u * buf);
+            continue;
+          }
           tc_fence_after_sync();
           const uint64_t s0 = pack_f32x2(f0, f0), s1 = pack_f32x2(f1, f1);
           const uint32_t from = lanes + buf * 256;

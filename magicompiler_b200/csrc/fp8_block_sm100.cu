@@ -144,7 +144,12 @@ static int launch_tiles(const Problem& p, int device, int sm_count, cudaStream_t
   if (pairs > most) pairs = (int)most;
   cfg.gridDim = dim3((unsigned)(2 * pairs));
   const int wide = ((uintptr_t)p.args.c & 31u) == 0 && p.N % 16 == 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_a, p.args, wide);
+  // A raster band of about 32 MB of A: it is read once per column tile and should stay in L2 beside the W rows that pass
+  // (8192 rows: K = 4096, N = 2 x 14336: bands of 8 / 16 / 32 groups 980 / 948 / 942 us; K = 14336: 447 / 451 / 468 us).
+  Args args = p.args;
+  const int64_t band = (32LL << 20) / (kTileRows * p.K);
+  args.band = (int)(band < 4 ? 4 : (band > 64 ? 64 : band));
+  e = cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_a, args, wide);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_tile_kernel");
 }
 
