@@ -56,6 +56,31 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, vola
   }
 }
 
+// The same for a whole warp whose lanes wait for different barriers at the same time: a wait takes about a hundred cycles
+// even when it is over, and waits one after the other add up on an MMA issuer's way.
+__device__ __forceinline__ bool wait_bounded_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned role,
+                                                 unsigned idx) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity) != 0)) return true;
+  const long long t0 = clock64();
+  unsigned spins = 0;
+  while (true) {
+    const bool here = mbar_try_wait(bar, parity) != 0;
+    if (__all_sync(0xffffffffu, here)) return true;
+    if ((++spins & 255u) == 0u) {
+      const bool late = clock64() - t0 > kWaitLimit;
+      if (late && !here) {
+        *abort_flag = 1;
+        if (atomicCAS(&g_fp8_watchdog[0], 0u, role) == 0u) {
+          g_fp8_watchdog[1] = blockIdx.x;
+          g_fp8_watchdog[2] = idx;
+          g_fp8_watchdog[3] = parity;
+        }
+      }
+      if (__any_sync(0xffffffffu, late || *abort_flag != 0)) return false;
+    }
+  }
+}
+
 struct Args {
   const float* a_scale;   // [R, kb] fp32, row stride ld_as
   const float* b_scale;   // [E][halves * nb][kb]
@@ -148,19 +173,21 @@ __device__ __forceinline__ void epilogue_sync(int threads) {  // named barrier o
 
 constexpr int kStreamThreads = 192;  // warps 0-3 epilogue (one tensor-memory lane quarter each), 4 TMA producer, 5 MMA issuer
 
-// Two CTAs share an SM where the sums of a thread leave the registers for it.
+// Two CTAs share an SM where the sums of a thread leave the registers for it.  kBufs accumulator buffers: a buffer's way
+// from the MMA through the epilogue and back takes about 700 cycles besides the MMA itself, and a block's MMAs only 200.
 template <int kHalves, int kTok>
 __global__ void __launch_bounds__(kStreamThreads, kHalves * kTok <= 64 ? 2 : 1)
 fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const Args a) {
   constexpr int kATile = kTok * kBlk;
   constexpr int kStage = kHalves * kWTile + kATile;
   constexpr int kAccCols = kHalves * kTok;
-  constexpr int kTmem = 2 * kAccCols < 32 ? 32 : 2 * kAccCols;
-  constexpr int kPiece = kTok < 32 ? kTok : 32;  // columns per tensor-memory load
-  constexpr int kScaleRow = kTok + 4;            // token scales of one K block, then the weights' scales of the halves
+  constexpr int kBufs = 4;
+  constexpr int kTmem = kBufs * kAccCols;
+  constexpr int kPiece = kAccCols < 32 ? kAccCols : 32;  // columns per tensor-memory load
+  constexpr int kStep = kAccCols < 64 ? kAccCols : 64;   // columns loaded before their arithmetic
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(16) float ring[2][4][kScaleRow];
-  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 4];
+  __shared__ __align__(16) float ring[2][4][kAccCols];  // as * bs of four K blocks: every column of both halves
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kBufs];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ Unit unit_slot;
@@ -171,7 +198,7 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
   auto acc_full = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
-  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 2 + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + kBufs + b); };
   const int split = a.splits > 1 ? (int)cluster_ctarank() : 0;
   const int n0 = (int)(blockIdx.x / a.splits) * kRowsW;
 
@@ -185,7 +212,7 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBufs; ++b) {
       mbar_init(acc_full(b), 1);
       mbar_init(acc_empty(b), 4);
     }
@@ -220,99 +247,109 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
       tma_load_2d_hint(dst + kHalves * kWTile, &tm_a, full_bar(stage), kb * kBlk, u.row0, keep);
       if (++stage == a.stages) stage = 0, phase ^= 1u;
     }
-  } else if (live && warp == 5 && lane == 0) {
+  } else if (live && warp == 5) {
     // ------------------------------------------------------------ MMA issuer
     const uint32_t idesc = umma_idesc_e4m3(kRowsW, kTok);
     int stage = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      const int buf = (kb - kb0) & 1;
-      const uint32_t buf_phase = ((kb - kb0) >> 1) & 1;
-      if (!wait_bounded(acc_empty(buf), buf_phase ^ 1u, &abort_flag, 2u, 16 + buf)) break;
-      if (!wait_bounded(full_bar(stage), phase, &abort_flag, 2u, stage)) break;
+      const int buf = (kb - kb0) % kBufs;
+      if (!wait_bounded_all(lane == 0 ? full_bar(stage) : acc_empty(buf), lane == 0 ? phase : (((kb - kb0) / kBufs) & 1) ^ 1u,
+                            &abort_flag, 2u, lane == 0 ? stage : 16 + buf))
+        break;
       tc_fence_after_sync();
-      const uint32_t src = tiles + stage * kStage;
-      const uint64_t tok = umma_desc_k_sw128(src + kHalves * kWTile);
+      if (lane == 0) {
+        const uint32_t src = tiles + stage * kStage;
+        const uint64_t tok = umma_desc_k_sw128(src + kHalves * kWTile);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const uint64_t w = umma_desc_k_sw128(src + h * kWTile);
+        for (int h = 0; h < kHalves; ++h) {
+          const uint64_t w = umma_desc_k_sw128(src + h * kWTile);
 #pragma unroll
-        for (int i = 0; i < kBlk / 32; ++i)
-          umma_fp8<1>(tmem + buf * kAccCols + h * kTok, w + 2 * i, tok + 2 * i, idesc, i > 0);
+          for (int i = 0; i < kBlk / 32; ++i)
+            umma_fp8<1>(tmem + buf * kAccCols + h * kTok, w + 2 * i, tok + 2 * i, idesc, i > 0);
+        }
+        umma_commit<1>(acc_full(buf));
+        umma_commit<1>(empty_bar(stage));
       }
-      umma_commit<1>(empty_bar(stage));
-      umma_commit<1>(acc_full(buf));
+      __syncwarp();
       if (++stage == a.stages) stage = 0, phase ^= 1u;
     }
   } else if (live && warp < 4) {
     // ------------------------------------------------------------ scale and add (one row of W per thread)
-    float acc[kHalves][kTok];
+    uint64_t sum[kAccCols / 2];  // pairs of neighbouring columns
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-      for (int c = 0; c < kTok; ++c) acc[h][c] = 0.0f;
-    // Scales travel four K blocks at a time: a prefetch into registers, then into one half of a shared ring.
+    for (int c = 0; c < kAccCols / 2; ++c) sum[c] = 0;
+    // Scales travel four K blocks at a time: a prefetch into registers, then their products into half of a shared ring.
     constexpr int kLoads = (4 * kTok + 127) / 128;
-    float next[kLoads], next_w = 0.0f;
+    float next[kLoads], next_w[kHalves];
     const float* ws = a.b_scale + ((long long)u.e * kHalves * a.nb + n0 / kBlk) * a.kb;
-    auto fetch = [&](int kb) {
+    auto fetch = [&](int kb) {  // thread i holds token i / 4 (and every 32nd after it) at K block kb + i % 4
+      const int b = kb + (threadIdx.x & 3);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int idx = threadIdx.x + 128 * i, c = idx >> 2, b = kb + (idx & 3);
+        const int c = (threadIdx.x >> 2) + 32 * i;
         next[i] = (c < u.rows && c < kTok && b < kb1) ? __ldg(a.a_scale + (long long)(u.row0 + c) * a.ld_as + b) : 0.0f;
       }
-      if (threadIdx.x < 4 * kHalves) {
-        const int b = kb + (threadIdx.x & 3), h = threadIdx.x >> 2;
-        next_w = b < kb1 ? __ldg(ws + (long long)h * a.nb * a.kb + b) : 0.0f;
-      }
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) next_w[h] = b < kb1 ? __ldg(ws + (long long)h * a.nb * a.kb + b) : 0.0f;
     };
     fetch(kb0);
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
     bool ok = true;
+    int never = a.never;
     for (int kb = kb0; kb < kb1; ++kb) {
-      const int i = kb - kb0, half = (i >> 2) & 1, buf = i & 1;
+      const int i = kb - kb0, half = (i >> 2) & 1, buf = i % kBufs;
       if ((i & 3) == 0) {
         // everyone is past the previous four blocks, so the other half of the ring is free
 #pragma unroll
         for (int q = 0; q < kLoads; ++q) {
-          const int idx = threadIdx.x + 128 * q;
-          if ((idx >> 2) < kTok) ring[half][idx & 3][idx >> 2] = next[q];
+          const int c = (threadIdx.x >> 2) + 32 * q;
+          if (c < kTok)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) ring[half][threadIdx.x & 3][h * kTok + c] = next[q] * next_w[h];
         }
-        if (threadIdx.x < 4 * kHalves) ring[half][threadIdx.x & 3][kTok + (threadIdx.x >> 2)] = next_w;
         epilogue_sync(128);
         fetch(kb + 4);
       }
-      const float* sc = ring[half][i & 3];
       // a wait that gave up skips the work but not the barrier above, which the other warps are counting on
-      ok = __all_sync(0xffffffffu, ok && wait_bounded(acc_full(buf), (i >> 1) & 1, &abort_flag, 3u, buf));
+      ok = __all_sync(0xffffffffu, ok && wait_bounded(acc_full(buf), (i / kBufs) & 1, &abort_flag, 3u, buf));
       if (!ok) continue;
       tc_fence_after_sync();
+      const uint32_t sc = smem_u32(ring[half][i & 3]);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const float w = sc[kTok + h];
+      for (int c0 = 0; c0 < kAccCols; c0 += kStep) {
+        uint32_t p[kStep / kPiece][32];
 #pragma unroll
-        for (int c0 = 0; c0 < kTok; c0 += kPiece) {
-          uint32_t p[32];
+        for (int j = 0; j < kStep / kPiece; ++j) {
           if constexpr (kPiece == 32)
-            tmem_ld_x32(lane_base + buf * kAccCols + h * kTok + c0, p);
+            tmem_ld_x32(lane_base + buf * kAccCols + c0 + 32 * j, p[j]);
           else
-            tmem_ld_x16_into32(lane_base + buf * kAccCols + h * kTok + c0, p);
-          tmem_ld_wait();
-          tmem_regs_ready(p);
+            tmem_ld_x16_into32(lane_base + buf * kAccCols + c0, p[j]);
+        }
+        tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < kPiece; c += 4) {
-            const float4 t = *reinterpret_cast<const float4*>(sc + c0 + c);
-            acc[h][c0 + c] = fmaf(__uint_as_float(p[c]), w * t.x, acc[h][c0 + c]);
-            acc[h][c0 + c + 1] = fmaf(__uint_as_float(p[c + 1]), w * t.y, acc[h][c0 + c + 1]);
-            acc[h][c0 + c + 2] = fmaf(__uint_as_float(p[c + 2]), w * t.z, acc[h][c0 + c + 2]);
-            acc[h][c0 + c + 3] = fmaf(__uint_as_float(p[c + 3]), w * t.w, acc[h][c0 + c + 3]);
-          }
+        for (int j = 0; j < kStep / kPiece; ++j) tmem_regs_ready(p[j]);
+        if (c0 + kStep >= kAccCols) {  // the last columns have been read: the buffer goes back before the arithmetic
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_relaxed(acc_empty(buf));
+          asm volatile("" : "+r"(never));  // see the tile kernel
+          if (never) break;
+        }
+#pragma unroll
+        for (int c = 0; c < kStep; c += 4) {
+          const uint32_t* v = p[c / kPiece] + c % kPiece;
+          const float4 t = ld_shared_f4(sc + (c0 + c) * 4);
+          fma_f32x2(sum[(c0 + c) / 2], v[0], v[1], pack_f32x2(t.x, t.y));
+          fma_f32x2(sum[(c0 + c) / 2 + 1], v[2], v[3], pack_f32x2(t.z, t.w));
         }
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_relaxed(acc_empty(buf));
     }
+    float acc[kHalves][kTok];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int c = 0; c < kTok; c += 2) unpack_f32x2(sum[(h * kTok + c) / 2], acc[h][c], acc[h][c + 1]);
     // Every MMA of this CTA is complete, so the stages are free: the sums go there as [token][half][128], which is
     // conflict-free here and gives the writer below a token's 128 columns in a row.
     const uint32_t mine = tiles + (warp * 32 + lane) * 4;
@@ -529,9 +566,8 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       }
     } else if ((warp == 1 || warp == 3) && rank == 0) {
       // ---------------------------------------------------------- MMA issuers: warp 1 the even K blocks, warp 3 the odd
-      // ones, each with a buffer of its own.  A wait costs about a hundred cycles even when it is over, and issuing four
-      // MMAs holds a thread until the tensor pipe has taken them; two issuers do their waits in each other's shadow, and
-      // lanes 0 and 1 of each wait for operands and buffer at the same time.
+      // ones, each with a buffer of its own.  Issuing four MMAs holds a thread until the tensor pipe has taken them, so two
+      // issuers do their waits in each other's shadow; lane 0 waits for the operands while the others wait for the buffer.
       const uint32_t idesc = umma_idesc_e4m3(256, 256);
       const int buf = warp >> 1;
       int it = 0, stage = 0;
@@ -540,9 +576,9 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       for (int t = pair; t < total && ok; t += pairs)
         for (int kb = 0; kb < a.kb; ++kb, ++it) {
           if ((it & 1) == buf) {
-            if (lane == 0) ok = wait_bounded(full_bar(stage), phase, &abort_flag, 2u, stage);
-            if (lane == 1) ok = wait_bounded(acc_empty(buf), ((it >> 1) & 1) ^ 1u, &abort_flag, 2u, 16 + buf);
-            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            ok = wait_bounded_all(lane == 0 ? full_bar(stage) : acc_empty(buf), lane == 0 ? phase : ((it >> 1) & 1) ^ 1u,
+                                  &abort_flag, 2u, lane == 0 ? stage : 16 + buf);
+            if (!ok) break;
             tc_fence_after_sync();
             if (lane == 0) {
               const uint64_t da = umma_desc_k_sw128(tiles + stage * kTileStage);
