@@ -10,7 +10,7 @@
 // so every K block of 128 is finished in tensor memory, read back, scaled and added to fp32 registers.  Two accumulator
 // buffers in tensor memory let the MMAs of the next block run meanwhile.
 //
-// fp8_block_stream_kernel: W's rows are the MMA's 128 rows ("M") and the tokens are its columns ("N", 16..128), so few
+// fp8_block_stream_kernel: W's rows are the MMA's 128 rows ("M") and the tokens are its columns ("N", 16..64), so few
 // tokens cost few MMA columns and few additions, and the kernel is a stream over W.  A CTA owns 128 output columns (128
 // gate rows and 128 up rows of W in the SwiGLU form) of up to kTok rows of one expert.
 #pragma once
@@ -90,7 +90,7 @@ struct Args {
   float* scales;          // SwiGLU: [R, nb]
   long long ld_as;
   int R, N, E, kb, nb;    // nb = ceil(N / 128)
-  int splits;             // CTAs of a cluster that share a tile's K blocks
+  int splits;             // CTAs (tile kernel: CTA pairs) of a cluster that share a tile's K blocks
   int stages;
   int zero_tail;          // rows from offsets[E] on: 1 = written as zeros, 0 = left alone
   int band;               // row groups a raster band of the tile kernel
@@ -164,6 +164,9 @@ __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
 __device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
   asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
@@ -173,10 +176,11 @@ __device__ __forceinline__ void epilogue_sync(int threads) {  // named barrier o
 
 constexpr int kStreamThreads = 192;  // warps 0-3 epilogue (one tensor-memory lane quarter each), 4 TMA producer, 5 MMA issuer
 
-// Two CTAs share an SM where the sums of a thread leave the registers for it.  kBufs accumulator buffers: a buffer's way
-// from the MMA through the epilogue and back takes about 700 cycles besides the MMA itself, and a block's MMAs only 200.
+// kTok 16, 32 or (plain) 64 tokens a tile: two CTAs share an SM.  (Tiles of 64 tokens in the SwiGLU form and of 128 in the
+// plain one leave registers for one CTA an SM only and lost to the smaller ones everywhere.)  kBufs accumulator buffers: a
+// buffer's way from the MMA through the epilogue and back takes about 700 cycles besides the MMA itself, which takes 400.
 template <int kHalves, int kTok>
-__global__ void __launch_bounds__(kStreamThreads, kHalves * kTok <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(kStreamThreads, 2)
 fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const Args a) {
   constexpr int kATile = kTok * kBlk;
   constexpr int kStage = kHalves * kWTile + kATile;
@@ -184,7 +188,6 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
   constexpr int kBufs = 4;
   constexpr int kTmem = kBufs * kAccCols;
   constexpr int kPiece = kAccCols < 32 ? kAccCols : 32;  // columns per tensor-memory load
-  constexpr int kStep = kAccCols < 64 ? kAccCols : 64;   // columns loaded before their arithmetic
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(16) float ring[2][4][kAccCols];  // as * bs of four K blocks: every column of both halves
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kBufs];
@@ -316,33 +319,28 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
       if (!ok) continue;
       tc_fence_after_sync();
       const uint32_t sc = smem_u32(ring[half][i & 3]);
+      uint32_t p[kAccCols / kPiece][32];
 #pragma unroll
-      for (int c0 = 0; c0 < kAccCols; c0 += kStep) {
-        uint32_t p[kStep / kPiece][32];
+      for (int j = 0; j < kAccCols / kPiece; ++j) {
+        if constexpr (kPiece == 32)
+          tmem_ld_x32(lane_base + buf * kAccCols + 32 * j, p[j]);
+        else
+          tmem_ld_x16_into32(lane_base + buf * kAccCols, p[j]);
+      }
+      tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < kStep / kPiece; ++j) {
-          if constexpr (kPiece == 32)
-            tmem_ld_x32(lane_base + buf * kAccCols + c0 + 32 * j, p[j]);
-          else
-            tmem_ld_x16_into32(lane_base + buf * kAccCols + c0, p[j]);
-        }
-        tmem_ld_wait();
+      for (int j = 0; j < kAccCols / kPiece; ++j) tmem_regs_ready(p[j]);
+      tc_fence_before_sync();  // all columns have been read: the buffer goes back before the arithmetic
+      __syncwarp();
+      if (lane == 0) mbar_arrive_relaxed(acc_empty(buf));
+      asm volatile("" : "+r"(never));  // see the tile kernel
+      if (never) break;
 #pragma unroll
-        for (int j = 0; j < kStep / kPiece; ++j) tmem_regs_ready(p[j]);
-        if (c0 + kStep >= kAccCols) {  // the last columns have been read: the buffer goes back before the arithmetic
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_relaxed(acc_empty(buf));
-          asm volatile("" : "+r"(never));  // see the tile kernel
-          if (never) break;
-        }
-#pragma unroll
-        for (int c = 0; c < kStep; c += 4) {
-          const uint32_t* v = p[c / kPiece] + c % kPiece;
-          const float4 t = ld_shared_f4(sc + (c0 + c) * 4);
-          fma_f32x2(sum[(c0 + c) / 2], v[0], v[1], pack_f32x2(t.x, t.y));
-          fma_f32x2(sum[(c0 + c) / 2 + 1], v[2], v[3], pack_f32x2(t.z, t.w));
-        }
+      for (int c = 0; c < kAccCols; c += 4) {
+        const uint32_t* v = p[c / kPiece] + c % kPiece;
+        const float4 t = ld_shared_f4(sc + c * 4);
+        fma_f32x2(sum[c / 2], v[0], v[1], pack_f32x2(t.x, t.y));
+        fma_f32x2(sum[c / 2 + 1], v[2], v[3], pack_f32x2(t.z, t.w));
       }
     }
     float acc[kHalves][kTok];
@@ -431,11 +429,15 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
 // scheduler keep up with the MMA (half of the issue slots) and the registers for them come from the other warpgroup.
 // Persistent: tiles go round-robin to the pairs in bands of row groups, column tile by column tile, so that the
 // pairs that run together share A rows and W rows in L2.
+// Few tiles: `splits` (2 or 4) pairs form a cluster and share a tile's K blocks.  At the end each pair keeps the rows of
+// 4 / splits lane quarters, sends the sums of the others to the pairs that keep those (distributed shared memory, into the
+// stages, which are free by then) and adds what it receives in the order of the splits.  One tile a cluster.
 constexpr int kTileThreads = 384;  // warps 0 TMA, 1 and 3 MMA, 2 tensor-memory allocator and scales; 4-11 epilogue
 constexpr int kTileRegs = 168;     // a thread's registers at launch: 384 * 168 = 64512 = 128 * 56 + 256 * 224
 constexpr int kTileRows = 256;     // rows of a pair
 constexpr int kTileStage = 2 * kWTile;
 constexpr int kTileStages = 6;
+constexpr int kTileSmem = kTileStages * kTileStage + 1024;
 constexpr int kMapExperts = 1024;
 constexpr int kScaleSlots = 4;     // ring of scale products, four K blocks a slot
 
@@ -459,8 +461,12 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   __shared__ int abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();  // rank 0 issues the pair's MMAs
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int cluster_rank = (int)cluster_ctarank();
+  const int rank = cluster_rank & 1, split = cluster_rank >> 1;  // rank 0 issues the pair's MMAs
+  const uint32_t leader = cluster_rank & ~1;
+  const uint16_t both = (uint16_t)(3u << leader);
+  const int pair = blockIdx.x / (2 * a.splits), pairs = gridDim.x / (2 * a.splits);  // pairs, or clusters of them
+  const int kb0 = (int)((long long)a.kb * split / a.splits), kb1 = (int)((long long)a.kb * (split + 1) / a.splits);
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -545,7 +551,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- TMA producer (each CTA its own halves)
       const uint64_t keep = l2_policy_evict_last(), normal = l2_policy_evict_normal();
-      const uint32_t full0 = map_to_cta(full_bar(0), 0);  // the bytes of both CTAs are counted on rank 0's barrier
+      const uint32_t full0 = map_to_cta(full_bar(0), leader);  // the bytes of both CTAs are counted on rank 0's barrier
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -555,7 +561,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
         // a CTA whose rows all lie behind the expert's end brings no A rows; what the MMA reads instead is never used
         const bool empty = row >= at.end, peer_empty = at.row0 + 128 >= at.end;
         const int wrow = kHalves == 1 ? at.n0 + 128 * rank : at.n0, whalf = kHalves == 1 ? at.e : at.e * 2 + rank;
-        for (int kb = 0; kb < a.kb; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = wait_bounded(empty_bar(stage), phase ^ 1u, &abort_flag, 1u, stage))) break;
           if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kTileStage - (peer_empty ? kWTile : 0));
           const uint32_t dst = tiles + stage * kTileStage;
@@ -574,7 +580,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; t < total && ok; t += pairs)
-        for (int kb = 0; kb < a.kb; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           if ((it & 1) == buf) {
             ok = wait_bounded_all(lane == 0 ? full_bar(stage) : acc_empty(buf), lane == 0 ? phase : ((it >> 1) & 1) ^ 1u,
                                   &abort_flag, 2u, lane == 0 ? stage : 16 + buf);
@@ -585,8 +591,8 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
               const uint64_t dw = umma_desc_k_sw128(tiles + stage * kTileStage + kWTile);
 #pragma unroll
               for (int i = 0; i < kBlk / 32; ++i) umma_fp8<2>(tmem + buf * 256, da + 2 * i, dw + 2 * i, idesc, i > 0);
-              umma_commit<2>(acc_full(buf));
-              umma_commit<2>(empty_bar(stage));
+              umma_commit<2>(acc_full(buf), both);
+              umma_commit<2>(empty_bar(stage), both);
             }
             __syncwarp();
           }
@@ -606,11 +612,11 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           rows[i] = a.a_scale + (long long)min(at.row0 + 128 * rank + 32 * i + lane, at.end - 1) * a.ld_as;
-        for (int kb = 0; kb < a.kb; kb += 4) {
+        for (int kb = kb0; kb < kb1; kb += 4) {
           if (!(ok = __all_sync(0xffffffffu, wait_bounded(scale_empty(slot), phase ^ 1u, &abort_flag, 4u, slot)))) break;
 #pragma unroll
           for (int b = 0; b < 4; b += 2) {
-            const int k0 = min(kb + b, a.kb - 1), k1 = min(kb + b + 1, a.kb - 1);
+            const int k0 = min(kb + b, kb1 - 1), k1 = min(kb + b + 1, kb1 - 1);
             float r0[4], r1[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) r0[i] = __ldg(rows[i] + k0), r1[i] = __ldg(rows[i] + k1);
@@ -625,12 +631,17 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
           }
           __syncwarp();
           if (lane == 0) {
-            if (kb == 0) tile_info[nth % kTileInfos] = at;
+            if (kb == kb0) tile_info[nth % kTileInfos] = at;
             mbar_arrive(scale_full(slot));
           }
           if (++slot == kScaleSlots) slot = 0, phase ^= 1u;
         }
       }
+    }
+    __syncwarp();
+    if (a.splits > 1 && pair < total) {  // the two barriers of the epilogue's exchange
+      cluster_sync_all();
+      cluster_sync_all();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
@@ -638,7 +649,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     const int q = warp & 3, part = (warp - 4) >> 2;  // lane quarter; which half of the columns
     const int my_row = 128 * rank + 32 * q + lane;
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
-    const uint32_t acc_empty0 = map_to_cta(acc_empty(0), 0);
+    const uint32_t acc_empty0 = map_to_cta(acc_empty(0), leader);
     // plain: 128 columns of one block of W; SwiGLU: 64 gate columns, then the 64 up columns that meet them
     const int col[4] = {kHalves == 1 ? 128 * part : 64 * part, kHalves == 1 ? 128 * part + 32 : 64 * part + 32,
                         kHalves == 1 ? 128 * part + 64 : 128 + 64 * part, kHalves == 1 ? 128 * part + 96 : 160 + 64 * part};
@@ -650,13 +661,13 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       uint64_t sum[64];  // pairs of neighbouring columns
 #pragma unroll
       for (int i = 0; i < 64; ++i) sum[i] = 0;
-      for (int kb = 0; kb < a.kb; kb += 4) {
+      for (int kb = kb0; kb < kb1; kb += 4) {
         ok = __all_sync(0xffffffffu, ok && wait_bounded(scale_full(slot), slot_phase, &abort_flag, 3u, 32 + slot));
         // a warp without rows only keeps the barriers going
         const bool idle = tile_info[nth % kTileInfos].row0 + 128 * rank + 32 * q >= tile_info[nth % kTileInfos].end;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (kb + i >= a.kb) break;
+          if (kb + i >= kb1) break;
           const float f0 = scale_ring[slot][i][kHalves == 1 ? part : 0][32 * q + lane];
           const float f1 = kHalves == 1 ? f0 : scale_ring[slot][i][1][32 * q + lane];
           const int buf = it & 1;
@@ -707,8 +718,33 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 64; ++i) unpack_f32x2(sum[i], acc[2 * i], acc[2 * i + 1]);
+      bool keeps = true;
+      if (a.splits > 1) {
+        const int per = 4 / a.splits, keeper = q / per;  // lane quarters a pair keeps; which pair keeps this one
+        keeps = split == keeper;
+        // [sender][warp of the keeper][32 x 16 bytes][lane]
+        const uint32_t slab = (uint32_t)((q % per) * 2 + part) * 16384u + lane * 16u;
+        cluster_sync_all();  // every MMA of the cluster is complete: the stages are free
+        if (!keeps) {
+          const uint32_t sender = (uint32_t)(split < keeper ? split : split - 1) * (uint32_t)(per * 2) * 16384u;
+          const uint32_t dst = map_to_cta(tiles + sender + slab, 2 * keeper + rank);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            st_cluster_v4(dst + i * 512, acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+        }
+        cluster_sync_all();
+        if (keeps)
+          for (int s = 0; s < a.splits - 1; ++s) {
+            const uint32_t src = tiles + (uint32_t)s * (uint32_t)(per * 2) * 16384u + slab;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float4 v = ld_shared_f4(src + i * 512);
+              acc[4 * i] += v.x, acc[4 * i + 1] += v.y, acc[4 * i + 2] += v.z, acc[4 * i + 3] += v.w;
+            }
+          }
+      }
       const long long row = at.row0 + my_row;
-      const bool here = ok && row < at.end;
+      const bool here = ok && keeps && row < at.end;
       if constexpr (kHalves == 1) {
         const int n = at.n0 + 128 * part;
         __nv_bfloat16* dst = a.c + row * a.N + n;

@@ -1,5 +1,6 @@
 // C ABI of the block-scaled fp8 products (include/magi_swiglu.h): argument checks, tile choice, tensor maps, launches.
 // Device code lives in fp8_block_kernels.cuh.
+#include <cmath>
 #include <cstring>
 
 #include "fp8_block_kernels.cuh"
@@ -40,11 +41,21 @@ struct Problem {
   Args args;
 };
 
+// Row groups of `rows` rows: every expert adds at most one partial group.
+static int64_t most_groups(const Problem& p, int rows) {
+  return p.args.offsets ? p.M / rows + (p.M < p.args.E + 1 ? p.M : p.args.E + 1) : (p.M + rows - 1) / rows;
+}
+// What to expect of them: experts' shares are uneven, so half a group more than the average share needs.
+static double expected_groups(const Problem& p, int rows) {
+  if (!p.args.offsets) return (double)((p.M + rows - 1) / rows);
+  const double used = (double)(p.M < p.args.E ? p.M : p.args.E), each = p.M / used / rows + 0.5;
+  return used * (each < 1.0 ? 1.0 : each);
+}
+
 template <int kHalves, int kTok>
-static int launch_stream(const Problem& p, int device, int sm_count, cudaStream_t stream) {
+static int launch_stream(const Problem& p, int device, int splits, cudaStream_t stream) {
   constexpr int kStage = kHalves * kWTile + kTok * kBlk;
-  constexpr int kBudget = kHalves * kTok <= 64 ? 108 * 1024 : 216 * 1024;  // two CTAs an SM, or one
-  constexpr int kFit = (kBudget - 1024) / kStage;
+  constexpr int kFit = (108 * 1024 - 1024) / kStage;  // two CTAs an SM
   constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
   static_assert(kStages >= 2 && kStages * kStage >= kTok * kHalves * 512, "stages hold the sums of a tile");
   const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.args.E * kHalves};
@@ -56,17 +67,11 @@ static int launch_stream(const Problem& p, int device, int sm_count, cudaStream_
   CUtensorMap tm_w, tm_a;
   if (int rc = encode_bytes_map(p.b, 3, wd, wst, wb, &tm_w, "B")) return rc;
   if (int rc = encode_bytes_map(p.a, 2, ad, ast, ab, &tm_a, "A")) return rc;
-  const int64_t n_tiles = (p.N + kRowsW - 1) / kRowsW;
-  // every expert adds at most one partial group of rows
-  const int64_t groups = p.args.offsets ? p.M / kTok + (p.M < p.args.E + 1 ? p.M : p.args.E + 1) : (p.M + kTok - 1) / kTok;
+  const int64_t n_tiles = (p.N + kRowsW - 1) / kRowsW, groups = most_groups(p, kTok);
   if (groups > 65535 || n_tiles > 0x7fffffffLL / 8)
     return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld rows are too many for one launch", (long long)p.M);
   Args args = p.args;
-  // Few tiles leave SMs idle: then up to eight CTAs of a cluster share a tile's K blocks (at least four each) and add
-  // their sums through distributed shared memory, until there are about two CTAs an SM.
-  const int64_t busy = n_tiles * (p.args.offsets ? (p.M < p.args.E ? p.M : p.args.E) : groups);
-  args.splits = 1;
-  while (args.splits < 8 && busy * args.splits * 2 <= 2 * sm_count && args.kb >= args.splits * 8) args.splits *= 2;
+  args.splits = splits;
   args.stages = kStages;
   const int smem = kStages * kStage + 1024;
   static int smem_set[kMaxDevices];
@@ -88,11 +93,55 @@ static int launch_stream(const Problem& p, int device, int sm_count, cudaStream_
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_stream_kernel");
 }
 
-// CTA pairs that the GPU holds at once, per device and form (0: not queried yet).
-static int g_tile_pairs[kMaxDevices][2];
+// Clusters of 1, 2 and 4 CTA pairs that the GPU holds at once, per device and form (first entry 0: not queried yet).
+static int g_tile_clusters[kMaxDevices][2][3];
 
 template <int kHalves>
-static int launch_tiles(const Problem& p, int device, int sm_count, cudaStream_t stream) {
+static int tile_clusters(int device, int sm_count, int (&clusters)[3]) {
+  auto kernel = fp8_block_tile_kernel<kHalves>;
+  std::lock_guard<std::mutex> lock(g_dev_mutex);
+  int(&known)[3] = g_tile_clusters[device][kHalves - 1];
+  if (known[0] == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem);
+    if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, kernel);
+    if (e != cudaSuccess) return fail_cuda(e, "cudaFuncGetAttributes");
+    // the warpgroups' register shares add up to the launch's total: fewer at launch and the larger share would wait for good
+    if (fa.numRegs != kTileRegs)
+      return fail(MAGI_SWIGLU_ERR_DEVICE, "fp8_block_tile_kernel was built with %d registers a thread, not %d", fa.numRegs, kTileRegs);
+    int found[3] = {0, 0, 0};
+    for (int i = 0; i < 3; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2u << i;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3((unsigned)(sm_count / (2 << i) * (2 << i)));
+      cfg.blockDim = dim3(kTileThreads);
+      cfg.dynamicSmemBytes = kTileSmem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&found[i], kernel, &cfg);
+      if (e != cudaSuccess) return fail_cuda(e, "cudaOccupancyMaxActiveClusters");
+    }
+    if (found[0] < 1) return fail(MAGI_SWIGLU_ERR_DEVICE, "this device cannot hold a CTA pair of fp8_block_tile_kernel");
+    for (int i = 0; i < 3; ++i) known[i] = found[i];
+  }
+  for (int i = 0; i < 3; ++i) clusters[i] = known[i];
+  return 0;
+}
+
+// When all tiles fit as clusters of several pairs, those share the tiles' K blocks (at least eight each).
+static int tile_log_splits(int64_t most, int kb, const int (&clusters)[3]) {
+  int s = 0;
+  while (s < 2 && most <= clusters[s + 1] && kb >= (16 << s)) ++s;
+  return s;
+}
+
+template <int kHalves>
+static int launch_tiles(const Problem& p, const int (&clusters)[3], cudaStream_t stream) {
   const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.args.E * kHalves};
   const cuuint64_t wst[2] = {(cuuint64_t)p.K, (cuuint64_t)p.N * (cuuint64_t)p.K};
   const cuuint64_t ad[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M};
@@ -102,9 +151,8 @@ static int launch_tiles(const Problem& p, int device, int sm_count, cudaStream_t
   if (int rc = encode_bytes_map(p.b, 3, wd, wst, wb, &tm_w, "B")) return rc;
   if (int rc = encode_bytes_map(p.a, 2, ad, ast, ab, &tm_a, "A")) return rc;
   const int64_t n_tiles = (p.N + 256 / kHalves - 1) / (256 / kHalves);
-  const int64_t units = p.M / kTileRows + (p.args.offsets ? p.args.E : 1);  // at most one partial group an expert
+  const int64_t units = most_groups(p, kTileRows);
   if (units * n_tiles > 0x7fffffffLL / 2) return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld x N=%lld is too large for one launch", (long long)p.M, (long long)p.N);
-  constexpr int kSmem = kTileStages * kTileStage + 1024;
   auto kernel = fp8_block_tile_kernel<kHalves>;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -113,43 +161,23 @@ static int launch_tiles(const Problem& p, int device, int sm_count, cudaStream_t
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.blockDim = dim3(kTileThreads);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = kTileSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaSuccess;
-  int pairs = 0;
-  {
-    std::lock_guard<std::mutex> lock(g_dev_mutex);
-    int& known = g_tile_pairs[device][kHalves - 1];
-    if (known == 0) {
-      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-      if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
-      cudaFuncAttributes fa;
-      e = cudaFuncGetAttributes(&fa, kernel);
-      if (e != cudaSuccess) return fail_cuda(e, "cudaFuncGetAttributes");
-      // the warpgroups' register shares add up to the launch's total: fewer at launch and the larger share would wait for good
-      if (fa.numRegs != kTileRegs)
-        return fail(MAGI_SWIGLU_ERR_DEVICE, "fp8_block_tile_kernel was built with %d registers a thread, not %d", fa.numRegs, kTileRegs);
-      cfg.gridDim = dim3((unsigned)(sm_count / 2 * 2));
-      int n = 0;
-      e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-      if (e != cudaSuccess) return fail_cuda(e, "cudaOccupancyMaxActiveClusters");
-      if (n < 1) return fail(MAGI_SWIGLU_ERR_DEVICE, "this device cannot hold a CTA pair of fp8_block_tile_kernel");
-      known = n;
-    }
-    pairs = known;
-  }
   const int64_t most = units * n_tiles;
-  if (pairs > most) pairs = (int)most;
-  cfg.gridDim = dim3((unsigned)(2 * pairs));
-  const int wide = ((uintptr_t)p.args.c & 31u) == 0 && p.N % 16 == 0;
+  const int log_splits = tile_log_splits(most, p.args.kb, clusters);
+  Args args = p.args;
+  args.splits = 1 << log_splits;
   // A raster band of about 32 MB of A: it is read once per column tile and should stay in L2 beside the W rows that pass
   // (8192 rows: K = 4096, N = 2 x 14336: bands of 8 / 16 / 32 groups 980 / 948 / 942 us; K = 14336: 447 / 451 / 468 us).
-  Args args = p.args;
   const int64_t band = (32LL << 20) / (kTileRows * p.K);
   args.band = (int)(band < 4 ? 4 : (band > 64 ? 64 : band));
-  e = cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_a, args, wide);
+  const int64_t workers = most < clusters[log_splits] ? most : clusters[log_splits];
+  attr[0].val.clusterDim.x = 2u << log_splits;
+  cfg.gridDim = dim3((unsigned)(workers * (2 << log_splits)));
+  const int wide = ((uintptr_t)p.args.c & 31u) == 0 && p.N % 16 == 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_a, args, wide);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_tile_kernel");
 }
 
@@ -160,20 +188,45 @@ static int run(const Problem& p, int device, void* cuda_stream) {
   cudaError_t e = guard.set(device);
   if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  // Tokens per tile of the stream kernel: enough for twice an expert's average share of the rows (shares are uneven), so
-  // that W is usually streamed once.  8 experts, 74 rows, N = 4096, K = 14336: 16 tokens a tile 86 us, 32 tokens 79 us.
-  const int64_t share = p.args.offsets ? (2 * p.M + p.args.E - 1) / p.args.E : p.M;
-  if (p.halves == 1) {
-    if (share <= 16) return launch_stream<1, 16>(p, device, di->sm_count, stream);
-    if (share <= 32) return launch_stream<1, 32>(p, device, di->sm_count, stream);
-    if (share <= 64) return launch_stream<1, 64>(p, device, di->sm_count, stream);
-    if (share <= 128) return launch_stream<1, 128>(p, device, di->sm_count, stream);
-    return launch_tiles<1>(p, device, di->sm_count, stream);
+  // The kernel and its tokens per tile by what the forms are expected to take: rounds of the GPU's CTAs (pairs), each a
+  // fixed part and a part per K block.  The constants are microseconds measured with everything in flight (148 SMs):
+  // stream kernel, two CTAs an SM, 0.36 / 0.43 / 0.50 a K block for 16 / 32 / 64 tokens, 0.75 / 0.90 for 16 / 32 in the
+  // SwiGLU form, about 0.6 of that with one CTA an SM; tile kernel 0.42 a K block and 2.5 a tile.  Both sides at N = 4096,
+  // K = 14336 (stream 16 / 32 / 64 tokens, tiles): M = 64 26 / 18 / 16 / 35 us, 256 - / 47 / 35 / 35 us, 512 - / - / 58 /
+  // 37 us; SwiGLU, N = 1408, K = 2048, 64 experts (16 / 32 tokens, tiles): 512 rows 52 / 48 / 78 us, 2048 rows 85 / 75 / 96
+  // us, 8192 rows 295 / 199 / 138 us.  A cluster's CTAs split K while the tiles leave SMs idle.
+  int clusters[3];
+  if (int rc = p.halves == 1 ? tile_clusters<1>(device, di->sm_count, clusters) : tile_clusters<2>(device, di->sm_count, clusters))
+    return rc;
+  const double n128 = (double)((p.N + 127) / 128);
+  double best = 0;
+  int tok = 0, splits = 1;
+  {
+    const int64_t n_tiles = (p.N * p.halves + 255) / 256;
+    const int log_splits = tile_log_splits(most_groups(p, kTileRows) * n_tiles, p.args.kb, clusters);
+    const double rounds = ceil(expected_groups(p, kTileRows) * n_tiles / clusters[log_splits]);
+    best = 5.0 + rounds * (p.args.kb * 0.42 / (1 << log_splits) + 2.5) + (log_splits ? 3.0 : 0.0);
   }
-  if (share <= 16) return launch_stream<2, 16>(p, device, di->sm_count, stream);
-  if (share <= 32) return launch_stream<2, 32>(p, device, di->sm_count, stream);
-  if (share <= 64) return launch_stream<2, 64>(p, device, di->sm_count, stream);
-  return launch_tiles<2>(p, device, di->sm_count, stream);
+  const int forms = p.halves == 1 ? 3 : 2;
+  static const double per_block[2][3] = {{0.36, 0.43, 0.50}, {0.75, 0.90, 0.0}};
+  for (int i = 0; i < forms; ++i) {
+    if (most_groups(p, 16 << i) > 65535) continue;
+    const double ctas = n128 * expected_groups(p, 16 << i);
+    int z = 1;  // up to eight CTAs share a tile's K blocks, at least four each, until there are about two CTAs an SM
+    while (z < 8 && ctas * z * 2 <= 2 * di->sm_count && p.args.kb >= z * 8) z *= 2;
+    const double rounds = ceil(ctas * z / (2 * di->sm_count));
+    const double cost = 2.5 + rounds * (p.args.kb * per_block[p.halves - 1][i] / z * (ctas * z <= di->sm_count ? 0.6 : 1.0) + 2.5);
+    if (cost < best) best = cost, tok = 16 << i, splits = z;
+  }
+  if (p.halves == 1) {
+    if (tok == 16) return launch_stream<1, 16>(p, device, splits, stream);
+    if (tok == 32) return launch_stream<1, 32>(p, device, splits, stream);
+    if (tok == 64) return launch_stream<1, 64>(p, device, splits, stream);
+    return launch_tiles<1>(p, clusters, stream);
+  }
+  if (tok == 16) return launch_stream<2, 16>(p, device, splits, stream);
+  if (tok == 32) return launch_stream<2, 32>(p, device, splits, stream);
+  return launch_tiles<2>(p, clusters, stream);
 }
 
 static int check(const void* a, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,

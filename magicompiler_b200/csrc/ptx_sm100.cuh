@@ -341,13 +341,13 @@ __device__ __forceinline__ void umma_fp8(uint32_t d_tmem, uint64_t a_desc, uint6
         : "memory");
 }
 // The mbarrier gets one arrival when every tcgen05 operation issued so far by this thread is done.
-// kCtas = 2: the barrier at the same shared-memory offset in BOTH CTAs of the pair gets the arrival.
+// kCtas = 2: the barrier at the same shared-memory offset in BOTH CTAs of the pair gets the arrival (`both` has a bit for
+// each of the two cluster ranks: a pair that is not the cluster's first passes its own).
 template <int kCtas>
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
+__device__ __forceinline__ void umma_commit(uint32_t bar, uint16_t both = 3) {
   if constexpr (kCtas == 1) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
   } else {
-    const uint16_t both = 3;
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"(both)
                  : "memory");

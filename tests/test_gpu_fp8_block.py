@@ -101,7 +101,8 @@ def check_fused(t, codes, scales):
 
 DENSE = [(1, 8, 16), (1, 128, 128), (1, 264, 144), (3, 136, 400), (16, 256, 512), (17, 384, 256), (31, 1000, 1040), (33, 128, 2048),
          (64, 520, 384), (65, 256, 640), (127, 136, 272), (128, 256, 256), (129, 264, 1152), (200, 2048, 512), (257, 776, 912),
-         (300, 256, 4096), (513, 512, 384), (1000, 392, 1296), (2049, 1024, 256), (5, 4096, 8192)]
+         (300, 256, 4096), (513, 512, 384), (1000, 392, 1296), (2049, 1024, 256), (5, 4096, 8192),
+         (300, 264, 2064), (260, 1032, 4112), (700, 136, 8192), (1030, 4096, 2048)]
 
 
 @pytest.mark.parametrize("M,N,K", DENSE)
@@ -134,6 +135,20 @@ def test_experts(E, counts, tail, N, K):
 @pytest.mark.parametrize("N,K", [(144, 272), (256, 512)])
 def test_experts_swiglu(E, counts, tail, N, K):
     t = case(sum(counts) + tail, N, K, E=E, counts=counts, halves=2, seed=E)
+    codes, scales = mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    check_fused(t, codes, scales)
+    assert (codes[sum(counts):].float() == 0).all() and (scales[sum(counts):] == 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("N,K", [(272, 2064), (144, 4112)])
+def test_few_tiles_with_many_k_blocks(N, K):
+    """Experts whose tiles share their K blocks among several CTA pairs, one of them empty, one with a partial group."""
+    counts, tail = [300, 0, 257, 100], 9
+    t = case(sum(counts) + tail, N, K, E=4, counts=counts)
+    got = mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    check_plain(t, got)
+    assert (got[sum(counts):] == 0).all()
+    t = case(sum(counts) + tail, N, K, E=4, counts=counts, halves=2)
     codes, scales = mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
     check_fused(t, codes, scales)
     assert (codes[sum(counts):].float() == 0).all() and (scales[sum(counts):] == 2.0 ** -126).all()
@@ -206,7 +221,8 @@ def test_bad_offsets_touch_nothing_outside(M, counts):
     assert mb.device_status(0)["code"] == 0
 
 
-@pytest.mark.parametrize("M,N,K,E", [(3, 512, 2048, 0), (40, 256, 512, 8), (700, 512, 384, 0), (900, 264, 512, 3)])
+@pytest.mark.parametrize("M,N,K,E", [(3, 512, 2048, 0), (40, 256, 512, 8), (700, 512, 384, 0), (900, 264, 512, 3),
+                                     (300, 512, 4096, 0), (300, 512, 2048, 0)])
 def test_the_same_bits_every_time(M, N, K, E):
     counts = [M // E] * E if E else None
     for halves, form in ((1, mb.gemm_fp8_block), (2, mb.gemm_swiglu_fp8_block)):
