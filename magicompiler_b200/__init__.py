@@ -16,6 +16,7 @@ from .register import COMPUTE_SENSITIVE_OPS, SPLITTING_OPS, magi_register_custom
 from .routed import (expert_combine, expert_combine_backward, expert_combine_out, expert_gather, expert_gather_fp8,  # noqa: F401
                      expert_gather_fp8_out, expert_gather_out, expert_sort, expert_sort_out, quantize_fp8_block,
                      quantize_fp8_block_out)
+from .routed_mlp import RoutedSwiGLUMLP  # noqa: F401
 from .sharding import (  # noqa: F401
     ColumnParallelSwiGLU,
     PeerScatterReducer,
@@ -33,6 +34,6 @@ __all__ = [
     "expert_sort", "expert_sort_out", "expert_gather", "expert_gather_out", "expert_combine", "expert_combine_out",
     "expert_combine_backward", "expert_gather_fp8", "expert_gather_fp8_out", "quantize_fp8_block", "quantize_fp8_block_out",
     "gemm_fp8_block", "gemm_fp8_block_out", "gemm_swiglu_fp8_block", "gemm_swiglu_fp8_block_out", "quantize_fp8_weight",
-    "quantize_fp8_gate_up",
+    "quantize_fp8_gate_up", "RoutedSwiGLUMLP",
     "COMPUTE_SENSITIVE_OPS", "build_library", "load_library", "plan", "workspace_bytes", "device_status", "kernel_clock", "MagiSwigluLibraryError",
 ]

@@ -143,10 +143,12 @@ def _check_weights(name: str, weights: torch.Tensor, tokens: int, k: int) -> Non
         raise ValueError(f"{name}: weights must be [{tokens}, {k}]; got shape {tuple(weights.shape)}")
 
 
-def _eager(grad: torch.Tensor) -> bool:
-    """A plain backward step: nothing traces it and no graph of it is wanted, so the op's body may be called without the
-    dispatcher (which costs about as much host time as the rest of a call)."""
-    return type(grad) is torch.Tensor and not torch.is_grad_enabled() and not torch.compiler.is_compiling()
+def _plain(t: torch.Tensor) -> bool:
+    """Whether nothing but autograd looks at a call on ``t``: no compiler, tracing mode, tensor subclass or functorch
+    transform.  Such a call may go to the op's body without the dispatcher, which with a registered autograd formula costs
+    more host time than a training step's kernels run (132 us for a gather of any size and its gradient)."""
+    return (type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and not torch.compiler.is_compiling() \
+        and torch._C._len_torch_dispatch_stack() == 0 and torch._C._functorch.peek_interpreter_stack() is None
 
 
 def _ld(t2: torch.Tensor) -> int:
@@ -178,18 +180,34 @@ def _gather_setup_context(ctx, inputs, output):
 
 def _gather_backward(ctx, grad):
     row_slot, slot_row = ctx.saved_tensors
-    combine = expert_combine_out if _eager(grad) else torch.ops.magi_swiglu.expert_combine
-    return combine(grad, None, row_slot, slot_row), None, None
+    return expert_combine(grad, None, row_slot, slot_row), None, None
 
 
 @magi_register_custom_op(
     name=GATHER_OP_NAME, mutates_args=(),
     infer_output_meta_fn=lambda x, row_slot, slot_row: x.new_empty((row_slot.shape[0], x.shape[1])),
     setup_context_fn=_gather_setup_context, backward_fn=_gather_backward, is_subgraph_boundary=True)
+def _expert_gather_op(x: torch.Tensor, row_slot: torch.Tensor, slot_row: torch.Tensor) -> torch.Tensor:
+    return expert_gather_out(x, row_slot, slot_row)
+
+
+class _Gather(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, row_slot, slot_row):
+        ctx.save_for_backward(row_slot, slot_row)
+        return expert_gather_out(x, row_slot, slot_row)
+
+    backward = staticmethod(_gather_backward)
+
+
 def expert_gather(x: torch.Tensor, row_slot: torch.Tensor, slot_row: torch.Tensor) -> torch.Tensor:
     """``xs[r] = x[row_slot[r] // k]`` (``[T, H]`` -> ``[T*k, H]`` bf16, H a multiple of 8), zeros where ``row_slot`` is -1
     (``magi_swiglu_expert_gather_bf16``).  Gradient: ``dx[t]`` is the fp32 sum of its rows' gradients in slot order,
-    rounded once."""
+    rounded once.  In compiled or traced code this is ``torch.ops.magi_swiglu.expert_gather``."""
+    if not (isinstance(x, torch.Tensor) and _plain(x)):
+        return torch.ops.magi_swiglu.expert_gather(x, row_slot, slot_row)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Gather.apply(x, row_slot, slot_row)
     return expert_gather_out(x, row_slot, slot_row)
 
 
@@ -264,10 +282,10 @@ def _combine_setup_context(ctx, inputs, output):
 
 def _combine_backward(ctx, grad):
     if not ctx.weighted:
-        gather = expert_gather_out if _eager(grad) else torch.ops.magi_swiglu.expert_gather
-        return gather(grad, *ctx.saved_tensors), None, None, None
+        return expert_gather(grad, *ctx.saved_tensors), None, None, None
     need_dy, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    backward = _combine_backward_body if _eager(grad) else torch.ops.magi_swiglu.expert_combine_backward
+    plain = _plain(grad) and not torch.is_grad_enabled()
+    backward = _combine_backward_body if plain else torch.ops.magi_swiglu.expert_combine_backward
     dy, dw = backward(grad, *ctx.saved_tensors, need_dy, need_dw)
     return dy if need_dy else None, dw if need_dw else None, None, None
 
@@ -276,11 +294,30 @@ def _combine_backward(ctx, grad):
     name=COMBINE_OP_NAME, mutates_args=(),
     infer_output_meta_fn=lambda y, weights, row_slot, slot_row: y.new_empty((slot_row.shape[0], y.shape[1])),
     setup_context_fn=_combine_setup_context, backward_fn=_combine_backward, is_subgraph_boundary=True)
+def _expert_combine_op(y: torch.Tensor, weights: Optional[torch.Tensor], row_slot: torch.Tensor,
+                       slot_row: torch.Tensor) -> torch.Tensor:
+    return expert_combine_out(y, weights, row_slot, slot_row)
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, row_slot, slot_row):
+        _combine_setup_context(ctx, (y, weights, row_slot, slot_row), None)
+        return expert_combine_out(y, weights, row_slot, slot_row)
+
+    backward = staticmethod(_combine_backward)
+
+
 def expert_combine(y: torch.Tensor, weights: Optional[torch.Tensor], row_slot: torch.Tensor,
                    slot_row: torch.Tensor) -> torch.Tensor:
     """``out[t] = sum_j weights[t, j] * y[slot_row[t, j]]`` (``[T*k, H]`` bf16 and ``[T, k]`` fp32 -> ``[T, H]`` bf16;
     fp32 sums in slot order, one rounding; ``weights`` None: ones; ``magi_swiglu_expert_combine_bf16``).  Slots without an
-    expert add nothing.  Gradients with respect to ``y`` and ``weights``."""
+    expert add nothing.  Gradients with respect to ``y`` and ``weights`` (once differentiable where weights are given).  In
+    compiled or traced code this is ``torch.ops.magi_swiglu.expert_combine``."""
+    if not (isinstance(y, torch.Tensor) and _plain(y)):
+        return torch.ops.magi_swiglu.expert_combine(y, weights, row_slot, slot_row)
+    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+        return _Combine.apply(y, weights, row_slot, slot_row)
     return expert_combine_out(y, weights, row_slot, slot_row)
 
 

@@ -1,0 +1,134 @@
+"""``RoutedSwiGLUMLP``: the routed operators and the experts' products as a user runs them, forward, gradients, fp8, graph."""
+import pytest
+import torch
+
+import magicompiler_b200 as mb
+
+BF = torch.bfloat16
+
+
+def weights(E, N, K, K_out, seed, device):
+    g = torch.Generator().manual_seed(seed)
+    w13 = (torch.randn(E, 2 * N, K, generator=g) * K ** -0.5).to(BF)
+    w2 = (torch.randn(E, K_out, N, generator=g) * N ** -0.5).to(BF)
+    return w13.to(device), w2.to(device)
+
+
+def batch(shape, k, E, K, seed, drop=0.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, K, generator=g).to(BF)
+    logits = torch.randn(*shape, E, generator=g)
+    top, ids = torch.topk(logits, k, dim=-1)
+    ids[torch.rand(*shape, k, generator=g) < drop] = -1
+    return x.cuda(), ids.cuda(), torch.softmax(top, -1).cuda()
+
+
+def plain(x, ids, w, w13, w2):
+    """The formula in 64 bits, differentiable, masked instead of sorted."""
+    N = w2.shape[2]
+    out = 0
+    for e in range(w13.shape[0]):
+        h = x @ w13[e].t()
+        y = (torch.nn.functional.silu(h[..., :N]) * h[..., N:]) @ w2[e].t()
+        out = out + y * (w * (ids == e)).sum(-1, keepdim=True)
+    return out
+
+
+def test_refusals():
+    w13, w2 = weights(2, 64, 32, 32, 0, "cpu")
+    with pytest.raises(ValueError, match="precision"):
+        mb.RoutedSwiGLUMLP(w13, w2, precision="int8")
+    with pytest.raises(ValueError, match="must be"):
+        mb.RoutedSwiGLUMLP(w13, w2[:1])
+    with pytest.raises(ValueError, match="must be"):
+        mb.RoutedSwiGLUMLP(w13[:, :100], w2)
+    with pytest.raises(TypeError, match="bf16"):
+        mb.RoutedSwiGLUMLP(w13.float(), w2.float())
+    mlp = mb.RoutedSwiGLUMLP(w13, w2)
+    x = torch.zeros(3, 32, dtype=BF)
+    with pytest.raises(ValueError, match="agree"):
+        mlp(x, torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 1))
+    with pytest.raises(ValueError, match="agree"):
+        mlp(x, torch.zeros(2, 2, dtype=torch.int64), torch.zeros(2, 2))
+    with pytest.raises(TypeError, match="CUDA tensors only"):
+        mlp(x, torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,k,E,K,N,drop", [((1,), 2, 4, 64, 128, 0), ((3, 17), 2, 4, 256, 272, 0.2), ((300,), 3, 8, 128, 64, 0),
+                                                ((40,), 2, 40, 64, 48, 0), ((5,), 2, 3, 64, 64, 1.0)])
+def test_training_step(shape, k, E, K, N, drop):
+    """bf16: the four roundings to bf16 of the chain (y, h, the experts' outputs, the result; a gradient has as many again)
+    are 2^-8 of a value each with random signs: 2-norm errors stay under 8 * 2^-8 of the norm."""
+    w13, w2 = weights(E, N, K, K, 1, "cuda")
+    x, ids, w = batch(shape, k, E, K, 2, drop)
+    mlp = mb.RoutedSwiGLUMLP(w13, w2)
+    x.requires_grad_(), w.requires_grad_()
+    out = mlp(x, ids, w)
+    leaves = [t.detach().double().requires_grad_() for t in (x, w, w13, w2)]
+    want = plain(leaves[0], ids, leaves[1], leaves[2], leaves[3])
+    d = torch.randn(*shape, K, generator=torch.Generator().manual_seed(3)).to(BF).cuda()
+    out.backward(d)
+    want.backward(d.double())
+    assert out.shape == (*shape, K) and out.dtype == BF
+    for name, got, ref in (("out", out, want), ("x", x.grad, leaves[0].grad), ("w", w.grad, leaves[1].grad),
+                           ("gate_up", mlp.w_gate_up.grad, leaves[2].grad), ("down", mlp.w_down.grad, leaves[3].grad)):
+        got, ref = got.detach().double(), ref.detach()
+        assert (got - ref).norm() <= 8 * 2.0 ** -8 * ref.norm() + 1e-30, (name, ((got - ref).norm() / ref.norm()).item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,k,E,K,N,drop", [((1,), 2, 8, 256, 272, 0), ((2, 33), 2, 4, 272, 256, 0.2), ((600,), 4, 6, 512, 384, 0)])
+def test_fp8_forward(shape, k, E, K, N, drop):
+    """Three quantisations at 2^-4 of a value at most each, uniform in their step: 3 * 2^-4 / sqrt(3) ~ 0.11 of the norm."""
+    w13, w2 = weights(E, N, K, K, 4, "cuda")
+    x, ids, w = batch(shape, k, E, K, 5, drop)
+    mlp = mb.RoutedSwiGLUMLP(w13, w2, precision="fp8")
+    out = mlp(x, ids, w)
+    want = plain(x.double(), ids, w.double(), w13.double(), w2.double())
+    assert out.shape == (*shape, K) and (out.double() - want).norm() <= 0.11 * want.norm()
+    assert set(mlp.state_dict()) == {"gate_up_codes", "gate_up_scales", "down_codes", "down_scales"}
+
+
+@pytest.mark.gpu
+def test_fp8_forward_captured_on_a_stream():
+    w13, w2 = weights(8, 256, 256, 256, 6, "cuda")
+    mlp = mb.RoutedSwiGLUMLP(w13, w2, precision="fp8")
+    x, ids, w = batch((24,), 2, 8, 256, 7)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mlp(x, ids, w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = mlp(x, ids, w)
+    for seed in (8, 9):
+        for dst, src in zip((x, ids, w), batch((24,), 2, 8, 256, seed, 0.3)):
+            dst.copy_(src)
+        graph.replay()
+        assert torch.equal(out, mlp(x, ids, w))
+
+
+@pytest.mark.gpu
+def test_traced_and_compiled_calls_go_through_the_ops():
+    """make_fx and autograd formulas of the registered ops: the same values as the direct calls."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, ids, w = batch((20,), 2, 4, 64, 1)
+    row_slot, slot_row, _ = mb.expert_sort(ids, 4)
+
+    def block(x, w):
+        return mb.expert_combine(mb.expert_gather(x, row_slot, slot_row), w, row_slot, slot_row)
+
+    graph = make_fx(block)(x, w)
+    targets = {str(n.target) for n in graph.graph.nodes if n.op == "call_function"}
+    assert {"magi_swiglu.expert_gather.default", "magi_swiglu.expert_combine.default"} <= targets
+    assert torch.equal(graph(x, w), block(x, w))
+    grads = []
+    for gather, combine in ((mb.expert_gather, mb.expert_combine),
+                            (torch.ops.magi_swiglu.expert_gather, torch.ops.magi_swiglu.expert_combine)):
+        lx, lw = x.clone().requires_grad_(), w.clone().requires_grad_()
+        combine(gather(lx, row_slot, slot_row), lw, row_slot, slot_row).sum().backward()
+        grads.append((lx.grad, lw.grad))
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
