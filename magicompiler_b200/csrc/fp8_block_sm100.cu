@@ -55,7 +55,10 @@ static double expected_groups(const Problem& p, int rows) {
 template <int kHalves, int kTok>
 static int launch_stream(const Problem& p, int device, int splits, cudaStream_t stream) {
   constexpr int kStage = kHalves * kWTile + kTok * kBlk;
-  constexpr int kFit = (108 * 1024 - 1024) / kStage;  // two CTAs an SM
+  // Two CTAs an SM, and no room beside one for a CTA of the bf16 kernels, which take at least 120 KB and all of tensor
+  // memory: two clusters whose CTAs wait for each other's tensor memory on two SMs would wait for good.
+  constexpr int kSmem = 108 * 1024;
+  constexpr int kFit = (kSmem - 1024) / kStage;
   constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
   static_assert(kStages >= 2 && kStages * kStage >= kTok * kHalves * 512, "stages hold the sums of a tile");
   const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.args.E * kHalves};
@@ -73,9 +76,8 @@ static int launch_stream(const Problem& p, int device, int splits, cudaStream_t 
   Args args = p.args;
   args.splits = splits;
   args.stages = kStages;
-  const int smem = kStages * kStage + 1024;
   static int smem_set[kMaxDevices];
-  cudaError_t e = allow_smem_once(fp8_block_stream_kernel<kHalves, kTok>, smem, device, smem_set);
+  cudaError_t e = allow_smem_once(fp8_block_stream_kernel<kHalves, kTok>, kSmem, device, smem_set);
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -85,7 +87,7 @@ static int launch_stream(const Problem& p, int device, int splits, cudaStream_t 
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(n_tiles * args.splits), (unsigned)groups);
   cfg.blockDim = dim3(kStreamThreads);
-  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = args.splits > 1 ? 1 : 0;

@@ -47,6 +47,8 @@ class RoutedSwiGLUMLP(torch.nn.Module):
         if expert_ids.shape != weights.shape or expert_ids.shape[:-1] != x.shape[:-1]:
             raise ValueError(f"x {tuple(x.shape)}, expert_ids {tuple(expert_ids.shape)} and weights {tuple(weights.shape)} "
                              "must agree in their leading dimensions, ids and weights in all")
+        if self.precision == "fp8" and torch.is_grad_enabled() and (x.requires_grad or weights.requires_grad):
+            raise RuntimeError("precision='fp8' is for inference: it has no gradients (run it under torch.no_grad())")
         x2, k = x.reshape(-1, x.shape[-1]), expert_ids.shape[-1]
         ids, w = expert_ids.reshape(-1, k), weights.reshape(-1, k)
         row_slot, slot_row, offsets = expert_sort_out(ids, self.num_experts)

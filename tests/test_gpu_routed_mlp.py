@@ -87,6 +87,8 @@ def test_fp8_forward(shape, k, E, K, N, drop):
     out = mlp(x, ids, w)
     want = plain(x.double(), ids, w.double(), w13.double(), w2.double())
     assert out.shape == (*shape, K) and (out.double() - want).norm() <= 0.11 * want.norm()
+    with pytest.raises(RuntimeError, match="inference"):
+        mlp(x.clone().requires_grad_(), ids, w)
     assert set(mlp.state_dict()) == {"gate_up_codes", "gate_up_scales", "down_codes", "down_scales"}
 
 
@@ -132,3 +134,27 @@ def test_traced_and_compiled_calls_go_through_the_ops():
         combine(gather(lx, row_slot, slot_row), lw, row_slot, slot_row).sum().backward()
         grads.append((lx.grad, lw.grad))
     assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
+@pytest.mark.gpu
+def test_registered_ops_keep_their_contracts():
+    """Schema, fake implementation (shapes, strides, types) and autograd registration of every new op against real calls."""
+    x, ids, w = batch((9,), 2, 4, 144, 2, 0.2)
+    row_slot, slot_row, offsets = mb.expert_sort(ids, 4)
+    xs, ops = mb.expert_gather(x, row_slot, slot_row), torch.ops.magi_swiglu
+    a, a_scale = mb.quantize_fp8_block(xs)
+    w13, w2 = weights(4, 64, 144, 144, 3, "cuda")
+    q13, q2 = mb.quantize_fp8_gate_up(w13), mb.quantize_fp8_weight(w2)
+    h, h_scale = mb.gemm_swiglu_fp8_block(a, a_scale, *q13, offsets)
+    grad = lambda t: t.clone().requires_grad_()  # noqa: E731
+    every = ("test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic")
+    with_fp8 = every[1:3]  # torch's schema check multiplies the values, which float8 tensors cannot do
+    for op, args, tests in (
+            (ops.expert_sort, (ids, 4), every), (ops.expert_gather, (grad(x), row_slot, slot_row), every),
+            (ops.expert_combine, (grad(xs), grad(w), row_slot, slot_row), every),
+            (ops.expert_combine, (grad(xs), None, row_slot, slot_row), every),
+            (ops.expert_combine_backward, (x, xs, w, row_slot, slot_row, True, True), every[:3]),
+            (ops.quantize_fp8_block, (x,), with_fp8), (ops.expert_gather_fp8, (x, row_slot, slot_row), with_fp8),
+            (ops.gemm_swiglu_fp8_block, (a, a_scale, *q13, offsets), with_fp8),
+            (ops.gemm_fp8_block, (h, h_scale, *q2, offsets), with_fp8), (ops.gemm_fp8_block, (a, a_scale, q13[0][0], q13[1][0][:1]), with_fp8)):
+        torch.library.opcheck(op.default, args, test_utils=tests)
