@@ -19,7 +19,7 @@
 namespace magi {
 
 constexpr int kMaxExperts = 1024;   // one 32-warp histogram of 1025 counters is 131 KB of shared memory
-constexpr int kSlotBatch = 8;       // expert rows of one token in flight per thread of the combine's backward
+constexpr int kSlotBatch = 4;       // expert rows of one token in flight per thread of the combine's backward
 constexpr float kFp8Max = 448.0f;   // largest e4m3 value
 constexpr float kScaleFloor = 1.17549435e-38f;  // 2^-126: a block of zeros (or of subnormals) keeps a normal scale
 
@@ -218,11 +218,11 @@ __device__ __forceinline__ uint4 f32_to_bf16x8(const float (&f)[8]) {
 }
 
 // out[t] = sum over j of w[t, j] * y[slot_row[t, j]] in fp32, j ascending, one rounding; w null: all ones (the gradient of
-// the gather).  Slots without an expert add nothing, whatever their weight.  A thread keeps kSlots * kPieces = 8 loads of
-// 16 bytes in flight: kSlots rows of its token, kPieces column pieces a block's width apart (only one of each for k = 2
-// ran at 3.0 TB/s, 8192 tokens, H = 4096).
+// the gather).  Slots without an expert add nothing, whatever their weight.  A thread keeps kSlots * kPieces loads of 16
+// bytes in flight: kSlots rows of its token, kPieces column pieces a block's width apart (8192 tokens of k = 2, H = 4096: two
+// loads 67 us, eight 40 us, eight with three blocks an SM 36 us).
 template <int kSlots, int kPieces>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
 expert_combine_kernel(const uint4* y, long long ldy, const float* w, const int* slot_row, uint4* out, long long T, int k,
                       int vecs, int col_chunks) {
   const long long t = (long long)(blockIdx.x / col_chunks) * blockDim.y + threadIdx.y;
@@ -272,8 +272,9 @@ expert_combine_kernel(const uint4* y, long long ldy, const float* w, const int* 
 
 // The combine's gradients in one pass: dy[slot_row[t, j]] = w[t, j] * dout[t] (rows without a slot are zeroed) and
 // dw[t, j] = <dout[t], y[slot_row[t, j]]> (0 for a slot without an expert), sums in fp32 in a fixed order.
-// token_warps warps (1, 2, 4 or 8) share a token.  dy or dw may be null (y is not read without dw).
-__global__ void __launch_bounds__(256)
+// token_warps warps (1, 2, 4 or 8) share a token.  dy or dw may be null (y is not read without dw).  Batches of four rows
+// and four blocks an SM: 8192 tokens x 8 rows of 2048, back to back, 100 us; of eight rows and two blocks 136 us.
+__global__ void __launch_bounds__(256, 4)
 expert_combine_backward_kernel(const uint4* dout, long long lddout, const uint4* y, long long ldy, const float* w,
                                const int* row_slot, const int* slot_row, uint4* dy, float* dw, long long T, int k, int vecs,
                                int token_warps) {

@@ -167,15 +167,15 @@ int magi_swiglu_expert_combine_bf16(const void* y, const float* weights, const i
   if (unaligned(y, out)) return fail(MAGI_SWIGLU_ERR_ALIGN, "y and out must be 16-byte aligned");
   const DeviceInfo* di = nullptr;
   if (int rc = require_b200(device, &di)) return rc;
-  // eight loads in flight per thread, split between the token's rows and column pieces
-  const int pieces = k <= 1 ? 8 : (k <= 2 ? 4 : (k <= 4 ? 2 : 1));
+  // up to eight loads in flight per thread, split between the token's rows and column pieces
+  const int pieces = k <= 2 ? 4 : (k <= 4 ? 2 : 1);
   RowGrid g;
   if (int rc = row_grid(T, (H / 8 + pieces - 1) / pieces, &g)) return rc;
   DeviceGuard guard;
   cudaError_t e = guard.set(device);
   if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
-  auto kernel = pieces == 8 ? expert_combine_kernel<1, 8> : pieces == 4 ? expert_combine_kernel<2, 4>
-                : pieces == 2 ? expert_combine_kernel<4, 2> : expert_combine_kernel<8, 1>;
+  auto kernel = k <= 1 ? expert_combine_kernel<1, 4> : k <= 2 ? expert_combine_kernel<2, 4>
+                : k <= 4 ? expert_combine_kernel<4, 2> : expert_combine_kernel<8, 1>;
   kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(cuda_stream)>>>(static_cast<const uint4*>(y), ldy / 8, weights,
                                                                          slot_row, static_cast<uint4*>(out), T, (int)k,
                                                                          (int)(H / 8), g.col_chunks);
