@@ -353,9 +353,9 @@ expert_combine_backward_kernel(const uint4* dout, long long lddout, const uint4*
 // all NaN.  Codes and scales equal the formula evaluated in fp32 with IEEE divisions bit for bit: x / s is x * r with
 // r = 1 / s rounded, corrected by its own remainder (Markstein 1990: q + r * (x - q * s) with fused multiply-adds), which
 // the tests compare with IEEE division for every pair of bf16 mantissas of x and of the block's maximum; powers of two
-// change nothing as long as the remainder stays normal, so blocks with an extreme or non-finite scale divide.  (Sixteen
-// divisions a thread took 26.6 us for 8192 x 4096, where the bytes take 15.5; back to back the correction takes 18.9 us, on two values an
-// instruction 17.7 us.)
+// change nothing as long as the remainder stays normal, so blocks with an extreme or non-finite scale divide.  8192 x 4096:
+// the bytes take 15.5 us; with sixteen divisions a thread 26.6 us, with the correction 18.9 us, with two values an
+// instruction 17.7 us.
 __device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));

@@ -5,9 +5,9 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from .fp8_block import gemm_fp8_block_out, gemm_swiglu_fp8_block_out, quantize_fp8_gate_up, quantize_fp8_weight
+from . import fp8_block, routed
+from .fp8_block import quantize_fp8_gate_up, quantize_fp8_weight
 from .ops import gemm_swiglu_auto
-from .routed import expert_combine, expert_combine_out, expert_gather, expert_gather_fp8_out, expert_sort_out
 
 
 class RoutedSwiGLUMLP(torch.nn.Module):
@@ -51,13 +51,15 @@ class RoutedSwiGLUMLP(torch.nn.Module):
             raise RuntimeError("precision='fp8' is for inference: it has no gradients (run it under torch.no_grad())")
         x2, k = x.reshape(-1, x.shape[-1]), expert_ids.shape[-1]
         ids, w = expert_ids.reshape(-1, k), weights.reshape(-1, k)
-        row_slot, slot_row, offsets = expert_sort_out(ids, self.num_experts)
+        out_form = "_out" if routed._plain(x) else ""  # compiled and traced code calls the registered ops
+        row_slot, slot_row, offsets = getattr(routed, "expert_sort" + out_form)(ids, self.num_experts)
         if self.precision == "fp8":
-            a, a_scale = expert_gather_fp8_out(x2, row_slot, slot_row)
-            h, h_scale = gemm_swiglu_fp8_block_out(a, a_scale, self.gate_up_codes, self.gate_up_scales, offsets)
-            y = gemm_fp8_block_out(h, h_scale, self.down_codes, self.down_scales, offsets)
-            return expert_combine_out(y, w, row_slot, slot_row).view(*x.shape[:-1], self.k_out)
-        xs = expert_gather(x2, row_slot, slot_row)
+            a, a_scale = getattr(routed, "expert_gather_fp8" + out_form)(x2, row_slot, slot_row)
+            h, h_scale = getattr(fp8_block, "gemm_swiglu_fp8_block" + out_form)(a, a_scale, self.gate_up_codes,
+                                                                                self.gate_up_scales, offsets)
+            y = getattr(fp8_block, "gemm_fp8_block" + out_form)(h, h_scale, self.down_codes, self.down_scales, offsets)
+            return routed.expert_combine(y, w, row_slot, slot_row).view(*x.shape[:-1], self.k_out)
+        xs = routed.expert_gather(x2, row_slot, slot_row)
         bounds = offsets.tolist()
         parts = []
         for e, (wg, wd) in enumerate(zip(self.w_gate_up.unbind(0), self.w_down.unbind(0))):
@@ -65,4 +67,4 @@ class RoutedSwiGLUMLP(torch.nn.Module):
             if hi > lo or (bounds[-1] == 0 and e == 0):  # without any routed row one empty call keeps the gradients zeros
                 parts.append(F.linear(gemm_swiglu_auto(xs[lo:hi], wg), wd))
         parts.append(xs.new_zeros((xs.shape[0] - bounds[-1], self.k_out)))  # rows without an expert
-        return expert_combine(torch.cat(parts), w, row_slot, slot_row).view(*x.shape[:-1], self.k_out)
+        return routed.expert_combine(torch.cat(parts), w, row_slot, slot_row).view(*x.shape[:-1], self.k_out)

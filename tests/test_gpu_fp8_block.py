@@ -233,6 +233,44 @@ def test_the_same_bits_every_time(M, N, K, E):
                 assert torch.equal(x.float(), y.float())
 
 
+def test_offsets_past_32_bits():
+    """An output of more than 2^31 elements: its last rows equal those of a call on them alone (whole tiles either way)."""
+    M, N, K = 262144 + 300, 8192, 128
+    t = case(M, N, K)
+    assert M * N > 2 ** 31
+    c = mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"])
+    tail = mb.gemm_fp8_block(t["a"][-812:], t["a_scale"][-812:], t["b"], t["b_scale"])
+    assert torch.equal(c[-812:], tail)
+    del c
+    t = case(M, N, K, halves=2)
+    codes, scales = mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"])
+    tail = mb.gemm_swiglu_fp8_block(t["a"][-812:], t["a_scale"][-812:], t["b"], t["b_scale"])
+    assert torch.equal(codes[-812:].float(), tail[0].float()) and torch.equal(scales[-812:], tail[1])
+
+
+def test_two_streams_at_once_and_beside_the_bf16_kernels():
+    """Calls that overlap on the GPU share nothing: split and unsplit forms on two streams, the bf16 op between them."""
+    small, large = case(24, 1024, 8192, seed=1), case(600, 1024, 8192, halves=2, seed=2)
+    x = torch.randn(600, 1024, generator=gen(3), device="cuda").to(BF)
+    w = (0.05 * torch.randn(2048, 1024, generator=gen(4), device="cuda")).to(BF)
+    calls = [lambda: (mb.gemm_fp8_block(small["a"], small["a_scale"], small["b"], small["b_scale"]),),
+             lambda: mb.gemm_swiglu_fp8_block(large["a"], large["a_scale"], large["b"], large["b_scale"]),
+             lambda: (mb.gemm_swiglu(x, w),)]
+    want = [[o.float() for o in call()] for call in calls]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for turn in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(((i + turn) % 3, calls[(i + turn) % 3]()))
+    torch.cuda.synchronize()
+    for i, outs in got:
+        assert all(torch.equal(o.float(), ref) for o, ref in zip(outs, want[i]))
+    assert mb.device_status(0)["code"] == 0
+
+
 def routed_block(s):
     row_slot, slot_row, offsets = mb.expert_sort_out(s["ids"], s["w2"].shape[0])
     a, sc = mb.expert_gather_fp8_out(s["x"], row_slot, slot_row)

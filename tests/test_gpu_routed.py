@@ -362,3 +362,25 @@ def test_out_arguments():
     assert mb.quantize_fp8_block_out(x, out=(codes, scales))[0] is codes
     with pytest.raises(TypeError, match="CUDA tensors only"):
         mb.expert_gather_out(x, out[0].cpu(), out[1])
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements on the experts' side: the last rows are right in every direction."""
+    T, k, H, E = 66000, 4, 8192, 16
+    ids = torch.randint(0, E, (T, k), generator=torch.Generator().manual_seed(1)).cuda()
+    row_slot, slot_row, _ = mb.expert_sort(ids, E)
+    assert T * k * H > 2 ** 31
+    x = torch.randn(T, 1, generator=torch.Generator().manual_seed(2)).to(BF).cuda().expand(T, H).contiguous()
+    xs = mb.expert_gather(x, row_slot, slot_row)
+    assert torch.equal(xs[:, 0], x[row_slot.long() // k, 0]) and torch.equal(xs[:, -1], xs[:, 0])
+    w = torch.full((T, k), 0.25, device="cuda")
+    assert torch.equal(mb.expert_combine(xs, w, row_slot, slot_row), x)
+    dy, dw = mb.expert_combine_backward(x, xs, w, row_slot, slot_row, True, True)
+    assert torch.equal(dy[:, 0], (0.25 * xs[:, 0]).to(BF)) and torch.equal(dy[:, -1], dy[:, 0])
+    want = (x[:, 0].double() ** 2 * H)[:, None].expand(T, k)
+    assert ((dw.double() - want).abs() <= want * (H + 1) * 2.0 ** -24).all()
+    del dy, dw, xs
+    codes, scales = mb.expert_gather_fp8(x, row_slot, slot_row)
+    full = mb.quantize_fp8_block(x)
+    assert torch.equal(codes[:, -1].float(), full[0][row_slot.long() // k, -1].float())
+    assert torch.equal(scales[:, -1], full[1][row_slot.long() // k, -1])

@@ -1,9 +1,14 @@
 """``RoutedSwiGLUMLP``: the routed operators and the experts' products as a user runs them, forward, gradients, fp8, graph."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
 import magicompiler_b200 as mb
 
+ROOT = Path(__file__).resolve().parent.parent
 BF = torch.bfloat16
 
 
@@ -93,6 +98,24 @@ def test_fp8_forward(shape, k, E, K, N, drop):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("precision", ["bf16", "fp8"])
+def test_no_tokens(precision):
+    mlp = mb.RoutedSwiGLUMLP(*weights(3, 64, 128, 128, 1, "cuda"), precision=precision)
+    out = mlp(*batch((0,), 2, 3, 128, 1))
+    assert out.shape == (0, 128) and out.dtype == BF
+
+
+@pytest.mark.gpu
+def test_compiled_fp8_forward():
+    """Under torch.compile the block is made of the registered ops: the same bits as the direct calls."""
+    mlp = mb.RoutedSwiGLUMLP(*weights(4, 128, 256, 256, 2, "cuda"), precision="fp8")
+    args = batch((30,), 2, 4, 256, 3, 0.1)
+    compiled = torch.compile(mlp, backend="aot_eager", fullgraph=True)
+    with torch.no_grad():
+        assert torch.equal(compiled(*args), mlp(*args))
+
+
+@pytest.mark.gpu
 def test_fp8_forward_captured_on_a_stream():
     w13, w2 = weights(8, 256, 256, 256, 6, "cuda")
     mlp = mb.RoutedSwiGLUMLP(w13, w2, precision="fp8")
@@ -110,6 +133,30 @@ def test_fp8_forward_captured_on_a_stream():
             dst.copy_(src)
         graph.replay()
         assert torch.equal(out, mlp(x, ids, w))
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_process_inside_a_capture():
+    """Whatever the library looks up once per device it may look up while a stream is being captured."""
+    code = """
+import torch, magicompiler_b200 as mb
+torch.manual_seed(0)
+w13, w2 = torch.randn(4, 512, 2048).bfloat16().cuda(), torch.randn(4, 2048, 256).bfloat16().cuda()
+mlp = mb.RoutedSwiGLUMLP(w13 * 0.02, w2 * 0.05, precision="fp8")
+for T in (5, 1200):
+    x, w = torch.randn(T, 2048).bfloat16().cuda(), torch.rand(T, 2).cuda()
+    ids = torch.randint(0, 4, (T, 2)).cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = mlp(x, ids, w)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, mlp(x, ids, w))
+assert mb.device_status(0)["code"] == 0
+print("captured")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
 
 
 @pytest.mark.gpu
