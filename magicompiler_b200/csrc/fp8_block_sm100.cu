@@ -196,11 +196,15 @@ static int run(const Problem& p, int device, void* cuda_stream) {
   // SwiGLU form, about 0.6 of that with one CTA an SM; tile kernel 0.42 a K block and 2.5 a tile.  Both sides at N = 4096,
   // K = 14336 (stream 16 / 32 / 64 tokens, tiles): M = 64 26 / 18 / 16 / 35 us, 256 - / 47 / 35 / 35 us, 512 - / - / 58 /
   // 37 us; SwiGLU, N = 1408, K = 2048, 64 experts (16 / 32 tokens, tiles): 512 rows 52 / 48 / 78 us, 2048 rows 85 / 75 / 96
-  // us, 8192 rows 295 / 199 / 138 us.  A cluster's CTAs split K while the tiles leave SMs idle.
+  // us, 8192 rows 295 / 199 / 138 us.  None is faster than W's bytes (6.2 TB/s).  Forms that are bound by them alike differ
+  // in what an uneven share costs: then the wider tile, up to 2.5 times the average share (8 experts, 74 rows, N = 4096, K =
+  // 14336: 16 tokens 69 to 87 us from routing to routing, 32 tokens 69 to 74 us).
   int clusters[3];
   if (int rc = p.halves == 1 ? tile_clusters<1>(device, di->sm_count, clusters) : tile_clusters<2>(device, di->sm_count, clusters))
     return rc;
   const double n128 = (double)((p.N + 127) / 128);
+  const double used = p.args.offsets ? (double)(p.M < p.args.E ? p.M : p.args.E) : 1.0, share = p.M / used;
+  const double bytes_us = used * p.halves * p.N * p.K / 6.2e6 + 3.0;
   double best = 0;
   int tok = 0, splits = 1;
   {
@@ -208,17 +212,19 @@ static int run(const Problem& p, int device, void* cuda_stream) {
     const int log_splits = tile_log_splits(most_groups(p, kTileRows) * n_tiles, p.args.kb, clusters);
     const double rounds = ceil(expected_groups(p, kTileRows) * n_tiles / clusters[log_splits]);
     best = 5.0 + rounds * (p.args.kb * 0.42 / (1 << log_splits) + 2.5) + (log_splits ? 3.0 : 0.0);
+    if (best < bytes_us) best = bytes_us;
   }
   const int forms = p.halves == 1 ? 3 : 2;
   static const double per_block[2][3] = {{0.36, 0.43, 0.50}, {0.75, 0.90, 0.0}};
   for (int i = 0; i < forms; ++i) {
     if (most_groups(p, 16 << i) > 65535) continue;
     const double ctas = n128 * expected_groups(p, 16 << i);
-    int z = 1;  // up to eight CTAs share a tile's K blocks, at least four each, until there are about two CTAs an SM
+    int z = 1;  // up to eight CTAs of a cluster share a tile's K blocks, at least four each, until there are about two CTAs an SM
     while (z < 8 && ctas * z * 2 <= 2 * di->sm_count && p.args.kb >= z * 8) z *= 2;
     const double rounds = ceil(ctas * z / (2 * di->sm_count));
-    const double cost = 2.5 + rounds * (p.args.kb * per_block[p.halves - 1][i] / z * (ctas * z <= di->sm_count ? 0.6 : 1.0) + 2.5);
-    if (cost < best) best = cost, tok = 16 << i, splits = z;
+    double cost = 2.5 + rounds * (p.args.kb * per_block[p.halves - 1][i] / z * (ctas * z <= di->sm_count ? 0.6 : 1.0) + 2.5);
+    if (cost < bytes_us) cost = bytes_us;
+    if (cost < best || (cost == best && (tok == 0 || (p.args.offsets && tok < 2.5 * share)))) best = cost, tok = 16 << i, splits = z;
   }
   if (p.halves == 1) {
     if (tok == 16) return launch_stream<1, 16>(p, device, splits, stream);
