@@ -101,38 +101,40 @@ struct Unit {  // rows [row0, row0 + rows) of expert e; e == E: rows behind the 
   int e, row0, rows;
 };
 
-// The unit-th group of at most kTok rows, counting every expert's groups in order (one whole warp calls this).  Offsets are
-// clamped to [0, R], so that a bad array cannot lead outside the operands.
+// First row of expert e, e == E: of the rows behind the last expert's.  Clamped to [0, R], so that a bad array cannot lead
+// outside the operands; without offsets one expert has all rows.
+__device__ __forceinline__ int start_of(const Args& a, int e) {
+  return a.offsets ? min(max(a.offsets[e], 0), a.R) : (e == 0 ? 0 : a.R);
+}
+__device__ __forceinline__ int warp_scan(int n) {  // inclusive sum over the warp's lanes
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, n, d);
+    if (lane >= d) n += up;
+  }
+  return n;
+}
+
+// The unit-th group of at most kTok rows, counting every expert's groups in order (one whole warp calls this).
 template <int kTok>
 __device__ __forceinline__ Unit find_unit(const Args& a, int unit) {
-  if (!a.offsets) {
-    const long long r0 = (long long)unit * kTok;
-    return r0 < a.R ? Unit{0, (int)r0, min(kTok, a.R - (int)r0)} : Unit{0, 0, 0};
-  }
   const int lane = threadIdx.x & 31;
   int seen = 0;
   for (int b = 0; b <= a.E; b += 32) {
     const int e = b + lane;
     int lo = 0, len = 0, n = 0;
     if (e <= a.E) {
-      lo = min(max(a.offsets[e], 0), a.R);
-      const int hi = e < a.E ? min(max(a.offsets[e + 1], lo), a.R) : a.R;
-      len = hi - lo;
+      lo = start_of(a, e);
+      len = e < a.E ? max(start_of(a, e + 1) - lo, 0) : a.R - lo;
       n = (e == a.E && !a.zero_tail) ? 0 : (len + kTok - 1) / kTok;
     }
-    int scan = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, scan, d);
-      if (lane >= d) scan += up;
-    }
-    const bool mine = n > 0 && unit >= seen + scan - n && unit < seen + scan;
-    const unsigned hit = __ballot_sync(0xffffffffu, mine);
+    const int scan = warp_scan(n);
+    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && unit >= seen + scan - n && unit < seen + scan);
     if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int first = __shfl_sync(0xffffffffu, lo, src), all = __shfl_sync(0xffffffffu, len, src);
-      const int i = unit - seen - __shfl_sync(0xffffffffu, scan - n, src);
-      return Unit{b + src, first + i * kTok, min(kTok, all - i * kTok)};
+      const int src = __ffs(hit) - 1, i = unit - seen - __shfl_sync(0xffffffffu, scan - n, src);
+      const int first = __shfl_sync(0xffffffffu, lo, src), rows = __shfl_sync(0xffffffffu, len, src);
+      return Unit{b + src, first + i * kTok, min(kTok, rows - i * kTok)};
     }
     seen += __shfl_sync(0xffffffffu, scan, 31);
   }
@@ -179,6 +181,9 @@ constexpr int kStreamThreads = 192;  // warps 0-3 epilogue (one tensor-memory la
 // kTok 16, 32 or (plain) 64 tokens a tile: two CTAs share an SM.  (Tiles of 64 tokens in the SwiGLU form and of 128 in the
 // plain one leave registers for one CTA an SM only and lost to the smaller ones everywhere.)  kBufs accumulator buffers: a
 // buffer's way from the MMA through the epilogue and back takes about 700 cycles besides the MMA itself, which takes 400.
+// Blocks set up (barriers, tensor memory, descriptors) while the previous kernel drains: 75.8 to 72.7 us back to back for 16
+// tokens, K 8192, N 28672; a routed fp8 block in a graph 68.7 to 66.4 us (1 token, 2 of 8 experts, K 4096, N 14336), 25.0
+// to 24.2 (8 of 128, K 2048, N 768), but 205 to 209 for 64 tokens, 8 of 256 experts.
 template <int kHalves, int kTok>
 __global__ void __launch_bounds__(kStreamThreads, 2)
 fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const Args a) {
@@ -205,10 +210,6 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
   const int split = a.splits > 1 ? (int)cluster_ctarank() : 0;
   const int n0 = (int)(blockIdx.x / a.splits) * kRowsW;
 
-  if (warp == 4) {
-    const Unit u = find_unit<kTok>(a, blockIdx.y);
-    if (lane == 0) unit_slot = u;
-  }
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < a.stages; ++s) {
@@ -225,9 +226,16 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
     tmem_alloc<1>(smem_u32(&tmem_slot), kTmem);
     tmem_relinquish<1>();
   }
+  if (warp == 4) {
+    grid_dependency_wait();
+    const Unit found = find_unit<kTok>(a, blockIdx.y);
+    if (lane == 0) unit_slot = found;
+  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  grid_launch_dependents();  // after the allocation: a later kernel cannot take the tensor memory this one still needs
+  grid_dependency_wait();
   const uint32_t tmem = tmem_slot;
   const Unit u = unit_slot;
   const bool live = u.rows > 0 && u.e < a.E;  // the same for every CTA of a cluster
@@ -291,10 +299,10 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int c = (threadIdx.x >> 2) + 32 * i;
-        next[i] = (c < u.rows && c < kTok && b < kb1) ? __ldg(a.a_scale + (long long)(u.row0 + c) * a.ld_as + b) : 0.0f;
+        next[i] = (c < u.rows && c < kTok && b < kb1) ? a.a_scale[(long long)(u.row0 + c) * a.ld_as + b] : 0.0f;
       }
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) next_w[h] = b < kb1 ? __ldg(ws + (long long)h * a.nb * a.kb + b) : 0.0f;
+      for (int h = 0; h < kHalves; ++h) next_w[h] = b < kb1 ? ws[(long long)h * a.nb * a.kb + b] : 0.0f;
     };
     fetch(kb0);
     const uint32_t lane_base = tmem + ((uint32_t)(warp * 32) << 16);
@@ -427,6 +435,7 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
 // half of W's, 32 KB per K block for 512 cycles of MMA.  A thread of the epilogue owns one row, so its scale is one number
 // per 128 columns and an addition is one fused multiply-add; with 128 of them per thread and block, two epilogue warps a
 // scheduler keep up with the MMA (half of the issue slots) and the registers for them come from the other warpgroup.
+// It is launched without programmatic overlap (the extra wait changes the loop's instruction schedule for the worse).
 // Persistent: tiles go round-robin to the pairs in bands of row groups, column tile by column tile, so that the
 // pairs that run together share A rows and W rows in L2.
 // Few tiles: `splits` (2 or 4) pairs form a cluster and share a tile's K blocks.  At the end each pair keeps the rows of

@@ -79,19 +79,8 @@ static int launch_stream(const Problem& p, int device, int splits, cudaStream_t 
   static int smem_set[kMaxDevices];
   cudaError_t e = allow_smem_once(fp8_block_stream_kernel<kHalves, kTok>, kSmem, device, smem_set);
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)args.splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(n_tiles * args.splits), (unsigned)groups);
-  cfg.blockDim = dim3(kStreamThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = args.splits > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, fp8_block_stream_kernel<kHalves, kTok>, tm_w, tm_a, args);
+  e = launch(fp8_block_stream_kernel<kHalves, kTok>, dim3((unsigned)(n_tiles * args.splits), (unsigned)groups),
+             dim3(kStreamThreads), kSmem, stream, (unsigned)args.splits, true, tm_w, tm_a, args);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_stream_kernel");
 }
 
@@ -155,18 +144,6 @@ static int launch_tiles(const Problem& p, const int (&clusters)[3], cudaStream_t
   const int64_t n_tiles = (p.N + 256 / kHalves - 1) / (256 / kHalves);
   const int64_t units = most_groups(p, kTileRows);
   if (units * n_tiles > 0x7fffffffLL / 2) return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld x N=%lld is too large for one launch", (long long)p.M, (long long)p.N);
-  auto kernel = fp8_block_tile_kernel<kHalves>;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kTileThreads);
-  cfg.dynamicSmemBytes = kTileSmem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   const int64_t most = units * n_tiles;
   const int log_splits = tile_log_splits(most, p.args.kb, clusters);
   Args args = p.args;
@@ -176,10 +153,9 @@ static int launch_tiles(const Problem& p, const int (&clusters)[3], cudaStream_t
   const int64_t band = (32LL << 20) / (kTileRows * p.K);
   args.band = (int)(band < 4 ? 4 : (band > 64 ? 64 : band));
   const int64_t workers = most < clusters[log_splits] ? most : clusters[log_splits];
-  attr[0].val.clusterDim.x = 2u << log_splits;
-  cfg.gridDim = dim3((unsigned)(workers * (2 << log_splits)));
   const int wide = ((uintptr_t)p.args.c & 31u) == 0 && p.N % 16 == 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_a, args, wide);
+  const cudaError_t e = launch(fp8_block_tile_kernel<kHalves>, dim3((unsigned)(workers * (2 << log_splits))),
+                               dim3(kTileThreads), kTileSmem, stream, 2u << log_splits, false, tm_w, tm_a, args, wide);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_tile_kernel");
 }
 

@@ -9,6 +9,9 @@
 // read ONCE however many experts it goes to (the kernels walk tokens, not sorted rows), that accesses are 16 bytes wide
 // and contiguous per row, and that a call is one launch.  Indices read from memory are bounds-checked: one that is out of
 // range counts as "no expert", so a bad index array gives wrong rows but no access outside the operands.
+// Every kernel may be scheduled while the previous one drains and waits for it before its first access to global memory
+// (gather of 8192 rows of 4096 for two experts each 35.5 to 34.4 us back to back, quantiser of 8192 x 4096 17.7 to 17.4,
+// of 2005 x 2064 for eight experts 9.05 to 8.55).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -77,6 +80,8 @@ expert_sort_kernel(const void* ids, int wide, int R, int E, int* row_slot, int* 
   const int lo = (int)(first < R ? first : R), hi = (int)(first + share < R ? first + share : R);
 
   for (int i = threadIdx.x; i < warps * buckets; i += blockDim.x) sort_smem[i] = 0;
+  grid_launch_dependents();
+  grid_dependency_wait();
   // the first steps' keys and matches stay in registers for the second pass
   int key[kSortKeep];
   unsigned same[kSortKeep];
@@ -183,12 +188,20 @@ __device__ __forceinline__ RowPiece row_piece(int col_chunks) {
   p.c = (blockIdx.x % col_chunks) * blockDim.x + threadIdx.x;
   return p;
 }
-__device__ __forceinline__ uint4 ld_stream(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
+// A load of data that is used once.  Volatile, so that it stays behind grid_dependency_wait (the compiler may move a
+// read-only load or the intrinsic in front of it).
+__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 
 // xs[slot_row[t, j]] = x[t]; row t * k + j is zeroed when it holds no slot.
 __global__ void __launch_bounds__(256)
 expert_gather_kernel(const uint4* x, long long ldx, const int* row_slot, const int* slot_row, uint4* xs, long long T, int k,
                      int vecs, int col_chunks) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   const RowPiece p = row_piece(col_chunks);
   if (p.t >= T || p.c >= vecs) return;
   const long long R = T * k;
@@ -225,6 +238,8 @@ template <int kSlots, int kPieces>
 __global__ void __launch_bounds__(256, 3)
 expert_combine_kernel(const uint4* y, long long ldy, const float* w, const int* slot_row, uint4* out, long long T, int k,
                       int vecs, int col_chunks) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   const long long t = (long long)(blockIdx.x / col_chunks) * blockDim.y + threadIdx.y;
   const int c0 = (blockIdx.x % col_chunks) * blockDim.x * kPieces + threadIdx.x;
   if (t >= T) return;
@@ -279,6 +294,8 @@ expert_combine_backward_kernel(const uint4* dout, long long lddout, const uint4*
                                const int* row_slot, const int* slot_row, uint4* dy, float* dw, long long T, int k, int vecs,
                                int token_warps) {
   __shared__ float red[8][kSlotBatch];
+  grid_launch_dependents();
+  grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = warp % token_warps;
   const long long t = (long long)blockIdx.x * (8 / token_warps) + warp / token_warps;
@@ -377,6 +394,8 @@ __device__ __forceinline__ void quotients(float& x0, float& x1, uint64_t minus_s
 __global__ void __launch_bounds__(256)
 quantize_fp8_block_kernel(const uint4* x, long long ldx, const int* row_slot, const int* slot_row, uint4* codes,
                           float* scales, long long T, int k, int pieces, int col_chunks, int kb) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   const RowPiece p = row_piece(col_chunks);
   const bool on = p.t < T && p.c < pieces;
   uint4 a = make_uint4(0, 0, 0, 0), b = a;

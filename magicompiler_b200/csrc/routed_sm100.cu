@@ -76,10 +76,9 @@ static int quantize(const void* x, const int32_t* row_slot, const int32_t* slot_
   DeviceGuard guard;
   cudaError_t e = guard.set(device);
   if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
-  quantize_fp8_block_kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint4*>(x), ldx / 8, row_slot, slot_row, static_cast<uint4*>(codes), scales, T, (int)k,
-      (int)(K / 16), g.col_chunks, (int)((K + 127) / 128));
-  e = cudaGetLastError();
+  e = launch(quantize_fp8_block_kernel, dim3(g.grid), g.block, 0, static_cast<cudaStream_t>(stream), 1u, true,
+             static_cast<const uint4*>(x), ldx / 8, row_slot, slot_row, static_cast<uint4*>(codes), scales, T,
+             (int)k, (int)(K / 16), g.col_chunks, (int)((K + 127) / 128));
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of quantize_fp8_block_kernel");
 }
 
@@ -120,20 +119,9 @@ int magi_swiglu_expert_sort(const void* ids, int ids_64bit, int64_t slots, int n
   int warps = (int)((all_warps + ctas - 1) / ctas);
   warps = warps < 4 ? 4 : (warps > 32 ? 32 : warps);
   const size_t smem = (size_t)(warps + 3) * (num_experts + 1) * sizeof(int);
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3((unsigned)warps * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = static_cast<cudaStream_t>(cuda_stream);
-  cfg.attrs = attr;
-  cfg.numAttrs = ctas > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, expert_sort_kernel, ids, ids_64bit, (int)slots, num_experts, (int*)row_slot, (int*)slot_row,
-                         (int*)offsets, ctas);
+  e = launch(expert_sort_kernel, dim3((unsigned)ctas), dim3((unsigned)warps * 32), smem,
+             static_cast<cudaStream_t>(cuda_stream), (unsigned)ctas, true, ids, ids_64bit, (int)slots, num_experts,
+             (int*)row_slot, (int*)slot_row, (int*)offsets, ctas);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_sort_kernel");
 }
 
@@ -151,10 +139,9 @@ int magi_swiglu_expert_gather_bf16(const void* x, const int32_t* row_slot, const
   DeviceGuard guard;
   cudaError_t e = guard.set(device);
   if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
-  expert_gather_kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
-      static_cast<const uint4*>(x), ldx / 8, row_slot, slot_row, static_cast<uint4*>(xs), T, (int)k, (int)(H / 8),
-      g.col_chunks);
-  e = cudaGetLastError();
+  e = launch(expert_gather_kernel, dim3(g.grid), g.block, 0, static_cast<cudaStream_t>(cuda_stream), 1u, true,
+             static_cast<const uint4*>(x), ldx / 8, row_slot, slot_row, static_cast<uint4*>(xs), T, (int)k,
+             (int)(H / 8), g.col_chunks);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_gather_kernel");
 }
 
@@ -176,10 +163,9 @@ int magi_swiglu_expert_combine_bf16(const void* y, const float* weights, const i
   if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
   auto kernel = k <= 1 ? expert_combine_kernel<1, 4> : k <= 2 ? expert_combine_kernel<2, 4>
                 : k <= 4 ? expert_combine_kernel<4, 2> : expert_combine_kernel<8, 1>;
-  kernel<<<g.grid, g.block, 0, static_cast<cudaStream_t>(cuda_stream)>>>(static_cast<const uint4*>(y), ldy / 8, weights,
-                                                                         slot_row, static_cast<uint4*>(out), T, (int)k,
-                                                                         (int)(H / 8), g.col_chunks);
-  e = cudaGetLastError();
+  e = launch(kernel, dim3(g.grid), g.block, 0, static_cast<cudaStream_t>(cuda_stream), 1u, true,
+             static_cast<const uint4*>(y), ldy / 8, weights, slot_row, static_cast<uint4*>(out), T, (int)k,
+             (int)(H / 8), g.col_chunks);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_combine_kernel");
 }
 
@@ -203,10 +189,10 @@ int magi_swiglu_expert_combine_backward_bf16(const void* dout, const void* y, co
   int token_warps = 1;
   while (token_warps < 8 && T * token_warps < (int64_t)di->sm_count * 32 && H / 8 > token_warps * 32) token_warps *= 2;
   const int64_t blocks = (T + 8 / token_warps - 1) / (8 / token_warps);
-  expert_combine_backward_kernel<<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
-      static_cast<const uint4*>(dout), lddout / 8, static_cast<const uint4*>(y), ldy / 8, weights, row_slot, slot_row,
-      static_cast<uint4*>(dy), dw, T, (int)k, (int)(H / 8), token_warps);
-  e = cudaGetLastError();
+  e = launch(expert_combine_backward_kernel, dim3((unsigned)blocks), dim3(256), 0,
+             static_cast<cudaStream_t>(cuda_stream), 1u, true, static_cast<const uint4*>(dout), lddout / 8,
+             static_cast<const uint4*>(y), ldy / 8, weights, row_slot, slot_row, static_cast<uint4*>(dy), dw, T,
+             (int)k, (int)(H / 8), token_warps);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of expert_combine_backward_kernel");
 }
 

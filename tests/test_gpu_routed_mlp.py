@@ -136,6 +136,60 @@ def test_fp8_forward_captured_on_a_stream():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_back_to_back_calls_that_reuse_every_buffer(captured):
+    """Kernels may be scheduled while the previous one drains: each has to see its writes, and must not write too early."""
+    E, k, T, H, N = 8, 2, 24, 512, 256
+    w13, w2 = weights(E, N, H, H, 7, "cuda")
+    qw, qws = mb.quantize_fp8_weight(w13)
+    qd, qds = mb.quantize_fp8_weight(w2)
+    inputs = [batch((T,), k, E, H, 100 + i, drop=0.1) for i in range(6)]
+    R = T * k
+    f8 = torch.float8_e4m3fn
+    xq, hq = torch.empty(R, H, dtype=f8, device="cuda"), torch.empty(R, N, dtype=f8, device="cuda")
+    xs, hs = torch.empty(R, H // 128, device="cuda"), torch.empty(R, N // 128, device="cuda")
+    y, x, ids, rw = (torch.empty(R, H, dtype=BF, device="cuda"), torch.empty_like(inputs[0][0]),
+                     torch.empty_like(inputs[0][1]), torch.empty_like(inputs[0][2]))
+    index = [torch.empty(R, dtype=torch.int32, device="cuda"), torch.empty(T, k, dtype=torch.int32, device="cuda"),
+             torch.empty(E + 1, dtype=torch.int32, device="cuda")]
+    out = [torch.empty(T, H, dtype=BF, device="cuda") for _ in inputs]
+
+    def run(i, wait=lambda: None):
+        for d, s in zip((x, ids, rw), inputs[i]):
+            d.copy_(s)
+        wait()
+        rs, sr, off = mb.expert_sort_out(ids, E, out=index)
+        wait()
+        mb.expert_gather_fp8_out(x, rs, sr, out=(xq, xs))
+        wait()
+        mb.gemm_swiglu_fp8_block_out(xq, xs, qw, qws, off, out=(hq, hs))
+        wait()
+        mb.gemm_fp8_block_out(hq, hs, qd, qds, off, out=y)
+        wait()
+        mb.expert_combine_out(y, rw, rs, sr, out=out[i])
+        wait()
+
+    for b in (xq, hq, xs, hs, y):
+        b.zero_()
+    want = []
+    for i in range(len(inputs)):
+        run(i, torch.cuda.synchronize)
+        want.append(out[i].clone())
+    steps = lambda: [run(i) for i in range(len(inputs))]
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            steps()
+        steps = graph.replay
+    for _ in range(20):
+        for o in out:
+            o.zero_()
+        steps()
+        for o, r in zip(out, want):
+            assert torch.equal(o, r)
+
+
+@pytest.mark.gpu
 def test_first_call_of_a_process_inside_a_capture():
     """Whatever the library looks up once per device it may look up while a stream is being captured."""
     code = """
