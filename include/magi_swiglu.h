@@ -272,7 +272,7 @@ int magi_swiglu_backward_dh_bf16(const void* x, const void* w_gate_up, const voi
 /* ---- Routed (mixture-of-experts) rows.  T tokens choose k experts each: slot s = t * k + j, R = T * k slots.
  * row_slot[r] = s says which slot sorted row r holds (-1: none), slot_row[s] = r is its inverse (-1: slot s has no
  * expert).  Index arrays are int32 in device memory; entries are bounds-checked by the kernels (out of range = none).
- * Outputs are contiguous; H is the row length.  T == 0 is a successful no-op (the sort still writes its offsets). */
+ * Outputs are contiguous and overlap no input; H is the row length.  T == 0 is a successful no-op (the sort still writes its offsets). */
 
 /* Stable counting sort of `slots` expert ids (int32, or int64 when ids_64bit) into num_experts (<= 1024) contiguous row
  * ranges: rows [offsets[e], offsets[e+1]) hold expert e's slots in slot order; ids outside [0, num_experts) have no
@@ -317,7 +317,7 @@ int magi_swiglu_expert_gather_fp8_block(const void* x, const int32_t* row_slot, 
  * device memory, the first one 0; the kernel clamps them to [0, M], they must not decrease) rows [offsets[e], offsets[e+1]) of A meet B[e];
  * rows from offsets[num_experts] on are written as zeros when zero_tail is set and left as they are otherwise.  Without
  * offsets num_experts is 1.  Sums are fp32.  K % 16 == 0, lda % 16 == 0, 16-byte aligned a, b, c, codes; B and the outputs
- * are contiguous.  M == 0 is a successful no-op.  Rows of A with a NaN scale or code give NaN. */
+ * are contiguous, the outputs overlap no input.  M == 0 is a successful no-op.  Rows of A with a NaN scale or code give NaN. */
 
 /* C[M, N] (bf16, one rounding) = sum over K blocks of a_scale * b_scale * (A codes . B codes^T): A [M, K], B
  * [num_experts, N, K], b_scale [num_experts, ceil(N/128), ceil(K/128)].  N % 8 == 0.

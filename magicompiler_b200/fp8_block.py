@@ -27,7 +27,7 @@ import torch
 from . import _loader
 from .ops import _raw_stream
 from .register import magi_register_custom_op
-from .routed import BLOCK, FP8_MAX, SCALE_FLOOR, _check_device, _raise, _result
+from .routed import BLOCK, FP8_MAX, SCALE_FLOOR, _check_device, _fp8_block_outputs, _raise, _result
 
 GEMM_OP_NAME = "magi_swiglu::gemm_fp8_block"
 SWIGLU_OP_NAME = "magi_swiglu::gemm_swiglu_fp8_block"
@@ -63,7 +63,7 @@ def quantize_fp8_gate_up(w_gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.T
     """``(codes, scales)`` of a packed gate/up weight ``[2N, K]`` or ``[E, 2N, K]`` (``pack_gate_up``) for
     ``gemm_swiglu_fp8_block``: each half is cut into blocks from its own first row, ``scales [.., 2 * ceil(N/128),
     ceil(K/128)]`` hold the gate half's blocks, then the up half's."""
-    if w_gate_up.shape[-2] % 2:
+    if w_gate_up.dim() in (2, 3) and w_gate_up.shape[-2] % 2:
         raise ValueError(f"w_gate_up has {w_gate_up.shape[-2]} rows; it must hold N gate rows followed by N up rows")
 
     def halves(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -135,7 +135,7 @@ def gemm_fp8_block_out(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, 
                        offsets: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """The body of ``gemm_fp8_block``.  With ``out`` the rows from ``offsets[E]`` on are left as they were."""
     m, n, k, experts, dev = _check("gemm_fp8_block", a, a_scale, b, b_scale, offsets, 1)
-    c = _result("gemm_fp8_block", out, (m, n), torch.bfloat16, a.device)
+    c = _result("gemm_fp8_block", out, (m, n), torch.bfloat16, a.device, a, a_scale, b, b_scale, offsets)
     if m == 0:
         return c
     a2, lda, s2, lds = _operand(a, a_scale)
@@ -165,9 +165,7 @@ def gemm_swiglu_fp8_block_out(a: torch.Tensor, a_scale: torch.Tensor, w_gate_up:
     were."""
     name = "gemm_swiglu_fp8_block"
     m, n, k, experts, dev = _check(name, a, a_scale, w_gate_up, w_scale, offsets, 2)
-    codes, scales = out if out is not None else (None, None)
-    codes = _result(name, codes, (m, n), torch.float8_e4m3fn, a.device)
-    scales = _result(name, scales, (m, -(-n // BLOCK)), torch.float32, a.device)
+    codes, scales = _fp8_block_outputs(name, out, m, n, a.device, a, a_scale, w_gate_up, w_scale, offsets)
     if m == 0:
         return codes, scales
     a2, lda, s2, lds = _operand(a, a_scale)

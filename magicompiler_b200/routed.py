@@ -41,14 +41,25 @@ def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else _rows_view(t, cols)
 
 
-def _result(name: str, out: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype,
-            device: torch.device) -> torch.Tensor:
-    """``out`` if it is what the kernel can write (contiguous, 16-byte aligned), a new tensor if it is None."""
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First byte of ``t`` and the byte behind its last."""
+    elements = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + elements * t.element_size()
+
+
+def _result(name: str, out: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype, device: torch.device,
+            *others: torch.Tensor | None) -> torch.Tensor:
+    """``out`` if it is what the kernel can write (contiguous, 16-byte aligned, apart from ``others``, the operands and the
+    call's other results), a new tensor if it is None."""
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
     if out.dtype != dtype or out.device != device or tuple(out.shape) != shape or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError(f"{name}: out must be a contiguous, 16-byte-aligned {dtype} tensor of shape {shape} on {device}")
+    lo, hi = _span(out)
+    for t in others:
+        if t is not None and _span(t)[0] < hi and lo < _span(t)[1]:
+            raise ValueError(f"{name}: out must not overlap an operand or another result")
     return out
 
 
@@ -80,9 +91,9 @@ def expert_sort_out(expert_ids: torch.Tensor, num_experts: int,
         slot_row = torch.empty(ids.shape, dtype=torch.int32, device=device)
         offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=device)
     else:
-        row_slot = _result("expert_sort", out[0], (slots,), torch.int32, device)
-        slot_row = _result("expert_sort", out[1], tuple(ids.shape), torch.int32, device)
-        offsets = _result("expert_sort", out[2], (num_experts + 1,), torch.int32, device)
+        row_slot = _result("expert_sort", out[0], (slots,), torch.int32, device, ids)
+        slot_row = _result("expert_sort", out[1], tuple(ids.shape), torch.int32, device, ids, row_slot)
+        offsets = _result("expert_sort", out[2], (num_experts + 1,), torch.int32, device, ids, row_slot, slot_row)
     rc = _loader.load_library().magi_swiglu_expert_sort(
         ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, slots, num_experts, row_slot.data_ptr(),
         slot_row.data_ptr(), offsets.data_ptr(), dev, _raw_stream(dev))
@@ -166,7 +177,7 @@ def expert_gather_out(x: torch.Tensor, row_slot: torch.Tensor, slot_row: torch.T
     h = _check_rows("expert_gather", "x", x, tokens, 8)
     dev = _check_device("expert_gather", x, row_slot, slot_row)
     x2 = _rows(x, h)
-    xs = _result("expert_gather", out, (tokens * k, h), torch.bfloat16, x.device)
+    xs = _result("expert_gather", out, (tokens * k, h), torch.bfloat16, x.device, x, row_slot, slot_row)
     rc = _loader.load_library().magi_swiglu_expert_gather_bf16(
         x2.data_ptr(), row_slot.data_ptr(), slot_row.data_ptr(), xs.data_ptr(), tokens, k, h, _ld(x2), dev, _raw_stream(dev))
     if rc != 0:
@@ -228,7 +239,7 @@ def expert_combine_out(y: torch.Tensor, weights: torch.Tensor | None, row_slot: 
     else:
         dev = _check_device("expert_combine", y, row_slot, slot_row)
     y2 = _rows(y, h)
-    res = _result("expert_combine", out, (tokens, h), torch.bfloat16, y.device)
+    res = _result("expert_combine", out, (tokens, h), torch.bfloat16, y.device, y, weights, slot_row)
     rc = _loader.load_library().magi_swiglu_expert_combine_bf16(
         y2.data_ptr(), weights.data_ptr() if weights is not None else None, slot_row.data_ptr(), res.data_ptr(), tokens, k,
         h, _ld(y2), dev, _raw_stream(dev))
@@ -326,10 +337,10 @@ QUANTIZE_OP_NAME = "magi_swiglu::quantize_fp8_block"
 GATHER_FP8_OP_NAME = "magi_swiglu::expert_gather_fp8"
 
 
-def _fp8_block_outputs(name, out, rows, cols, device):
+def _fp8_block_outputs(name, out, rows, cols, device, *operands):
     codes, scales = out if out is not None else (None, None)
-    return (_result(name, codes, (rows, cols), torch.float8_e4m3fn, device),
-            _result(name, scales, (rows, -(-cols // BLOCK)), torch.float32, device))
+    codes = _result(name, codes, (rows, cols), torch.float8_e4m3fn, device, *operands)
+    return codes, _result(name, scales, (rows, -(-cols // BLOCK)), torch.float32, device, codes, *operands)
 
 
 def quantize_fp8_block_out(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None
@@ -338,7 +349,7 @@ def quantize_fp8_block_out(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tenso
     cols = _check_rows("quantize_fp8_block", "x", x, x.shape[0] if isinstance(x, torch.Tensor) and x.dim() else 0, 16)
     dev = _check_device("quantize_fp8_block", x)
     x2 = _rows(x, cols)
-    codes, scales = _fp8_block_outputs("quantize_fp8_block", out, x.shape[0], cols, x.device)
+    codes, scales = _fp8_block_outputs("quantize_fp8_block", out, x.shape[0], cols, x.device, x)
     rc = _loader.load_library().magi_swiglu_quantize_fp8_block(
         x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.shape[0], cols, _ld(x2), dev, _raw_stream(dev))
     if rc != 0:
@@ -364,7 +375,7 @@ def expert_gather_fp8_out(x: torch.Tensor, row_slot: torch.Tensor, slot_row: tor
     cols = _check_rows("expert_gather_fp8", "x", x, tokens, 16)
     dev = _check_device("expert_gather_fp8", x, row_slot, slot_row)
     x2 = _rows(x, cols)
-    codes, scales = _fp8_block_outputs("expert_gather_fp8", out, tokens * k, cols, x.device)
+    codes, scales = _fp8_block_outputs("expert_gather_fp8", out, tokens * k, cols, x.device, x, row_slot, slot_row)
     rc = _loader.load_library().magi_swiglu_expert_gather_fp8_block(
         x2.data_ptr(), row_slot.data_ptr(), slot_row.data_ptr(), codes.data_ptr(), scales.data_ptr(), tokens, k, cols,
         _ld(x2), dev, _raw_stream(dev))

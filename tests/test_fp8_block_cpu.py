@@ -116,3 +116,10 @@ def test_c_entry_points_reject_on_the_host():
     base = dict(a=p, asc=p, b=p, bsc=p, off=None, e=1, c=p, s=p, M=4, N=16, K=32, lda=32, lds=1, zt=1, dev=0, st=None)
     fused = lambda **o: lib.magi_swiglu_gemm_swiglu_fp8_block(*{**base, **o}.values())  # noqa: E731
     assert fused(N=8) == -2 and fused(s=None) == -1 and fused(c=p + 4) == -3 and fused(M=0) == 0
+
+
+@pytest.mark.parametrize("shape", [(32,), (), (1, 2, 32, 32)])
+def test_weights_of_other_ranks_are_refused(shape):
+    for quantiser in (mb.quantize_fp8_weight, mb.quantize_fp8_gate_up):
+        with pytest.raises(ValueError, match="a weight is"):
+            quantiser(torch.zeros(shape))

@@ -364,6 +364,35 @@ def test_out_arguments():
         mb.expert_gather_out(x, out[0].cpu(), out[1])
 
 
+def test_results_that_overlap_operands_are_refused():
+    """With one choice a token the shapes agree, so an in-place permutation looks possible: the kernels read after they write."""
+    T, k, H, E = 12, 1, 128, 4
+    ids = routing(T, k, E).int()
+    row_slot, slot_row, offsets = mb.expert_sort(ids, E)
+    x = rows_of(T, H, 1)
+    new = lambda *shape: torch.empty(*shape, dtype=torch.int32, device="cuda")
+    codes, scales = mb.quantize_fp8_block(x)
+    w, ws = mb.quantize_fp8_weight(rows_of(H, H, 2))
+    w13, w13s = mb.quantize_fp8_gate_up(rows_of(2 * H, H, 3))
+    raw = codes.view(torch.uint8)
+    shared = torch.empty(T * H * 2, dtype=torch.uint8, device="cuda")
+    for call in (lambda: mb.expert_sort_out(ids, E, out=(row_slot, ids, offsets)),
+                 lambda: mb.expert_sort_out(ids, T - 1, out=(row_slot, new(T, k), row_slot)),
+                 lambda: mb.expert_gather_out(x, row_slot, slot_row, out=x),
+                 lambda: mb.expert_combine_out(x, None, row_slot, slot_row, out=x),
+                 lambda: mb.expert_gather_fp8_out(x, row_slot, slot_row, out=(x.view(torch.float8_e4m3fn).view(-1)[T * H:].view(T, H), scales)),
+                 lambda: mb.quantize_fp8_block_out(x, out=(codes, raw.view(-1)[:4 * T].view(torch.float32).view(T, 1))),
+                 lambda: mb.gemm_fp8_block_out(shared[:T * H].view(torch.float8_e4m3fn).view(T, H), scales, w, ws,
+                                               out=shared.view(BF).view(T, H)),
+                 lambda: mb.gemm_swiglu_fp8_block_out(codes, scales, w13, w13s, out=(codes, new(T, 1).float())),
+                 lambda: mb.gemm_swiglu_fp8_block_out(codes, scales, w13, w13s, out=(torch.empty_like(codes), scales))):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    both = torch.empty(2 * T, H, dtype=BF, device="cuda")  # neighbours in one buffer are apart
+    both[:T] = x
+    assert torch.equal(mb.expert_gather_out(both[:T], row_slot, slot_row, out=both[T:]), mb.expert_gather(x, row_slot, slot_row))
+
+
 def test_offsets_past_32_bits():
     """More than 2^31 elements on the experts' side: the last rows are right in every direction."""
     T, k, H, E = 66000, 4, 8192, 16
