@@ -212,7 +212,12 @@ class _Gather(torch.autograd.Function):
         ctx.save_for_backward(row_slot, slot_row)
         return expert_gather_out(x, row_slot, slot_row)
 
-    backward = staticmethod(_gather_backward)
+    @staticmethod
+    def backward(ctx, grad):
+        if torch.is_grad_enabled() or not _plain(grad):
+            return _gather_backward(ctx, grad)
+        # the forward has checked the maps and autograd the gradient: not again (5 us on the thread of the backward pass)
+        return _combine_rows(grad, None, ctx.saved_tensors[1], grad.shape[1], grad.get_device()), None, None
 
 
 def expert_gather(x: torch.Tensor, row_slot: torch.Tensor, slot_row: torch.Tensor) -> torch.Tensor:
@@ -242,14 +247,24 @@ def expert_combine_out(y: torch.Tensor, weights: torch.Tensor | None, row_slot: 
         weights = weights.contiguous()
     else:
         dev = _check_device("expert_combine", y, row_slot, slot_row)
+    if out is not None:
+        _result("expert_combine", out, (tokens, h), torch.bfloat16, y.device, y, weights, slot_row)
+    return _combine_rows(y, weights, slot_row, h, dev, out)
+
+
+def _combine_rows(y: torch.Tensor, weights: torch.Tensor | None, slot_row: torch.Tensor, h: int, dev: int,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The launch of ``expert_combine`` on operands that have been checked."""
+    tokens, k = slot_row.shape
     y2 = _rows(y, h)
-    res = _result("expert_combine", out, (tokens, h), torch.bfloat16, y.device, y, weights, slot_row)
+    if out is None:
+        out = torch.empty(tokens, h, dtype=torch.bfloat16, device=y.device)
     rc = _loader.load_library().magi_swiglu_expert_combine_bf16(
-        y2.data_ptr(), weights.data_ptr() if weights is not None else None, slot_row.data_ptr(), res.data_ptr(), tokens, k,
+        y2.data_ptr(), weights.data_ptr() if weights is not None else None, slot_row.data_ptr(), out.data_ptr(), tokens, k,
         h, _ld(y2), dev, _raw_stream(dev))
     if rc != 0:
         _raise("expert_combine", rc)
-    return res
+    return out
 
 
 def _combine_backward_meta(dout, y, weights, row_slot, slot_row, need_dy, need_dw):
@@ -266,14 +281,22 @@ def _combine_backward_body(dout: torch.Tensor, y: torch.Tensor, weights: torch.T
         raise ValueError(f"{name}: y {tuple(y.shape)} and dout {tuple(dout.shape)} differ in row length")
     _check_weights(name, weights, tokens, k)
     dev = _check_device(name, dout, y, weights, row_slot, slot_row)
+    return _combine_backward_rows(dout, y, weights, row_slot, slot_row, need_dy, need_dw, h, dev)
+
+
+def _combine_backward_rows(dout: torch.Tensor, y: torch.Tensor, weights: torch.Tensor, row_slot: torch.Tensor,
+                           slot_row: torch.Tensor, need_dy: bool, need_dw: bool, h: int, dev: int
+                           ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The launch of ``expert_combine_backward`` on operands that have been checked."""
+    tokens, k = slot_row.shape
     d2, y2, w = _rows(dout, h), _rows(y, h), weights.contiguous()
-    dy = torch.empty((tokens * k, h) if need_dy else (0,), dtype=torch.bfloat16, device=y.device)
-    dw = torch.empty((tokens, k) if need_dw else (0,), dtype=torch.float32, device=y.device)
+    dy = torch.empty(*((tokens * k, h) if need_dy else (0,)), dtype=torch.bfloat16, device=y.device)
+    dw = torch.empty(*((tokens, k) if need_dw else (0,)), dtype=torch.float32, device=y.device)
     rc = _loader.load_library().magi_swiglu_expert_combine_backward_bf16(
         d2.data_ptr(), y2.data_ptr(), w.data_ptr(), row_slot.data_ptr(), slot_row.data_ptr(),
         dy.data_ptr() if need_dy else None, dw.data_ptr() if need_dw else None, tokens, k, h, _ld(d2), _ld(y2), dev, _raw_stream(dev))
     if rc != 0:
-        _raise(name, rc)
+        _raise("expert_combine_backward", rc)
     return dy, dw
 
 
@@ -299,9 +322,10 @@ def _combine_backward(ctx, grad):
     if not ctx.weighted:
         return expert_gather(grad, *ctx.saved_tensors), None, None, None
     need_dy, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    plain = _plain(grad) and not torch.is_grad_enabled()
-    backward = _combine_backward_body if plain else torch.ops.magi_swiglu.expert_combine_backward
-    dy, dw = backward(grad, *ctx.saved_tensors, need_dy, need_dw)
+    if torch.is_grad_enabled() or not _plain(grad):
+        dy, dw = torch.ops.magi_swiglu.expert_combine_backward(grad, *ctx.saved_tensors, need_dy, need_dw)
+    else:  # checked by the forward and by autograd
+        dy, dw = _combine_backward_rows(grad, *ctx.saved_tensors, need_dy, need_dw, grad.shape[1], grad.get_device())
     return dy if need_dy else None, dw if need_dw else None, None, None
 
 
