@@ -438,28 +438,35 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
 // It is launched without programmatic overlap (the extra wait changes the loop's instruction schedule for the worse).
 // Persistent: tiles go round-robin to the pairs in bands of row groups, column tile by column tile, so that the
 // pairs that run together share A rows and W rows in L2.
+// kCtas 1: the same loop for one CTA with 128 rows of A and all 256 of W, 48 KB a K block; less padding for small experts
+// (SwiGLU, 64 experts, 6000 rows, N 1408, K 2048: 91 us against 128 with pairs), more L2 traffic (8192 dense rows, N 14336,
+// K 4096: 1052 against 1002).  Additions come in the same order: the results are the same bits.
 // Few tiles: `splits` (2 or 4) pairs form a cluster and share a tile's K blocks.  At the end each pair keeps the rows of
 // 4 / splits lane quarters, sends the sums of the others to the pairs that keep those (distributed shared memory, into the
 // stages, which are free by then) and adds what it receives in the order of the splits.  One tile a cluster.
 constexpr int kTileThreads = 384;  // warps 0 TMA, 1 and 3 MMA, 2 tensor-memory allocator and scales; 4-11 epilogue
 constexpr int kTileRegs = 168;     // a thread's registers at launch: 384 * 168 = 64512 = 128 * 56 + 256 * 224
-constexpr int kTileRows = 256;     // rows of a pair
-constexpr int kTileStage = 2 * kWTile;
-constexpr int kTileStages = 6;
-constexpr int kTileSmem = kTileStages * kTileStage + 1024;
+template <int kCtas>
+struct Tile {
+  static constexpr int kRows = 128 * kCtas;
+  static constexpr int kStage = kCtas == 2 ? 2 * kWTile : 3 * kWTile;
+  static constexpr int kStages = kCtas == 2 ? 6 : 4;
+  static constexpr int kSmem = kStages * kStage + 1024;
+};
 constexpr int kMapExperts = 1024;
 constexpr int kScaleSlots = 4;     // ring of scale products, four K blocks a slot
 
 struct TileAt {
-  int e, row0, end, n0;  // rows [row0, min(row0 + 256, end)), first output column
+  int e, row0, end, n0;  // rows [row0, min(row0 + kRows, end)), first output column
 };
 constexpr int kTileInfos = 2 * kScaleSlots;  // the scale warp is at most kScaleSlots tiles ahead
 
-template <int kHalves>
+template <int kHalves, int kCtas>
 __global__ void __launch_bounds__(kTileThreads, 1)
 fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const Args a,
                       const int wide_store) {
   constexpr int kOutCols = 256 / kHalves;
+  constexpr int kTileRows = Tile<kCtas>::kRows, kTileStage = Tile<kCtas>::kStage, kTileStages = Tile<kCtas>::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int row_start[kMapExperts + 1], unit_first[kMapExperts + 1];
   __shared__ unsigned top_half[2][128];
@@ -471,10 +478,10 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cluster_rank = (int)cluster_ctarank();
-  const int rank = cluster_rank & 1, split = cluster_rank >> 1;  // rank 0 issues the pair's MMAs
-  const uint32_t leader = cluster_rank & ~1;
+  const int rank = kCtas == 2 ? cluster_rank & 1 : 0, split = kCtas == 2 ? cluster_rank >> 1 : 0;  // rank 0 issues the pair's MMAs
+  const uint32_t leader = kCtas == 2 ? cluster_rank & ~1 : 0;
   const uint16_t both = (uint16_t)(3u << leader);
-  const int pair = blockIdx.x / (2 * a.splits), pairs = gridDim.x / (2 * a.splits);  // pairs, or clusters of them
+  const int pair = blockIdx.x / (kCtas * a.splits), pairs = gridDim.x / (kCtas * a.splits);  // pairs, or clusters of them
   const int kb0 = (int)((long long)a.kb * split / a.splits), kb1 = (int)((long long)a.kb * (split + 1) / a.splits);
   const uint32_t tiles = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bar0 = smem_u32(bars);
@@ -493,7 +500,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), 16);  // the epilogue warps of both CTAs
+      mbar_init(acc_empty(b), 8 * kCtas);  // the epilogue warps of both CTAs
     }
     for (int s = 0; s < kScaleSlots; ++s) {
       mbar_init(scale_full(s), 1);
@@ -504,8 +511,8 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     prefetch_tensormap(&tm_a);
   }
   if (warp == 2) {
-    tmem_alloc<2>(smem_u32(&tmem_slot), 512);
-    tmem_relinquish<2>();
+    tmem_alloc<kCtas>(smem_u32(&tmem_slot), 512);
+    tmem_relinquish<kCtas>();
   }
   if (warp == 3) {  // where each expert's rows and row groups begin; clamped, see find_unit
     int seen = 0;
@@ -572,10 +579,18 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
         const int wrow = kHalves == 1 ? at.n0 + 128 * rank : at.n0, whalf = kHalves == 1 ? at.e : at.e * 2 + rank;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = wait_bounded(empty_bar(stage), phase ^ 1u, &abort_flag, 1u, stage))) break;
-          if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kTileStage - (peer_empty ? kWTile : 0));
           const uint32_t dst = tiles + stage * kTileStage;
-          if (!empty) tma_load_2d_pair_hint(dst, &tm_a, full0 + 8u * stage, kb * kBlk, row, keep);
-          tma_load_3d_pair_hint(dst + kWTile, &tm_w, full0 + 8u * stage, kb * kBlk, wrow, whalf, normal);
+          if constexpr (kCtas == 2) {
+            if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kTileStage - (peer_empty ? kWTile : 0));
+            if (!empty) tma_load_2d_pair_hint(dst, &tm_a, full0 + 8u * stage, kb * kBlk, row, keep);
+            tma_load_3d_pair_hint(dst + kWTile, &tm_w, full0 + 8u * stage, kb * kBlk, wrow, whalf, normal);
+          } else {
+            mbar_arrive_expect_tx(full_bar(stage), kTileStage);
+            tma_load_2d_hint(dst, &tm_a, full_bar(stage), kb * kBlk, row, keep);
+            tma_load_3d_hint(dst + kWTile, &tm_w, full_bar(stage), kb * kBlk, wrow, whalf, normal);
+            tma_load_3d_hint(dst + 2 * kWTile, &tm_w, full_bar(stage), kb * kBlk, kHalves == 1 ? wrow + 128 : wrow,
+                             kHalves == 1 ? whalf : whalf + 1, normal);
+          }
           if (++stage == kTileStages) stage = 0, phase ^= 1u;
         }
       }
@@ -583,7 +598,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       // ---------------------------------------------------------- MMA issuers: warp 1 the even K blocks, warp 3 the odd
       // ones, each with a buffer of its own.  Issuing four MMAs holds a thread until the tensor pipe has taken them, so two
       // issuers do their waits in each other's shadow; lane 0 waits for the operands while the others wait for the buffer.
-      const uint32_t idesc = umma_idesc_e4m3(256, 256);
+      const uint32_t idesc = umma_idesc_e4m3(128 * kCtas, 256);
       const int buf = warp >> 1;
       int it = 0, stage = 0;
       uint32_t phase = 0;
@@ -599,9 +614,9 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
               const uint64_t da = umma_desc_k_sw128(tiles + stage * kTileStage);
               const uint64_t dw = umma_desc_k_sw128(tiles + stage * kTileStage + kWTile);
 #pragma unroll
-              for (int i = 0; i < kBlk / 32; ++i) umma_fp8<2>(tmem + buf * 256, da + 2 * i, dw + 2 * i, idesc, i > 0);
-              umma_commit<2>(acc_full(buf), both);
-              umma_commit<2>(empty_bar(stage), both);
+              for (int i = 0; i < kBlk / 32; ++i) umma_fp8<kCtas>(tmem + buf * 256, da + 2 * i, dw + 2 * i, idesc, i > 0);
+              umma_commit<kCtas>(acc_full(buf), both);
+              umma_commit<kCtas>(empty_bar(stage), both);
             }
             __syncwarp();
           }
@@ -833,7 +848,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   cluster_sync_all();  // the pair leaves together: MMAs read both CTAs' shared memory, both share barriers
   if (warp == 2) {
     tc_fence_after_sync();
-    tmem_dealloc<2>(tmem, 512);
+    tmem_dealloc<kCtas>(tmem, 512);
   }
 }
 

@@ -87,20 +87,29 @@ static int launch_stream(const Problem& p, int device, int splits, cudaStream_t 
 // Clusters of 1, 2 and 4 CTA pairs that the GPU holds at once, per device and form (first entry 0: not queried yet).
 static int g_tile_clusters[kMaxDevices][2][3];
 
+template <int kHalves, int kCtas>
+static int tile_ready() {
+  cudaError_t e = cudaFuncSetAttribute(fp8_block_tile_kernel<kHalves, kCtas>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Tile<kCtas>::kSmem);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+  cudaFuncAttributes fa;
+  e = cudaFuncGetAttributes(&fa, fp8_block_tile_kernel<kHalves, kCtas>);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncGetAttributes");
+  // the warpgroups' register shares add up to the launch's total: fewer at launch and the larger share would wait for good
+  if (fa.numRegs != kTileRegs)
+    return fail(MAGI_SWIGLU_ERR_DEVICE, "fp8_block_tile_kernel was built with %d registers a thread, not %d", fa.numRegs, kTileRegs);
+  return 0;
+}
+
 template <int kHalves>
 static int tile_clusters(int device, int sm_count, int (&clusters)[3]) {
-  auto kernel = fp8_block_tile_kernel<kHalves>;
+  auto kernel = fp8_block_tile_kernel<kHalves, 2>;
   std::lock_guard<std::mutex> lock(g_dev_mutex);
   int(&known)[3] = g_tile_clusters[device][kHalves - 1];
   if (known[0] == 0) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem);
-    if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
-    cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, kernel);
-    if (e != cudaSuccess) return fail_cuda(e, "cudaFuncGetAttributes");
-    // the warpgroups' register shares add up to the launch's total: fewer at launch and the larger share would wait for good
-    if (fa.numRegs != kTileRegs)
-      return fail(MAGI_SWIGLU_ERR_DEVICE, "fp8_block_tile_kernel was built with %d registers a thread, not %d", fa.numRegs, kTileRegs);
+    if (int rc = tile_ready<kHalves, 1>()) return rc;
+    if (int rc = tile_ready<kHalves, 2>()) return rc;
+    cudaError_t e;
     int found[3] = {0, 0, 0};
     for (int i = 0; i < 3; ++i) {
       cudaLaunchConfig_t cfg = {};
@@ -111,7 +120,7 @@ static int tile_clusters(int device, int sm_count, int (&clusters)[3]) {
       attr[0].val.clusterDim.z = 1;
       cfg.gridDim = dim3((unsigned)(sm_count / (2 << i) * (2 << i)));
       cfg.blockDim = dim3(kTileThreads);
-      cfg.dynamicSmemBytes = kTileSmem;
+      cfg.dynamicSmemBytes = Tile<2>::kSmem;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       e = cudaOccupancyMaxActiveClusters(&found[i], kernel, &cfg);
@@ -131,8 +140,9 @@ static int tile_log_splits(int64_t most, int kb, const int (&clusters)[3]) {
   return s;
 }
 
-template <int kHalves>
-static int launch_tiles(const Problem& p, const int (&clusters)[3], cudaStream_t stream) {
+template <int kHalves, int kCtas>
+static int launch_tiles(const Problem& p, int log_splits, int most_workers, cudaStream_t stream) {
+  constexpr int kTileRows = Tile<kCtas>::kRows;
   const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.args.E * kHalves};
   const cuuint64_t wst[2] = {(cuuint64_t)p.K, (cuuint64_t)p.N * (cuuint64_t)p.K};
   const cuuint64_t ad[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M};
@@ -145,17 +155,16 @@ static int launch_tiles(const Problem& p, const int (&clusters)[3], cudaStream_t
   const int64_t units = most_groups(p, kTileRows);
   if (units * n_tiles > 0x7fffffffLL / 2) return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld x N=%lld is too large for one launch", (long long)p.M, (long long)p.N);
   const int64_t most = units * n_tiles;
-  const int log_splits = tile_log_splits(most, p.args.kb, clusters);
   Args args = p.args;
   args.splits = 1 << log_splits;
   // A raster band of about 32 MB of A: it is read once per column tile and should stay in L2 beside the W rows that pass
   // (8192 rows: K = 4096, N = 2 x 14336: bands of 8 / 16 / 32 groups 980 / 948 / 942 us; K = 14336: 447 / 451 / 468 us).
   const int64_t band = (32LL << 20) / (kTileRows * p.K);
   args.band = (int)(band < 4 ? 4 : (band > 64 ? 64 : band));
-  const int64_t workers = most < clusters[log_splits] ? most : clusters[log_splits];
+  const int64_t workers = most < most_workers ? most : most_workers;
   const int wide = ((uintptr_t)p.args.c & 31u) == 0 && p.N % 16 == 0;
-  const cudaError_t e = launch(fp8_block_tile_kernel<kHalves>, dim3((unsigned)(workers * (2 << log_splits))),
-                               dim3(kTileThreads), kTileSmem, stream, 2u << log_splits, false, tm_w, tm_a, args, wide);
+  const cudaError_t e = launch(fp8_block_tile_kernel<kHalves, kCtas>, dim3((unsigned)(workers * (kCtas << log_splits))),
+                               dim3(kTileThreads), Tile<kCtas>::kSmem, stream, (unsigned)kCtas << log_splits, false, tm_w, tm_a, args, wide);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_tile_kernel");
 }
 
@@ -183,11 +192,20 @@ static int run(const Problem& p, int device, void* cuda_stream) {
   const double bytes_us = used * p.halves * p.N * p.K / 6.2e6 + 3.0;
   double best = 0;
   int tok = 0, splits = 1;
+  const int64_t n_tiles = (p.N * p.halves + 255) / 256;
+  const int log_splits = tile_log_splits(most_groups(p, Tile<2>::kRows) * n_tiles, p.args.kb, clusters);
+  // CTA pairs (256 rows) or single CTAs (128): half as much of a small expert's last group is padding, but a CTA fetches
+  // 48 KB a K block and not 32, more yet when rows of K bytes start inside a 32-byte sector.  Pairs / singles: SwiGLU, 64
+  // experts, 15200 rows, N = 1408: K = 2048 156 / 139 us, 2064 170 / 188, 2112 178 / 155; 6000 rows, K = 2048 128 / 91; 128
+  // experts, 32768 rows, plain, N = 2048, K = 768 125 / 105; dense SwiGLU, N = 14336, K = 4096: 384 rows 79 / 64, 8192 rows
+  // 1002 / 1052.  Both add in the same order.
+  bool single = false;
   {
-    const int64_t n_tiles = (p.N * p.halves + 255) / 256;
-    const int log_splits = tile_log_splits(most_groups(p, kTileRows) * n_tiles, p.args.kb, clusters);
-    const double rounds = ceil(expected_groups(p, kTileRows) * n_tiles / clusters[log_splits]);
+    const double rounds = ceil(expected_groups(p, Tile<2>::kRows) * n_tiles / clusters[log_splits]);
     best = 5.0 + rounds * (p.args.kb * 0.42 / (1 << log_splits) + 2.5) + (log_splits ? 3.0 : 0.0);
+    const double rounds1 = ceil(expected_groups(p, Tile<1>::kRows) * n_tiles / di->sm_count);
+    const double cost1 = 5.0 + rounds1 * (p.args.kb * 0.42 + 2.5) * (p.K % 32 ? 1.5 : 1.12);
+    if (cost1 < best) best = cost1, single = true;
     if (best < bytes_us) best = bytes_us;
   }
   const int forms = p.halves == 1 ? 3 : 2;
@@ -206,11 +224,11 @@ static int run(const Problem& p, int device, void* cuda_stream) {
     if (tok == 16) return launch_stream<1, 16>(p, device, splits, stream);
     if (tok == 32) return launch_stream<1, 32>(p, device, splits, stream);
     if (tok == 64) return launch_stream<1, 64>(p, device, splits, stream);
-    return launch_tiles<1>(p, clusters, stream);
+    return single ? launch_tiles<1, 1>(p, 0, di->sm_count, stream) : launch_tiles<1, 2>(p, log_splits, clusters[log_splits], stream);
   }
   if (tok == 16) return launch_stream<2, 16>(p, device, splits, stream);
   if (tok == 32) return launch_stream<2, 32>(p, device, splits, stream);
-  return launch_tiles<2>(p, clusters, stream);
+  return single ? launch_tiles<2, 1>(p, 0, di->sm_count, stream) : launch_tiles<2, 2>(p, log_splits, clusters[log_splits], stream);
 }
 
 static int check(const void* a, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,

@@ -140,6 +140,35 @@ def test_experts_swiglu(E, counts, tail, N, K):
     assert (codes[sum(counts):].float() == 0).all() and (scales[sum(counts):] == 2.0 ** -126).all()
 
 
+@pytest.mark.parametrize("halves,N,K", [(1, 2056, 128), (1, 2048, 400), (1, 2040, 256), (1, 4088, 1056), (2, 1040, 128),
+                                        (2, 1024, 272), (2, 1008, 272), (2, 4080, 1056)])
+def test_uneven_experts_with_half_empty_groups(halves, N, K):
+    """Sizes at which tiles of 128 rows are expected to beat those of 256: an empty expert, one row over a group, a tail; the
+    result does not depend on what the neighbouring experts' rows hold, guard rows stay."""
+    counts, tail = [1003, 0, 129, 855], 13
+    n = sum(counts)
+    t = case(n + tail, N, K, E=4, counts=counts, halves=halves, seed=N)
+    args = (t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    if halves == 1:
+        got = mb.gemm_fp8_block(*args)
+        check_plain(t, got)
+        assert (got[n:] == 0).all()
+        out = torch.full((n + tail + 2, N), 7.0, dtype=BF, device="cuda")
+        mb.gemm_fp8_block_out(*args, out=out[1:-1])
+        assert torch.equal(out[1:1 + n], got[:n]) and (out[0] == 7).all() and (out[1 + n:] == 7).all()
+    else:
+        codes, scales = mb.gemm_swiglu_fp8_block(*args)
+        check_fused(t, codes, scales)
+        assert (codes[n:].float() == 0).all() and (scales[n:] == 2.0 ** -126).all()
+        got = codes
+    t["a"].view(torch.uint8)[1003:1003 + 129] = 127  # NaN in e4m3: all of the third expert
+    again = (mb.gemm_fp8_block if halves == 1 else lambda *x: mb.gemm_swiglu_fp8_block(*x)[0])(*args)
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[1003:1003 + 129] = False
+    assert torch.equal(again[:n][keep].view(torch.uint8), got[:n][keep].view(torch.uint8))
+    assert again[:n][~keep].float().isnan().all()
+
+
 @pytest.mark.parametrize("N,K", [(272, 2064), (144, 4112)])
 def test_few_tiles_with_many_k_blocks(N, K):
     """Experts whose tiles share their K blocks among several CTA pairs, one of them empty, one with a partial group."""
@@ -207,6 +236,17 @@ def test_nan_and_infinite_rows_stay_by_themselves(M):
     codes, scales = mb.gemm_swiglu_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
     assert scales[2].isnan().all() and codes[2].float().isnan().all()
     assert scales[keep].isfinite().all() and not codes[keep].float().isnan().any()
+
+
+@pytest.mark.parametrize("bad", [[-9, 900, 2 ** 31 - 1], [0, 10 ** 6, 1000], [1000, 1000, 1000], [600, 200, 100]])
+def test_bad_offsets_with_tiles_of_128_rows(bad):
+    t = case(1000, 2048, 256, E=2, counts=[900, 100], halves=2)
+    codes = torch.full((1002, 2048), 5.0, device="cuda").to(torch.float8_e4m3fn)
+    scales = torch.full((1002, 16), 5.0, device="cuda")
+    off = torch.tensor(bad, dtype=torch.int32, device="cuda")
+    mb.gemm_swiglu_fp8_block_out(t["a"], t["a_scale"], t["b"], t["b_scale"], off, out=(codes[1:-1], scales[1:-1]))
+    for guarded in (codes.float(), scales):
+        assert (guarded[0] == 5).all() and (guarded[-1] == 5).all()
 
 
 @pytest.mark.parametrize("M,counts", [(12, [5, 7]), (600, [280, 320])])
