@@ -345,6 +345,36 @@ def test_on_a_side_stream():
         assert torch.equal(got, want)
 
 
+def test_a_captured_step_with_its_gradients():
+    """Forward and backward in one graph, replayed with new routing, rows and weights; leaves are made inside the capture."""
+    T, k, H, E = 40, 3, 256, 6
+    static = dict(ids=routing(T, k, E), x=rows_of(T, H, 1), w=torch.rand(T, k, device="cuda"), dout=rows_of(T, H, 2))
+
+    def step(ids, x, w, dout):
+        x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+        row_slot, slot_row, _ = mb.expert_sort_out(ids, E)
+        out = mb.expert_combine(mb.expert_gather(x, row_slot, slot_row), w, row_slot, slot_row)
+        return (out.detach(), *torch.autograd.grad(out, (x, w), dout))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(**static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(**static)
+    for seed in (5, 6):
+        new = dict(ids=routing(T, k, E, seed=seed, drop=0.2), x=rows_of(T, H, seed), w=torch.rand(T, k, device="cuda"),
+                   dout=rows_of(T, H, seed + 10))
+        want = step(**new)
+        for name, t in new.items():
+            static[name].copy_(t)
+        graph.replay()
+        for g, r in zip(got, want):
+            assert torch.equal(g, r)
+
+
 def test_out_arguments():
     T, k, H, E = 12, 2, 64, 4
     ids = routing(T, k, E)
