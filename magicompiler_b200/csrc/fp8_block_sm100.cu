@@ -45,11 +45,16 @@ struct Problem {
 static int64_t most_groups(const Problem& p, int rows) {
   return p.args.offsets ? p.M / rows + (p.M < p.args.E + 1 ? p.M : p.args.E + 1) : (p.M + rows - 1) / rows;
 }
-// What to expect of them: experts' shares are uneven, so half a group more than the average share needs.
+// What to expect of them: experts' shares are uneven, and an exponentially distributed share of mean s needs 1 / (1 -
+// exp(-rows / s)) groups on average (one for a small share, s / rows + 1/2 for a large one).
 static double expected_groups(const Problem& p, int rows) {
   if (!p.args.offsets) return (double)((p.M + rows - 1) / rows);
-  const double used = (double)(p.M < p.args.E ? p.M : p.args.E), each = p.M / used / rows + 0.5;
-  return used * (each < 1.0 ? 1.0 : each);
+  const double used = (double)(p.M < p.args.E ? p.M : p.args.E);
+  return used / (1.0 - exp(-rows * used / (double)p.M));
+}
+// Rounds of `workers` at a time; an expected count may miss by a few per cent, which must not make a round.
+static double rounds_of(const Problem& p, double tiles, double workers) {
+  return p.args.offsets ? fmax(1.0, ceil(0.97 * tiles / workers)) : ceil(tiles / workers);
 }
 
 template <int kHalves, int kTok>
@@ -178,7 +183,7 @@ static int run(const Problem& p, int device, void* cuda_stream) {
   // The kernel and its tokens per tile by what the forms are expected to take: rounds of the GPU's CTAs (pairs), each a
   // fixed part and a part per K block.  The constants are microseconds measured with everything in flight (148 SMs):
   // stream kernel, two CTAs an SM, 0.36 / 0.43 / 0.50 a K block for 16 / 32 / 64 tokens, 0.75 / 0.90 for 16 / 32 in the
-  // SwiGLU form, about 0.6 of that with one CTA an SM; tile kernel 0.42 a K block and 2.5 a tile.  Both sides at N = 4096,
+  // SwiGLU form, about 0.6 of that with one CTA an SM, and 3.0; tile kernel 0.42 a K block and 2.5 a tile.  Both sides at N = 4096,
   // K = 14336 (stream 16 / 32 / 64 tokens, tiles): M = 64 26 / 18 / 16 / 35 us, 256 - / 47 / 35 / 35 us, 512 - / - / 58 /
   // 37 us; SwiGLU, N = 1408, K = 2048, 64 experts (16 / 32 tokens, tiles): 512 rows 52 / 48 / 78 us, 2048 rows 85 / 75 / 96
   // us, 8192 rows 295 / 199 / 138 us.  None is faster than W's bytes (6.2 TB/s).  Forms that are bound by them alike differ
@@ -198,13 +203,17 @@ static int run(const Problem& p, int device, void* cuda_stream) {
   // 48 KB a K block and not 32, more yet when rows of K bytes start inside a 32-byte sector.  Pairs / singles: SwiGLU, 64
   // experts, 15200 rows, N = 1408: K = 2048 156 / 139 us, 2064 170 / 188, 2112 178 / 155; 6000 rows, K = 2048 128 / 91; 128
   // experts, 32768 rows, plain, N = 2048, K = 768 125 / 105; dense SwiGLU, N = 14336, K = 4096: 384 rows 79 / 64, 8192 rows
-  // 1002 / 1052.  Both add in the same order.
+  // 1002 / 1052.  Both add in the same order.  Short K and few rows of many experts suit single CTAs better than the stream
+  // kernel, whose CTAs are set up anew for every tile: plain, 128 experts, N = 2048, K = 768, singles / 32 tokens: 1024 rows
+  // 35 / 48 us, 4096 rows 45 / 81.
   bool single = false;
   {
-    const double rounds = ceil(expected_groups(p, Tile<2>::kRows) * n_tiles / clusters[log_splits]);
+    const double rounds = rounds_of(p, expected_groups(p, Tile<2>::kRows) * n_tiles, clusters[log_splits]);
     best = 5.0 + rounds * (p.args.kb * 0.42 / (1 << log_splits) + 2.5) + (log_splits ? 3.0 : 0.0);
-    const double rounds1 = ceil(expected_groups(p, Tile<1>::kRows) * n_tiles / di->sm_count);
-    const double cost1 = 5.0 + rounds1 * (p.args.kb * 0.42 + 2.5) * (p.K % 32 ? 1.5 : 1.12);
+    const double rounds1 = rounds_of(p, expected_groups(p, Tile<1>::kRows) * n_tiles, di->sm_count);
+    // warps without rows skip their work: nearly empty tiles take about 0.7 of a full one's time
+    const double fill = share < 64 ? share / 64 : 1.0;
+    const double cost1 = 3.0 + rounds1 * (p.args.kb * 0.42 + 2.5) * (p.K % 32 ? 1.5 : 1.12) * (0.7 + 0.3 * fill);
     if (cost1 < best) best = cost1, single = true;
     if (best < bytes_us) best = bytes_us;
   }
@@ -215,8 +224,8 @@ static int run(const Problem& p, int device, void* cuda_stream) {
     const double ctas = n128 * expected_groups(p, 16 << i);
     int z = 1;  // up to eight CTAs of a cluster share a tile's K blocks, at least four each, until there are about two CTAs an SM
     while (z < 8 && ctas * z * 2 <= 2 * di->sm_count && p.args.kb >= z * 8) z *= 2;
-    const double rounds = ceil(ctas * z / (2 * di->sm_count));
-    double cost = 2.5 + rounds * (p.args.kb * per_block[p.halves - 1][i] / z * (ctas * z <= di->sm_count ? 0.6 : 1.0) + 2.5);
+    const double rounds = rounds_of(p, ctas * z, 2 * di->sm_count);
+    double cost = 2.5 + rounds * (p.args.kb * per_block[p.halves - 1][i] / z * (ctas * z <= di->sm_count ? 0.6 : 1.0) + 3.0);
     if (cost < bytes_us) cost = bytes_us;
     if (cost < best || (cost == best && (tok == 0 || (p.args.offsets && tok < 2.5 * share)))) best = cost, tok = 16 << i, splits = z;
   }

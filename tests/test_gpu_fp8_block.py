@@ -140,6 +140,17 @@ def test_experts_swiglu(E, counts, tail, N, K):
     assert (codes[sum(counts):].float() == 0).all() and (scales[sum(counts):] == 2.0 ** -126).all()
 
 
+@pytest.mark.parametrize("halves,N,K", [(1, 2048, 256), (1, 1992, 640), (2, 1040, 256)])
+def test_many_experts_with_a_few_rows_each(halves, N, K):
+    counts, tail = [(0, 1, 2, 17, 0)[i % 5] for i in range(60)], 3
+    t = case(sum(counts) + tail, N, K, E=60, counts=counts, halves=halves, seed=K)
+    args = (t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"])
+    if halves == 1:
+        check_plain(t, mb.gemm_fp8_block(*args))
+    else:
+        check_fused(t, *mb.gemm_swiglu_fp8_block(*args))
+
+
 @pytest.mark.parametrize("halves,N,K", [(1, 2056, 128), (1, 2048, 400), (1, 2040, 256), (1, 4088, 1056), (2, 1040, 128),
                                         (2, 1024, 272), (2, 1008, 272), (2, 4080, 1056)])
 def test_uneven_experts_with_half_empty_groups(halves, N, K):
