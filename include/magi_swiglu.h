@@ -314,7 +314,8 @@ int magi_swiglu_expert_gather_fp8_block(const void* x, const int32_t* row_slot, 
 
 /* ---- Block-scaled fp8 products.  Codes are e4m3 bytes; a_scale holds one fp32 scale per row of A and 128 K elements
  * ([M, ceil(K/128)], row stride ld_scale), b_scale one per 128 x 128 block of B.  With `offsets` (num_experts + 1 int32 in
- * device memory, the first one 0; the kernel clamps them to [0, M], they must not decrease) rows [offsets[e], offsets[e+1]) of A meet B[e];
+ * device memory, the first one 0, none below the one before it; the kernels clamp them to [0, M] and take one that is below
+ * an earlier one for that one, so a bad array gives wrong rows and nothing worse) rows [offsets[e], offsets[e+1]) of A meet B[e];
  * rows from offsets[num_experts] on are written as zeros when zero_tail is set and left as they are otherwise.  Without
  * offsets num_experts is 1.  Sums are fp32.  K % 16 == 0, lda % 16 == 0, 16-byte aligned a, b, c, codes; B and the outputs
  * are contiguous, the outputs overlap no input.  M == 0 is a successful no-op.  Rows of A with a NaN scale or code give NaN. */

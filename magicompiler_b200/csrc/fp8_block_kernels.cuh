@@ -101,11 +101,6 @@ struct Unit {  // rows [row0, row0 + rows) of expert e; e == E: rows behind the 
   int e, row0, rows;
 };
 
-// First row of expert e, e == E: of the rows behind the last expert's.  Clamped to [0, R], so that a bad array cannot lead
-// outside the operands; without offsets one expert has all rows.
-__device__ __forceinline__ int start_of(const Args& a, int e) {
-  return a.offsets ? min(max(a.offsets[e], 0), a.R) : (e == 0 ? 0 : a.R);
-}
 __device__ __forceinline__ int warp_scan(int n) {  // inclusive sum over the warp's lanes
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -116,24 +111,42 @@ __device__ __forceinline__ int warp_scan(int n) {  // inclusive sum over the war
   return n;
 }
 
+// Rows [first, first + rows) of expert e, this lane's (the whole warp calls this, 32 experts at a time in order; `from`
+// starts at 0); e == E: the rows behind the last expert's; beyond: none.  A bad array leads neither outside the operands nor
+// to more groups than the host has counted on: offsets are clamped to [0, R], and one below an earlier one counts as that
+// one, so that no row belongs to two experts.  Without offsets one expert has all rows.
+struct Rows {
+  int first, count;
+};
+__device__ __forceinline__ Rows rows_of(const Args& a, int e, int& from) {
+  int lo = 0, next = 0;
+  if (e <= a.E) {
+    lo = a.offsets ? min(max(a.offsets[e], 0), a.R) : (e == 0 ? 0 : a.R);
+    next = a.offsets && e < a.E ? min(max(a.offsets[e + 1], 0), a.R) : a.R;
+  }
+  if (__any_sync(0xffffffffu, e <= a.E && (lo < from || next < lo))) {  // never for offsets as they should be
+    lo = max(lo, from);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) lo = max(lo, __shfl_up_sync(0xffffffffu, lo, d));  // a lane below d gets its own
+  }
+  from = __shfl_sync(0xffffffffu, lo, 31);
+  return Rows{lo, e <= a.E ? max(next - lo, 0) : 0};
+}
+
 // The unit-th group of at most kTok rows, counting every expert's groups in order (one whole warp calls this).
 template <int kTok>
 __device__ __forceinline__ Unit find_unit(const Args& a, int unit) {
   const int lane = threadIdx.x & 31;
-  int seen = 0;
+  int seen = 0, from = 0;
   for (int b = 0; b <= a.E; b += 32) {
     const int e = b + lane;
-    int lo = 0, len = 0, n = 0;
-    if (e <= a.E) {
-      lo = start_of(a, e);
-      len = e < a.E ? max(start_of(a, e + 1) - lo, 0) : a.R - lo;
-      n = (e == a.E && !a.zero_tail) ? 0 : (len + kTok - 1) / kTok;
-    }
+    const Rows r = rows_of(a, e, from);
+    const int n = (e == a.E && !a.zero_tail) ? 0 : (r.count + kTok - 1) / kTok;
     const int scan = warp_scan(n);
     const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && unit >= seen + scan - n && unit < seen + scan);
     if (hit) {
       const int src = __ffs(hit) - 1, i = unit - seen - __shfl_sync(0xffffffffu, scan - n, src);
-      const int first = __shfl_sync(0xffffffffu, lo, src), rows = __shfl_sync(0xffffffffu, len, src);
+      const int first = __shfl_sync(0xffffffffu, r.first, src), rows = __shfl_sync(0xffffffffu, r.count, src);
       return Unit{b + src, first + i * kTok, min(kTok, rows - i * kTok)};
     }
     seen += __shfl_sync(0xffffffffu, scan, 31);
@@ -443,7 +456,8 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
 // K 4096: 1052 against 1002).  Additions come in the same order: the results are the same bits.
 // Few tiles: `splits` (2 or 4) pairs form a cluster and share a tile's K blocks.  At the end each pair keeps the rows of
 // 4 / splits lane quarters, sends the sums of the others to the pairs that keep those (distributed shared memory, into the
-// stages, which are free by then) and adds what it receives in the order of the splits.  One tile a cluster.
+// stages, which are free by then) and adds what it receives in the order of the splits.  One tile a cluster: the host splits
+// only what fits, and rows_of makes no more groups than the host counts on, whatever the offsets hold.
 constexpr int kTileThreads = 384;  // warps 0 TMA, 1 and 3 MMA, 2 tensor-memory allocator and scales; 4-11 epilogue
 constexpr int kTileRegs = 168;     // a thread's registers at launch: 384 * 168 = 64512 = 128 * 56 + 256 * 224
 template <int kCtas>
@@ -514,26 +528,16 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     tmem_alloc<kCtas>(smem_u32(&tmem_slot), 512);
     tmem_relinquish<kCtas>();
   }
-  if (warp == 3) {  // where each expert's rows and row groups begin; clamped, see find_unit
-    int seen = 0;
+  if (warp == 3) {  // where each expert's rows and row groups begin
+    int seen = 0, from = 0;
     for (int b = 0; b <= a.E; b += 32) {
       const int e = b + lane;
-      int lo = 0, n = 0;
+      const Rows r = rows_of(a, e, from);
+      const int n = e < a.E ? (r.count + kTileRows - 1) / kTileRows : 0, scan = warp_scan(n);
       if (e <= a.E) {
-        lo = a.offsets ? min(max(a.offsets[e], 0), a.R) : (e == 0 ? 0 : a.R);
-        if (e < a.E) {
-          const int hi = a.offsets ? min(max(a.offsets[e + 1], lo), a.R) : a.R;
-          n = (hi - lo + kTileRows - 1) / kTileRows;
-        }
-        row_start[e] = lo;
+        row_start[e] = r.first;
+        unit_first[e] = seen + scan - n;
       }
-      int scan = n;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, scan, d);
-        if (lane >= d) scan += up;
-      }
-      if (e <= a.E) unit_first[e] = seen + scan - n;
       seen += __shfl_sync(0xffffffffu, scan, 31);
     }
   }
@@ -558,7 +562,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     }
     at.e = lo;
     at.row0 = row_start[lo] + (unit - unit_first[lo]) * kTileRows;
-    at.end = max(row_start[lo], row_start[lo + 1]);
+    at.end = row_start[lo + 1];
     return at;
   };
 
@@ -822,7 +826,7 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     }
     // rows behind the last expert's: one contiguous piece of each output
     if (a.zero_tail && a.offsets) {
-      const long long from = max(0, min(row_start[a.E], a.R)), rows = a.R - from;
+      const long long from = row_start[a.E], rows = a.R - from;
       const long long me = (long long)blockIdx.x * 256 + threadIdx.x - 128, all = (long long)gridDim.x * 256;
       const uint4 zero = make_uint4(0, 0, 0, 0);
       if constexpr (kHalves == 1) {

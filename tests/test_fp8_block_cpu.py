@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+from hypothesis import given, settings, strategies as st
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 import magicompiler_b200 as mb
@@ -99,6 +100,30 @@ def test_gate_up_halves_are_blocked_from_their_own_first_row():
     assert torch.equal(codes.float(), torch.cat([g.float(), u.float()])) and torch.equal(scales, torch.cat([gs, us]))
     assert tuple(mb.quantize_fp8_gate_up(torch.zeros(3, 400, 136))[1].shape) == (3, 4, 2)
     assert (mb.quantize_fp8_weight(torch.zeros(8, 16))[1] == 2.0 ** -126).all()
+
+
+def row_groups(offsets, M, rows, running_maximum):
+    """The kernels' count of groups of `rows` rows: every offset clamped to [0, M] and, with `running_maximum`, one below an
+    earlier one taken for that one."""
+    starts = []
+    for o in offsets:
+        o = min(max(o, 0), M)
+        starts.append(max(o, starts[-1]) if running_maximum and starts else o)
+    return sum(-(-max(hi - lo, 0) // rows) for lo, hi in zip(starts, starts[1:]))
+
+
+@settings(max_examples=300, deadline=None)
+@given(st.integers(1, 3000), st.sampled_from([16, 32, 64, 128, 256]), st.lists(st.integers(-10, 4000), min_size=2, max_size=70))
+def test_no_offsets_make_more_row_groups_than_a_launch_has_room_for(M, rows, offsets):
+    """The host counts on at most M / rows whole groups and one partial one for each expert with rows; a cluster that shares a
+    tile's K blocks relies on it (a second tile would put its barriers out of step)."""
+    room = M // rows + min(M, len(offsets))
+    assert row_groups(offsets, M, rows, True) <= room
+
+
+def test_clamping_alone_would_let_falling_offsets_make_more_row_groups():
+    assert row_groups([0, 1100, 0, 1100], 1100, 256, False) == 10 > 1100 // 256 + 4
+    assert row_groups([0, 1100, 0, 1100], 1100, 256, True) == 5
 
 
 def test_c_entry_points_reject_on_the_host():

@@ -272,6 +272,42 @@ def test_bad_offsets_touch_nothing_outside(M, counts):
     assert mb.device_status(0)["code"] == 0
 
 
+def fallen(offsets, M):
+    """What the kernels make of an offsets array: clamped to [0, M], one below an earlier one counted as that one."""
+    out = []
+    for o in offsets:
+        out.append(max(min(max(o, 0), M), out[-1] if out else 0))
+    return out
+
+
+FALLING = [(1100, [0, 1100, 0, 1100]), (600, [0, 600, 0, 600, 0, 600, 0, 600]), (1000, [0, 2 ** 31 - 1, -5, 700, 300, 900]),
+           (40, [0] + [40, 0] * 20), (700, [0] * 20 + [650, 10] + [300] * 30 + [660, -2 ** 31]), (90, [90 - i for i in range(65)])]
+
+
+@pytest.mark.parametrize("M,offsets", FALLING)
+@pytest.mark.parametrize("halves,N,K", [(1, 272, 512), (1, 136, 8192), (2, 256, 8192), (2, 144, 272), (1, 2048, 256), (2, 1040, 272)])
+def test_falling_offsets_count_as_the_largest_before(M, offsets, halves, N, K):
+    """No row belongs to two experts, whichever kernel runs: the result is that of the array's running maximum, guard rows stay."""
+    E, hull = len(offsets) - 1, fallen(offsets, M)
+    t = case(M, N, K, E=E, counts=[0] * E, halves=halves, seed=M)
+    bad, t["offsets"] = (torch.tensor(o, dtype=torch.int32, device="cuda") for o in (offsets, hull))
+    args, lo, hi, nb = (t["a"], t["a_scale"], t["b"], t["b_scale"]), hull[0], hull[-1], -(-N // 128)
+    if halves == 1:
+        guarded = [torch.full((M + 8, N), 5.0, dtype=BF, device="cuda")]
+        mb.gemm_fp8_block_out(*args, bad, out=guarded[0][4:-4])
+        want = [mb.gemm_fp8_block(*args, t["offsets"])]
+    else:
+        guarded = [torch.full((M + 8, N), 5.0, device="cuda").to(F8), torch.full((M + 8, nb), 5.0, device="cuda")]
+        mb.gemm_swiglu_fp8_block_out(*args, bad, out=(guarded[0][4:-4], guarded[1][4:-4]))
+        want = mb.gemm_swiglu_fp8_block(*args, t["offsets"])
+    for got, ref in zip(guarded, want):
+        got, ref = got.float(), ref.float()
+        assert torch.equal(got[4 + lo:4 + hi], ref[lo:hi]) and (got[4 + hi:] == 5).all() and (got[:4 + lo] == 5).all()
+    if lo == 0:  # otherwise nothing has written the rows before the first expert's
+        check_plain(t, *want) if halves == 1 else check_fused(t, *want)
+    assert mb.device_status(0)["code"] == 0
+
+
 @pytest.mark.parametrize("M,N,K,E", [(3, 512, 2048, 0), (40, 256, 512, 8), (700, 512, 384, 0), (900, 264, 512, 3),
                                      (300, 512, 4096, 0), (300, 512, 2048, 0)])
 def test_the_same_bits_every_time(M, N, K, E):
