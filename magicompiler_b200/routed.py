@@ -159,11 +159,12 @@ def _check_weights(name: str, weights: torch.Tensor, tokens: int, k: int) -> Non
 
 
 def _plain(t: torch.Tensor) -> bool:
-    """Whether nothing but autograd looks at a call on ``t``: no compiler, tracing mode, tensor subclass or functorch
+    """Whether nothing but autograd looks at a call on ``t``: no compiler, tracer, tracing mode, tensor subclass or functorch
     transform.  Such a call may go to the op's body without the dispatcher, which with a registered autograd formula costs
     more host time than a small step's kernels run (113 us against 93 us for a gather and its gradient)."""
     return (type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and not torch.compiler.is_compiling() \
-        and torch._C._len_torch_dispatch_stack() == 0 and torch._C._functorch.peek_interpreter_stack() is None
+        and not torch._C._is_tracing() and torch._C._len_torch_dispatch_stack() == 0 \
+        and torch._C._functorch.peek_interpreter_stack() is None
 
 
 def _ld(t2: torch.Tensor) -> int:

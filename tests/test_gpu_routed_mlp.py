@@ -259,3 +259,28 @@ def test_registered_ops_keep_their_contracts():
             (ops.gemm_swiglu_fp8_block, (a, a_scale, *q13, offsets), with_fp8),
             (ops.gemm_fp8_block, (h, h_scale, *q2, offsets), with_fp8), (ops.gemm_fp8_block, (a, a_scale, q13[0][0], q13[1][0][:1]), with_fp8)):
         torch.library.opcheck(op.default, args, test_utils=tests)
+
+
+@pytest.mark.gpu
+def test_traced_calls_follow_their_inputs():
+    """torch.jit.trace records the operators: the traced functions answer other inputs, of other lengths, like eager calls."""
+    E, k, H = 6, 2, 64
+
+    def inputs(T, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        return (torch.randn(T, H, generator=g, device="cuda").to(BF), torch.randint(-1, E, (T, k), generator=g, device="cuda"),
+                torch.rand(T, k, generator=g, device="cuda"))
+
+    def there_and_back(x, ids, w):
+        row_slot, slot_row, _ = mb.expert_sort(ids, E)
+        return mb.expert_combine(mb.expert_gather(x, row_slot, slot_row), w, row_slot, slot_row)
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    mlp = mb.RoutedSwiGLUMLP((0.1 * torch.randn(E, 64, H, generator=g, device="cuda")).to(BF),
+                             (0.1 * torch.randn(E, H, 32, generator=g, device="cuda")).to(BF), precision="fp8")
+    for fn in (there_and_back, mlp):
+        with torch.no_grad():
+            traced = torch.jit.trace(fn, inputs(20, 0), check_trace=False)
+            for T, seed in ((20, 2), (7, 3), (300, 4)):
+                args = inputs(T, seed)
+                assert torch.equal(traced(*args), fn(*args))

@@ -109,6 +109,45 @@ def test_fake_implementations():
         assert tuple(dy.shape) == (15, 144) and dy.dtype == BF and tuple(dw.shape) == (0,)
 
 
+class _NoKernels:
+    """In the place of the library: every entry point succeeds and writes nothing."""
+
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+@pytest.fixture
+def without_kernels(monkeypatch):
+    """Operator bodies that run on CPU tensors up to the launch."""
+    from magicompiler_b200 import fp8_block, routed
+
+    monkeypatch.setattr(_loader, "load_library", lambda: _NoKernels())
+    for module in (routed, fp8_block):
+        monkeypatch.setattr(module, "_check_device", lambda *a: 0)
+        monkeypatch.setattr(module, "_raw_stream", lambda dev: 0)
+
+
+def recorded(fn, *args):
+    """The package's operators in the graph that ``torch.jit.trace`` makes of ``fn``."""
+    graph = torch.jit.trace(fn, args, check_trace=False).inlined_graph
+    return [n.kind() for n in graph.nodes() if n.kind().startswith("magi_swiglu::")]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_tracer_records_the_operators(without_kernels, grad):
+    rs, sr = maps()
+    x, y, w = torch.zeros(3, 16, dtype=BF, requires_grad=grad), torch.zeros(6, 16, dtype=BF, requires_grad=grad), torch.zeros(3, 2)
+    assert recorded(lambda *a: mb.expert_gather(*a), x, rs, sr) == ["magi_swiglu::expert_gather"]
+    assert recorded(lambda *a: mb.expert_combine(*a), y, w, rs, sr) == ["magi_swiglu::expert_combine"]
+
+
+def test_a_tracer_records_the_operators_of_the_routed_block(without_kernels):
+    mlp = mb.RoutedSwiGLUMLP(torch.zeros(4, 64, 16, dtype=BF), torch.zeros(4, 16, 32, dtype=BF), precision="fp8")
+    assert recorded(mlp, torch.zeros(3, 16, dtype=BF), torch.zeros(3, 2, dtype=I64), torch.zeros(3, 2)) == [
+        "magi_swiglu::expert_sort", "magi_swiglu::expert_gather_fp8", "magi_swiglu::gemm_swiglu_fp8_block",
+        "magi_swiglu::gemm_fp8_block", "magi_swiglu::expert_combine"]
+
+
 def test_the_row_movements_split_graphs():
     for op in ("expert_sort", "expert_gather", "expert_combine", "expert_gather_fp8"):
         assert f"magi_swiglu::{op}" in mb.SPLITTING_OPS
