@@ -158,13 +158,16 @@ def _check_weights(name: str, weights: torch.Tensor, tokens: int, k: int) -> Non
         raise ValueError(f"{name}: weights must be [{tokens}, {k}]; got shape {tuple(weights.shape)}")
 
 
-def _plain(t: torch.Tensor) -> bool:
-    """Whether nothing but autograd looks at a call on ``t``: no compiler, tracer, tracing mode, tensor subclass or functorch
-    transform.  Such a call may go to the op's body without the dispatcher, which with a registered autograd formula costs
-    more host time than a small step's kernels run (113 us against 93 us for a gather and its gradient)."""
-    return (type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and not torch.compiler.is_compiling() \
-        and not torch._C._is_tracing() and torch._C._len_torch_dispatch_stack() == 0 \
-        and torch._C._functorch.peek_interpreter_stack() is None
+def _plain(*operands: torch.Tensor | None) -> bool:
+    """Whether nothing but autograd looks at a call on these operands: no compiler, tracer, tracing or torch-function mode,
+    tensor subclass or functorch transform.  Such a call may go to the op's body without the dispatcher, which with a
+    registered autograd formula costs more host time than a small step's kernels run (113 us against 93 us for a gather and
+    its gradient)."""
+    for t in operands:
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter and t is not None:
+            return False
+    return not torch.compiler.is_compiling() and not torch._C._is_tracing() and torch._C._len_torch_dispatch_stack() == 0 \
+        and torch._C._len_torch_function_stack() == 0 and torch._C._functorch.peek_interpreter_stack() is None
 
 
 def _ld(t2: torch.Tensor) -> int:
@@ -225,7 +228,7 @@ def expert_gather(x: torch.Tensor, row_slot: torch.Tensor, slot_row: torch.Tenso
     """``xs[r] = x[row_slot[r] // k]`` (``[T, H]`` -> ``[T*k, H]`` bf16, H a multiple of 8), zeros where ``row_slot`` is -1
     (``magi_swiglu_expert_gather_bf16``).  Gradient: ``dx[t]`` is the fp32 sum of its rows' gradients in slot order,
     rounded once.  In compiled or traced code this is ``torch.ops.magi_swiglu.expert_gather``."""
-    if not (isinstance(x, torch.Tensor) and _plain(x)):
+    if not _plain(x, row_slot, slot_row):
         return torch.ops.magi_swiglu.expert_gather(x, row_slot, slot_row)
     if x.requires_grad and torch.is_grad_enabled():
         return _Gather.apply(x, row_slot, slot_row)
@@ -354,7 +357,7 @@ def expert_combine(y: torch.Tensor, weights: Optional[torch.Tensor], row_slot: t
     fp32 sums in slot order, one rounding; ``weights`` None: ones; ``magi_swiglu_expert_combine_bf16``).  Slots without an
     expert add nothing.  Gradients with respect to ``y`` and ``weights`` (once differentiable where weights are given).  In
     compiled or traced code this is ``torch.ops.magi_swiglu.expert_combine``."""
-    if not (isinstance(y, torch.Tensor) and _plain(y)):
+    if not _plain(y, weights, row_slot, slot_row):
         return torch.ops.magi_swiglu.expert_combine(y, weights, row_slot, slot_row)
     if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
         return _Combine.apply(y, weights, row_slot, slot_row)

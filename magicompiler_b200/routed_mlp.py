@@ -51,7 +51,7 @@ class RoutedSwiGLUMLP(torch.nn.Module):
             raise RuntimeError("precision='fp8' is for inference: it has no gradients (run it under torch.no_grad())")
         x2, k = x.reshape(-1, x.shape[-1]), expert_ids.shape[-1]
         ids, w = expert_ids.reshape(-1, k), weights.reshape(-1, k)
-        out_form = "_out" if routed._plain(x) else ""  # compiled and traced code calls the registered ops
+        out_form = "_out" if routed._plain(x, expert_ids, weights) else ""  # compiled and traced code calls the registered ops
         row_slot, slot_row, offsets = getattr(routed, "expert_sort" + out_form)(ids, self.num_experts)
         if self.precision == "fp8":
             a, a_scale = getattr(routed, "expert_gather_fp8" + out_form)(x2, row_slot, slot_row)

@@ -148,6 +148,60 @@ def test_a_tracer_records_the_operators_of_the_routed_block(without_kernels):
         "magi_swiglu::gemm_fp8_block", "magi_swiglu::expert_combine"]
 
 
+class _Wrapped(torch.Tensor):
+    """A tensor without memory of its own; operators get the tensor inside."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    seen = []
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        cls.seen.append(str(func))
+        return func(*[a.inner if isinstance(a, cls) else a for a in args], **(kwargs or {}))
+
+
+class _Watch(torch.overrides.TorchFunctionMode):
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        self.seen.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+def test_any_operand_may_be_a_subclass(without_kernels, which):
+    rs, sr = maps()
+    args = [torch.zeros(6, 16, dtype=BF), torch.zeros(3, 2), rs, sr]
+    args[which] = _Wrapped(args[which])
+    _Wrapped.seen.clear()
+    mb.expert_combine(*args)
+    assert any("expert_combine" in f for f in _Wrapped.seen)
+    if which != 1:
+        args = [torch.zeros(3, 16, dtype=BF), None, rs, sr]
+        args[which] = _Wrapped(args[which])
+        _Wrapped.seen.clear()
+        mb.expert_gather(args[0], args[2], args[3])
+        assert any("expert_gather" in f for f in _Wrapped.seen)
+
+
+def test_a_torch_function_mode_sees_the_operators(without_kernels):
+    rs, sr = maps()
+    mlp = mb.RoutedSwiGLUMLP(torch.zeros(4, 64, 16, dtype=BF), torch.zeros(4, 16, 32, dtype=BF), precision="fp8")
+    with _Watch() as watch:
+        mb.expert_gather(torch.zeros(3, 16, dtype=BF), rs, sr)
+        mlp(torch.zeros(3, 16, dtype=BF), torch.zeros(3, 2, dtype=I64), torch.zeros(3, 2))
+    for op in ("expert_sort", "expert_gather", "expert_gather_fp8", "gemm_swiglu_fp8_block", "gemm_fp8_block", "expert_combine"):
+        assert {f"magi_swiglu.{op}", f"magi_swiglu.{op}.default"} & set(watch.seen), op
+
+
 def test_the_row_movements_split_graphs():
     for op in ("expert_sort", "expert_gather", "expert_combine", "expert_gather_fp8"):
         assert f"magi_swiglu::{op}" in mb.SPLITTING_OPS
