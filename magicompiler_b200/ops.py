@@ -63,7 +63,7 @@ def _rows_view(t: torch.Tensor, cols: int) -> torch.Tensor:
     t2 = t.reshape(-1, cols)
     ok = t2.stride(1) == 1 and (t2.shape[0] <= 1 or (t2.stride(0) >= cols and t2.stride(0) % 8 == 0)) \
         and t2.data_ptr() % 16 == 0
-    return t2 if ok else t2.contiguous()
+    return t2 if ok else t2.clone(memory_format=torch.contiguous_format)  # contiguous() would keep an unaligned base
 
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:

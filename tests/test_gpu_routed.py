@@ -178,6 +178,34 @@ def test_broadcast_and_strided_operands():
                        mb.expert_combine(y.detach(), w.contiguous(), row_slot, slot_row))
 
 
+def unaligned(t):
+    """The same values, contiguous, two bytes past a 16-byte boundary."""
+    flat = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)[1:1 + t.numel()]
+    assert flat.data_ptr() % 16 == 2
+    return flat.copy_(t.reshape(-1)).view(t.shape)
+
+
+def test_contiguous_operands_and_gradients_off_a_16_byte_boundary():
+    T, k, H, E = 50, 2, 256, 4
+    row_slot, slot_row, _ = mb.expert_sort(routing(T, k, E, drop=0.1), E)
+    x, y, w, dx, dy = rows_of(T, H, 1), rows_of(T * k, H, 2), torch.rand(T, k, device="cuda"), rows_of(T * k, H, 3), rows_of(T, H, 4)
+    for form in (mb.expert_gather, mb.expert_gather_fp8, torch.ops.magi_swiglu.expert_gather):
+        got, want = form(unaligned(x), row_slot, slot_row), form(x, row_slot, slot_row)
+        for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+            assert torch.equal(a.float(), b.float())
+    for a, b in zip(mb.quantize_fp8_block(unaligned(x)), mb.quantize_fp8_block(x)):
+        assert torch.equal(a.float(), b.float())
+    assert torch.equal(mb.expert_combine(unaligned(y), w, row_slot, slot_row), mb.expert_combine(y, w, row_slot, slot_row))
+
+    def gradients(ddx, ddy):
+        lx, ly, lw = x.clone().requires_grad_(), y.clone().requires_grad_(), w.clone().requires_grad_()
+        return (*torch.autograd.grad(mb.expert_gather(lx, row_slot, slot_row), lx, ddx),
+                *torch.autograd.grad(mb.expert_combine(ly, lw, row_slot, slot_row), (ly, lw), ddy))
+
+    for a, b in zip(gradients(unaligned(dx), unaligned(dy)), gradients(dx, dy)):
+        assert torch.equal(a, b)
+
+
 def test_masked_slots_may_hold_anything():
     T, k, H, E = 20, 4, 128, 4
     ids = routing(T, k, E, drop=0.5, seed=8)

@@ -109,6 +109,20 @@ def test_fake_implementations():
         assert tuple(dy.shape) == (15, 144) and dy.dtype == BF and tuple(dw.shape) == (0,)
 
 
+@pytest.mark.parametrize("shift", [1, 4, 8])
+@pytest.mark.parametrize("rows", [1, 4])
+def test_rows_that_start_off_a_16_byte_boundary_are_copied(rows, shift):
+    from magicompiler_b200 import ops, routed
+
+    whole = torch.arange(4 * 64 + 16, dtype=torch.float32).to(BF)
+    whole = whole[(-whole.data_ptr() % 16) // 2:]
+    t = whole[shift:shift + rows * 64].view(rows, 64)
+    assert t.is_contiguous() and (t.data_ptr() % 16 == 0) == (shift == 8)
+    for view in (ops._rows_view, routed._rows):
+        got = view(t, 64)
+        assert got.data_ptr() % 16 == 0 and torch.equal(got, t) and (got.data_ptr() == t.data_ptr()) == (shift == 8)
+
+
 class _NoKernels:
     """In the place of the library: every entry point succeeds and writes nothing."""
 
