@@ -53,12 +53,15 @@ def _per_expert(w: torch.Tensor, fn) -> tuple[torch.Tensor, torch.Tensor]:
     return (torch.stack([p[0].view(torch.uint8) for p in parts]).view(torch.float8_e4m3fn), torch.stack([p[1] for p in parts]))
 
 
+@torch.no_grad()
 def quantize_fp8_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` of a weight ``[N, K]`` or ``[E, N, K]`` for ``gemm_fp8_block``: one scale ``max|w| / 448`` per
-    128 x 128 block, ``scales [.., ceil(N/128), ceil(K/128)]``.  Plain torch, once at load."""
+    128 x 128 block, ``scales [.., ceil(N/128), ceil(K/128)]``.  Plain torch, once at load; no gradients (a parameter may be
+    given as it is)."""
     return _per_expert(w, _quantize_blocks)
 
 
+@torch.no_grad()
 def quantize_fp8_gate_up(w_gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` of a packed gate/up weight ``[2N, K]`` or ``[E, 2N, K]`` (``pack_gate_up``) for
     ``gemm_swiglu_fp8_block``: each half is cut into blocks from its own first row, ``scales [.., 2 * ceil(N/128),

@@ -1,5 +1,6 @@
 """Block-scaled fp8 products without a GPU: refusals, fake implementations, the load-time weight quantisers and the host
 checks of the C entry points."""
+import copy
 import ctypes
 
 import pytest
@@ -141,6 +142,22 @@ def test_c_entry_points_reject_on_the_host():
     base = dict(a=p, asc=p, b=p, bsc=p, off=None, e=1, c=p, s=p, M=4, N=16, K=32, lda=32, lds=1, zt=1, dev=0, st=None)
     fused = lambda **o: lib.magi_swiglu_gemm_swiglu_fp8_block(*{**base, **o}.values())  # noqa: E731
     assert fused(N=8) == -2 and fused(s=None) == -1 and fused(c=p + 4) == -3 and fused(M=0) == 0
+
+
+@pytest.mark.parametrize("lead", [(), (3,)])
+def test_quantised_parameters_keep_no_graph(lead):
+    w = torch.nn.Parameter(torch.randn(*lead, 64, 48))
+    for quantiser in (mb.quantize_fp8_weight, mb.quantize_fp8_gate_up):
+        for got, want in zip(quantiser(w), quantiser(w.detach())):
+            assert not got.requires_grad and torch.equal(got.float(), want.float())
+
+
+def test_a_routed_block_made_from_parameters_can_be_copied():
+    w13, w2 = (torch.nn.Parameter(torch.randn(s).to(torch.bfloat16)) for s in ((3, 64, 48), (3, 48, 32)))
+    mlp = mb.RoutedSwiGLUMLP(w13, w2, precision="fp8")
+    assert not any(b.requires_grad for b in mlp.buffers())
+    for a, b in zip(copy.deepcopy(mlp).buffers(), mlp.buffers()):
+        assert torch.equal(a.float(), b.float())
 
 
 @pytest.mark.parametrize("shape", [(32,), (), (1, 2, 32, 32)])
