@@ -20,7 +20,8 @@ class RoutedSwiGLUMLP(torch.nn.Module):
       forward reads the E + 1 row offsets on the host (it cannot be captured in a CUDA graph).
     * ``precision="fp8"``: inference.  The weights are quantised once, here (one fp32 scale per 128 x 128 block), and all
       experts run in one launch per projection (``gemm_swiglu_fp8_block``, ``gemm_fp8_block``); nothing is read on the host,
-      a forward of fixed shape can be captured.
+      a forward of fixed shape can be captured.  Moving the module to another dtype (``.bfloat16()``, ``.to(dtype)`` of a whole
+      model) moves the codes and the fp32 scales to the device it names and leaves their types alone.
     """
 
     def __init__(self, w_gate_up: torch.Tensor, w_down: torch.Tensor, precision: str = "bf16"):
@@ -41,6 +42,16 @@ class RoutedSwiGLUMLP(torch.nn.Module):
         for name, pair in (("gate_up", quantize_fp8_gate_up(w_gate_up)), ("down", quantize_fp8_weight(w_down))):
             self.register_buffer(f"{name}_codes", pair[0])
             self.register_buffer(f"{name}_scales", pair[1])
+
+    def _apply(self, fn, recurse=True):
+        if self.precision != "fp8":
+            return super()._apply(fn, recurse)
+
+        def keep_type(t: torch.Tensor) -> torch.Tensor:
+            moved = fn(t)
+            return moved if moved.dtype is t.dtype else t.to(moved.device)
+
+        return super()._apply(keep_type, recurse)
 
     def forward(self, x: torch.Tensor, expert_ids: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
         """``x [..., K]`` bf16, ``expert_ids [..., k]`` int32 or int64, ``weights [..., k]`` fp32 -> ``[..., K_out]``."""

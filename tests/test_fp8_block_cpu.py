@@ -160,6 +160,21 @@ def test_a_routed_block_made_from_parameters_can_be_copied():
         assert torch.equal(a.float(), b.float())
 
 
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(), lambda m: m.to(torch.bfloat16),
+                                  lambda m: torch.nn.Sequential(m).to(torch.float16)[0], lambda m: m.type(torch.float64)])
+def test_a_cast_of_the_module_leaves_codes_and_scales(cast):
+    w13, w2 = torch.randn(3, 64, 48).to(torch.bfloat16), torch.randn(3, 48, 32).to(torch.bfloat16)
+    mlp = mb.RoutedSwiGLUMLP(w13, w2, precision="fp8")
+    before = {k: v.clone() for k, v in mlp.named_buffers()}
+    assert len(before) == 4
+    for k, v in cast(mlp).named_buffers():
+        assert v.dtype == before[k].dtype == (F8 if k.endswith("codes") else F32) and torch.equal(v.float(), before[k].float())
+    moved = mlp.to("meta", torch.bfloat16)
+    assert all(b.device.type == "meta" and b.dtype == before[k].dtype for k, b in moved.named_buffers())
+    trainable = mb.RoutedSwiGLUMLP(w13, w2).float()
+    assert all(p.dtype == F32 for p in trainable.parameters())
+
+
 @pytest.mark.parametrize("shape", [(32,), (), (1, 2, 32, 32)])
 def test_weights_of_other_ranks_are_refused(shape):
     for quantiser in (mb.quantize_fp8_weight, mb.quantize_fp8_gate_up):
