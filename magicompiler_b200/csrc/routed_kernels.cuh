@@ -188,6 +188,11 @@ __device__ __forceinline__ RowPiece row_piece(int col_chunks) {
   p.c = (blockIdx.x % col_chunks) * blockDim.x + threadIdx.x;
   return p;
 }
+// Whether row s holds no slot.
+__device__ __forceinline__ bool empty_row(const int* row_slot, long long s, long long R) {
+  const int slot = row_slot[s];
+  return slot < 0 || slot >= R;
+}
 // A load of data that is used once.  Volatile, so that it stays behind grid_dependency_wait (the compiler may move a
 // read-only load or the intrinsic in front of it).
 __device__ __forceinline__ uint4 ld_stream(const uint4* p) {
@@ -210,7 +215,7 @@ expert_gather_kernel(const uint4* x, long long ldx, const int* row_slot, const i
     const long long s = p.t * k + j;
     const int r = slot_row[s];
     if (r >= 0 && r < R) xs[(long long)r * vecs + p.c] = v;
-    if (row_slot[s] < 0) xs[s * vecs + p.c] = make_uint4(0, 0, 0, 0);
+    if (empty_row(row_slot, s, R)) xs[s * vecs + p.c] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -314,7 +319,7 @@ expert_combine_backward_kernel(const uint4* dout, long long lddout, const uint4*
       r[i] = on ? slot_row[s] : -1;
       if (r[i] >= R) r[i] = -1;
       wj[i] = (r[i] >= 0 && dy) ? w[s] : 0.0f;
-      if (on && dy && row_slot[s] < 0) empty |= 1u << i;
+      if (on && dy && empty_row(row_slot, s, R)) empty |= 1u << i;
     }
     if (here)
       for (int c = part * 32 + lane; c < vecs; c += step) {
@@ -445,7 +450,7 @@ quantize_fp8_block_kernel(const uint4* x, long long ldx, const int* row_slot, co
       codes[(long long)r * pieces + p.c] = q;
       if (writes_scale) scales[(long long)r * kb + (p.c >> 3)] = s;
     }
-    if (row_slot[sl] < 0) {
+    if (empty_row(row_slot, sl, R)) {
       codes[sl * pieces + p.c] = make_uint4(0, 0, 0, 0);
       if (writes_scale) scales[sl * kb + (p.c >> 3)] = kScaleFloor;
     }

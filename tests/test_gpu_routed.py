@@ -242,6 +242,26 @@ def test_indices_out_of_range_touch_nothing_outside():
     assert torch.equal(mb.expert_combine(y, None, row_slot, slot_row)[0], y[0])
 
 
+def test_a_row_whose_slot_is_out_of_range_holds_none():
+    """As for -1: zero rows, zero codes and the smallest scale, zero gradients, also in memory that held something else."""
+    T, k, H = 6, 2, 256
+    ids = torch.arange(T * k, device="cuda").view(T, k) % 3
+    ids[4:] = -1
+    row_slot, slot_row, offsets = mb.expert_sort(ids, 3)
+    n, bad = int(offsets[-1]), row_slot.clone()
+    bad[n:] = torch.tensor([T * k, 2 ** 31 - 1, -1, -(2 ** 31)], dtype=torch.int32, device="cuda")
+    x, y, w, d = rows_of(T, H, 1), rows_of(T * k, H, 2), torch.rand(T, k, device="cuda"), rows_of(T, H, 3)
+    xs = mb.expert_gather_out(x, bad, slot_row, out=torch.full((T * k, H), 7.0, dtype=BF, device="cuda"))
+    assert torch.equal(xs, mb.expert_gather(x, row_slot, slot_row)) and (xs[n:] == 0).all()
+    filled = (torch.full((T * k, H), 7.0, device="cuda").to(torch.float8_e4m3fn), torch.full((T * k, 2), 7.0, device="cuda"))
+    codes, scales = mb.expert_gather_fp8_out(x, bad, slot_row, out=filled)
+    assert (codes[n:].float() == 0).all() and (scales[n:] == 2.0 ** -126).all()
+    assert torch.equal(codes.float(), mb.expert_gather_fp8(x, row_slot, slot_row)[0].float())
+    torch.full((T * k, H), float("nan"), dtype=BF, device="cuda")  # the block that dy is likely to get
+    dy, _ = mb.expert_combine_backward(d, y, w, bad, slot_row, True, False)
+    assert torch.equal(dy, mb.expert_combine_backward(d, y, w, row_slot, slot_row, True, False)[0]) and (dy[n:] == 0).all()
+
+
 def plain_quantise(x):
     """The formula in fp32, element by element (IEEE divisions)."""
     M, K = x.shape
