@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define MAGI_SWIGLU_ABI_VERSION 9
+#define MAGI_SWIGLU_ABI_VERSION 10
 
 /* variant selector of magi_swiglu_forward_bf16 */
 #define MAGI_SWIGLU_VARIANT_AUTO   0  /* M <= 128 -> STREAM, else MMA2           */
@@ -362,8 +362,10 @@ int magi_swiglu_plan(int64_t M, int64_t N, int64_t K, int variant,
 
 /* Reads (and clears) the device-side watchdog word of `device`.  Every wait in
  * the kernels is bounded; a wait that expires records
- * out[0]=code (0 = none; 1 = X producer, 2 = mma issuer, 3 = epilogue, 4 = W producer, 7 = self-test),
- * out[1]=block index, out[2]=pipeline stage or accumulator buffer, out[3]=phase.
+ * out[0]=code (0 = none; 1 = X producer, 2 = mma issuer, 3 = epilogue, 4 = W producer, in the fp8 products the
+ * scales' warp, 7 = self-test), out[1]=block index, out[2]=pipeline stage or accumulator buffer, out[3]=phase.
+ * The bf16 kernels and the fp8 products keep a word each: when both are set, the first call reads (and clears) the
+ * bf16 kernels' and the next one the other, so a caller that clears asks until the code is 0.
  * A kernel whose wait expired returns normally (tensor memory freed, context usable) but its output is
  * incomplete, and the host learns of it ONLY here: callers poll this at a point where they synchronise anyway.
  * This call SYNCHRONISES the device; it is for tests and debugging.
@@ -406,6 +408,10 @@ int magi_swiglu_tuning(int knob, int value);
  * faults.  For tests of the give-up / report / clear path.
  * Replaces: nothing in the reference. */
 int magi_swiglu_watchdog_selftest(int device, void* cuda_stream, int64_t limit_cycles);
+
+/* The same for the bounded wait of the block-scaled fp8 products: records {code 7, block 0, index 43, phase 0}.
+ * Replaces: nothing in the reference. */
+int magi_swiglu_fp8_block_watchdog_selftest(int device, void* cuda_stream, int64_t limit_cycles);
 
 /* SM clock the most recent MMA/MMA2/STREAM kernel on `device` really ran at: out[0] = average MHz
  * (SM cycles / wall nanoseconds, both read inside the kernel by block 0), out[1] = that span in

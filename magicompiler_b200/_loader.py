@@ -26,7 +26,7 @@ NVCC_FLAGS = [
     "-shared", "-Xcompiler", "-fPIC",
 ]
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 VARIANT_AUTO, VARIANT_MMA, VARIANT_STREAM, VARIANT_SIMT, VARIANT_MMA2 = 0, 1, 2, 3, 4
 VARIANTS = {"auto": VARIANT_AUTO, "mma": VARIANT_MMA, "stream": VARIANT_STREAM, "simt": VARIANT_SIMT,
             "mma2": VARIANT_MMA2}
@@ -141,6 +141,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.magi_swiglu_tuning.argtypes = [i32, i32]
     lib.magi_swiglu_watchdog_selftest.restype = i32
     lib.magi_swiglu_watchdog_selftest.argtypes = [i32, vp, i64]
+    lib.magi_swiglu_fp8_block_watchdog_selftest.restype = i32
+    lib.magi_swiglu_fp8_block_watchdog_selftest.argtypes = [i32, vp, i64]
     lib.magi_swiglu_kernel_clock.restype = i32
     lib.magi_swiglu_kernel_clock.argtypes = [i32, ctypes.POINTER(ctypes.c_double)]
     lib.magi_swiglu_last_error.restype = ctypes.c_char_p
@@ -234,7 +236,8 @@ def workspace_bytes(M: int, N: int, K: int, variant: str | int = "auto", block_n
 
 
 def device_status(device: int = 0) -> dict:
-    """Read and clear the kernels' watchdog word (synchronises the device)."""
+    """Read and clear the kernels' watchdog word (synchronises the device).  The bf16 kernels and the fp8 products have one
+    each; when both are set, the next call reads the second."""
     lib = load_library()
     out = (ctypes.c_int32 * 4)()
     rc = lib.magi_swiglu_device_status(device, out)

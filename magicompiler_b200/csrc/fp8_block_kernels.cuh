@@ -35,7 +35,7 @@ __device__ unsigned int g_fp8_watchdog[4];  // {role that gave up, block, stage/
 
 // Bounded wait: after kWaitLimit the waiting role records itself, raises the CTA's abort flag and every role leaves.
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned role,
-                                             unsigned idx) {
+                                             unsigned idx, long long limit = kWaitLimit) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   unsigned spins = 0;
@@ -43,7 +43,7 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, vola
     if (mbar_try_wait(bar, parity)) return true;
     if ((++spins & 255u) == 0u) {
       if (*abort_flag) return false;
-      if (clock64() - t0 > kWaitLimit) {
+      if (clock64() - t0 > limit) {
         *abort_flag = 1;
         if (atomicCAS(&g_fp8_watchdog[0], 0u, role) == 0u) {
           g_fp8_watchdog[1] = blockIdx.x;
@@ -79,6 +79,20 @@ __device__ __forceinline__ bool wait_bounded_all(uint32_t bar, uint32_t parity, 
       if (__any_sync(0xffffffffu, late || *abort_flag != 0)) return false;
     }
   }
+}
+
+// The wait by itself, on a barrier that nothing signals: records {role 7, block 0, index 43, parity 0} after `limit` cycles.
+__global__ void fp8_watchdog_selftest_kernel(long long limit) {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ int abort_flag;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    mbar_init(smem_u32(&bar), 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) wait_bounded(smem_u32(&bar), 0u, &abort_flag, 7u, 43u, limit);
+  __syncthreads();
 }
 
 struct Args {

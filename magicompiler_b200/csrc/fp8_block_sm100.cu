@@ -320,4 +320,17 @@ int magi_swiglu_gemm_swiglu_fp8_block(const void* a, const float* a_scale, const
   return fp8::run(p, device, cuda_stream);
 }
 
+int magi_swiglu_fp8_block_watchdog_selftest(int device, void* cuda_stream, int64_t limit_cycles) {
+  g_err[0] = 0;
+  if (limit_cycles < 1000 || limit_cycles > 2000000000LL)
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "limit_cycles=%lld out of range [1000, 2e9]", (long long)limit_cycles);
+  if (!device_info(device)) return fail(MAGI_SWIGLU_ERR_DEVICE, "device %d is not available", device);
+  DeviceGuard guard;
+  cudaError_t e = guard.set(device);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  fp8::fp8_watchdog_selftest_kernel<<<1, 32, 0, static_cast<cudaStream_t>(cuda_stream)>>>((long long)limit_cycles);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_watchdog_selftest_kernel");
+}
+
 }  // extern "C"

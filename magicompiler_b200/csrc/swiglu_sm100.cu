@@ -746,10 +746,10 @@ int magi_swiglu_device_status(int device, int32_t out[4]) {
     e = cudaMemcpyToSymbol(magi::g_watchdog, zero, sizeof(zero));
     if (e != cudaSuccess) return magi::fail_cuda(e, "cudaMemcpyToSymbol(g_watchdog)");
   }
-  unsigned int fp8[4] = {0, 0, 0, 0};  // the block-scaled products keep a word of their own
-  e = magi::fp8_block_watchdog(fp8);
-  if (e != cudaSuccess) return magi::fail_cuda(e, "reading the watchdog of the fp8 products");
-  if (host[0] == 0) memcpy(host, fp8, sizeof(host));
+  if (host[0] == 0) {  // the block-scaled products keep a word of their own: with both set, the next call reports it
+    e = magi::fp8_block_watchdog(host);
+    if (e != cudaSuccess) return magi::fail_cuda(e, "reading the watchdog of the fp8 products");
+  }
   for (int i = 0; i < 4; ++i) out[i] = (int32_t)host[i];
   return 0;
 }

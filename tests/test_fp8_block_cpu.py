@@ -175,6 +175,11 @@ def test_a_cast_of_the_module_leaves_codes_and_scales(cast):
     assert all(p.dtype == F32 for p in trainable.parameters())
 
 
+def test_watchdog_selftest_rejects_on_the_host():
+    selftest = mb.load_library().magi_swiglu_fp8_block_watchdog_selftest
+    assert selftest(0, None, 10) == -2 and selftest(0, None, 10 ** 10) == -2 and selftest(1000, None, 2000) == -5
+
+
 @pytest.mark.parametrize("shape", [(32,), (), (1, 2, 32, 32)])
 def test_weights_of_other_ranks_are_refused(shape):
     for quantiser in (mb.quantize_fp8_weight, mb.quantize_fp8_gate_up):

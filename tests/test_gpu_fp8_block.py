@@ -11,6 +11,7 @@ import pytest
 import torch
 
 import magicompiler_b200 as mb
+from magicompiler_b200 import _loader
 
 pytestmark = pytest.mark.gpu
 F8, BF = torch.float8_e4m3fn, torch.bfloat16
@@ -355,6 +356,21 @@ def test_two_streams_at_once_and_beside_the_bf16_kernels():
     torch.cuda.synchronize()
     for i, outs in got:
         assert all(torch.equal(o.float(), ref) for o, ref in zip(outs, want[i]))
+    assert mb.device_status(0)["code"] == 0
+
+
+def test_both_watchdog_records_are_reported():
+    """A wait of each kind runs out (on a barrier that nothing signals): neither record is lost."""
+    lib, stream = _loader.load_library(), torch.cuda.current_stream().cuda_stream
+    assert mb.device_status(0)["code"] == 0
+    assert lib.magi_swiglu_fp8_block_watchdog_selftest(0, stream, 2_000_000) == 0, _loader.last_error()
+    assert mb.device_status(0) == {"code": 7, "block": 0, "index": 43, "parity": 0}
+    assert mb.device_status(0)["code"] == 0
+    assert lib.magi_swiglu_watchdog_selftest(0, stream, 2_000_000) == 0
+    assert lib.magi_swiglu_fp8_block_watchdog_selftest(0, stream, 2_000_000) == 0
+    assert [mb.device_status(0)["index"] for _ in range(3)] == [42, 43, 0]
+    t = case(17, 384, 256)
+    check_plain(t, mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"]))
     assert mb.device_status(0)["code"] == 0
 
 
