@@ -360,6 +360,15 @@ int magi_swiglu_plan(int64_t M, int64_t N, int64_t K, int variant,
                      int block_n, int stages, int group_m, int max_ctas,
                      int device, int sm_count, int32_t out[16]);
 
+/* Describes the kernel the block-scaled fp8 products would use, without launching: halves 1 = magi_swiglu_gemm_fp8_block,
+ * 2 = magi_swiglu_gemm_swiglu_fp8_block; num_experts 0 = no offsets.  out[0] = rows of A a tile of the stream kernel holds
+ * (0 = tile kernel), out[1] = CTAs a tile (stream and single-CTA tiles 1, pairs 2), out[2] = CTAs (of pairs: pairs) that
+ * share a tile's K blocks, out[3] = 0 (reserved).  `sm_count` <= 0 means "query `device`".  Needs no GPU when sm_count > 0
+ * (it then takes every cluster size to fit as often as there are SMs for it).
+ * Replaces: nothing in the reference. */
+int magi_swiglu_fp8_block_plan(int halves, int64_t M, int64_t N, int64_t K, int num_experts, int device, int sm_count,
+                               int32_t out[4]);
+
 /* Reads (and clears) the device-side watchdog word of `device`.  Every wait in
  * the kernels is bounded; a wait that expires records
  * out[0]=code (0 = none; 1 = X producer, 2 = mma issuer, 3 = epilogue, 4 = W producer, in the fp8 products the
@@ -392,6 +401,10 @@ int magi_swiglu_schedule(int64_t M, int64_t N, int64_t K, int variant, int block
  *   STREAM_K  0 / 1: never / whenever possible, balance the last waves of the tile schedules by K ranges (-1 = choose)
  *   L2_HINTS  three decimal digits xwy, each 0 normal / 1 evict-first / 2 evict-last, for X tiles, W tiles and Y
  *             stores (-1 = defaults)
+ *   FP8_FORM  the kernel of the block-scaled fp8 products (0 = choose): 16, 32, 64 (64: plain only) = the stream kernel
+ *             with that many rows of A a tile, plus 256 * z (z 1, 2, 4, 8) to let z CTAs share a tile's K blocks;
+ *             1 = tiles of one CTA; 2, 4, 8 = tiles of CTA pairs, 1, 2 or 4 pairs to a tile's K blocks.  A call that
+ *             the form cannot serve is refused with MAGI_SWIGLU_ERR_VARIANT.
  *   SCATTER_WIDE 0 / 1: the scattered GEMM stores 32-column boxes always / 64-column boxes where the tile allows
  * Replaces: nothing in the reference. */
 #define MAGI_SWIGLU_TUNE_K_SPLITS 0
@@ -400,6 +413,7 @@ int magi_swiglu_schedule(int64_t M, int64_t N, int64_t K, int variant, int block
 #define MAGI_SWIGLU_TUNE_L2_HINTS 3
 #define MAGI_SWIGLU_TUNE_STREAM_K 4
 #define MAGI_SWIGLU_TUNE_SCATTER_WIDE 5
+#define MAGI_SWIGLU_TUNE_FP8_FORM 6
 int magi_swiglu_tuning(int knob, int value);
 
 /* Runs the kernels' bounded wait by itself: a one-block kernel whose thread 0 waits on an mbarrier that nothing

@@ -132,6 +132,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.magi_swiglu_workspace_bytes.argtypes = [i64, i64, i64, i32, i32, i32, i32, i32, i32, i32]
     lib.magi_swiglu_plan.restype = i32
     lib.magi_swiglu_plan.argtypes = [i64, i64, i64, i32, i32, i32, i32, i32, i32, i32, ctypes.POINTER(ctypes.c_int32)]
+    lib.magi_swiglu_fp8_block_plan.restype = i32
+    lib.magi_swiglu_fp8_block_plan.argtypes = [i32, i64, i64, i64, i32, i32, i32, ctypes.POINTER(ctypes.c_int32)]
     lib.magi_swiglu_device_status.restype = i32
     lib.magi_swiglu_device_status.argtypes = [i32, ctypes.POINTER(ctypes.c_int32)]
     lib.magi_swiglu_schedule.restype = i32
@@ -173,12 +175,12 @@ def load_library() -> ctypes.CDLL:
     return lib
 
 
-TUNING_KNOBS = {"k_splits": 0, "no_split": 1, "y_tma": 2, "l2_hints": 3, "stream_k": 4, "scatter_wide": 5}
+TUNING_KNOBS = {"k_splits": 0, "no_split": 1, "y_tma": 2, "l2_hints": 3, "stream_k": 4, "scatter_wide": 5, "fp8_form": 6}
 _tuning_epoch = 0  # bumped by set_tuning so host-side caches keyed on the schedule notice
 
 
 def set_tuning(knob: str, value: int) -> int:
-    """Set a tuning aid of the library (``magi_swiglu_tuning``: k_splits, no_split, y_tma, l2_hints) and return its
+    """Set a tuning aid of the library (``magi_swiglu_tuning``; ``TUNING_KNOBS``) and return its
     previous value.  Process-wide; for tests and sweeps."""
     global _tuning_epoch
     lib = load_library()
@@ -207,6 +209,17 @@ def plan(M: int, N: int, K: int, variant: str | int = "auto", block_n: int = 0, 
     keys = ["variant", "block_n", "stages", "grid", "tiles", "smem_bytes", "acc_bufs", "n_mma", "ctas", "group_m", "split", "k_splits",
             "y_tma", "sk_tiles"]
     return dict(zip(keys, list(out)[:len(keys)]))
+
+
+def fp8_block_plan(M: int, N: int, K: int, halves: int = 1, experts: int = 0, device: int = 0, sm_count: int = 0) -> dict:
+    """The kernel a block-scaled fp8 product would use (``magi_swiglu_fp8_block_plan``; ``halves`` 2: the SwiGLU form;
+    ``experts`` 0: without offsets): ``tokens`` a tile of the stream kernel (0: tile kernel), ``ctas`` a tile, ``splits``
+    of its K blocks.  Pure host arithmetic when ``sm_count`` > 0."""
+    out = (ctypes.c_int32 * 4)()
+    rc = load_library().magi_swiglu_fp8_block_plan(halves, M, N, K, experts, device, sm_count, out)
+    if rc != 0:
+        raise ValueError(f"magi_swiglu_fp8_block_plan failed ({rc}): {last_error()}")
+    return {"tokens": out[0], "ctas": out[1], "splits": out[2]}
 
 
 def schedule(M: int, N: int, K: int, unit: int, variant: str | int = "auto", block_n: int = 0, stages: int = 0,

@@ -38,23 +38,30 @@ struct Problem {
   long long lda;
   int64_t M, N, K;
   int halves;
+  bool routed;  // rows belong to experts (offsets)
   Args args;
+};
+
+// Which kernel runs: the stream kernel with `tok` rows a tile, or (tok 0) tiles of `ctas` CTAs; `splits` CTAs or pairs of a
+// cluster share a tile's K blocks.
+struct Form {
+  int tok, ctas, splits;
 };
 
 // Row groups of `rows` rows: every expert adds at most one partial group.
 static int64_t most_groups(const Problem& p, int rows) {
-  return p.args.offsets ? p.M / rows + (p.M < p.args.E + 1 ? p.M : p.args.E + 1) : (p.M + rows - 1) / rows;
+  return p.routed ? p.M / rows + (p.M < p.args.E + 1 ? p.M : p.args.E + 1) : (p.M + rows - 1) / rows;
 }
 // What to expect of them: experts' shares are uneven, and an exponentially distributed share of mean s needs 1 / (1 -
 // exp(-rows / s)) groups on average (one for a small share, s / rows + 1/2 for a large one).
 static double expected_groups(const Problem& p, int rows) {
-  if (!p.args.offsets) return (double)((p.M + rows - 1) / rows);
+  if (!p.routed) return (double)((p.M + rows - 1) / rows);
   const double used = (double)(p.M < p.args.E ? p.M : p.args.E);
   return used / (1.0 - exp(-rows * used / (double)p.M));
 }
 // Rounds of `workers` at a time; an expected count may miss by a few per cent, which must not make a round.
 static double rounds_of(const Problem& p, double tiles, double workers) {
-  return p.args.offsets ? fmax(1.0, ceil(0.97 * tiles / workers)) : ceil(tiles / workers);
+  return p.routed ? fmax(1.0, ceil(0.97 * tiles / workers)) : ceil(tiles / workers);
 }
 
 template <int kHalves, int kTok>
@@ -146,7 +153,7 @@ static int tile_log_splits(int64_t most, int kb, const int (&clusters)[3]) {
 }
 
 template <int kHalves, int kCtas>
-static int launch_tiles(const Problem& p, int log_splits, int most_workers, cudaStream_t stream) {
+static int launch_tiles(const Problem& p, int splits, int most_workers, cudaStream_t stream) {
   constexpr int kTileRows = Tile<kCtas>::kRows;
   const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.args.E * kHalves};
   const cuuint64_t wst[2] = {(cuuint64_t)p.K, (cuuint64_t)p.N * (cuuint64_t)p.K};
@@ -161,39 +168,30 @@ static int launch_tiles(const Problem& p, int log_splits, int most_workers, cuda
   if (units * n_tiles > 0x7fffffffLL / 2) return fail(MAGI_SWIGLU_ERR_SHAPE, "M=%lld x N=%lld is too large for one launch", (long long)p.M, (long long)p.N);
   const int64_t most = units * n_tiles;
   Args args = p.args;
-  args.splits = 1 << log_splits;
+  args.splits = splits;
   // A raster band of about 32 MB of A: it is read once per column tile and should stay in L2 beside the W rows that pass
   // (8192 rows: K = 4096, N = 2 x 14336: bands of 8 / 16 / 32 groups 980 / 948 / 942 us; K = 14336: 447 / 451 / 468 us).
   const int64_t band = (32LL << 20) / (kTileRows * p.K);
   args.band = (int)(band < 4 ? 4 : (band > 64 ? 64 : band));
   const int64_t workers = most < most_workers ? most : most_workers;
   const int wide = ((uintptr_t)p.args.c & 31u) == 0 && p.N % 16 == 0;
-  const cudaError_t e = launch(fp8_block_tile_kernel<kHalves, kCtas>, dim3((unsigned)(workers * (kCtas << log_splits))),
-                               dim3(kTileThreads), Tile<kCtas>::kSmem, stream, (unsigned)kCtas << log_splits, false, tm_w, tm_a, args, wide);
+  const cudaError_t e = launch(fp8_block_tile_kernel<kHalves, kCtas>, dim3((unsigned)(workers * kCtas * splits)),
+                               dim3(kTileThreads), Tile<kCtas>::kSmem, stream, (unsigned)(kCtas * splits), false, tm_w, tm_a, args, wide);
   return e == cudaSuccess ? 0 : fail_cuda(e, "launch of fp8_block_tile_kernel");
 }
 
-static int run(const Problem& p, int device, void* cuda_stream) {
-  const DeviceInfo* di = nullptr;
-  if (int rc = require_b200(device, &di)) return rc;
-  DeviceGuard guard;
-  cudaError_t e = guard.set(device);
-  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
-  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  // The kernel and its tokens per tile by what the forms are expected to take: rounds of the GPU's CTAs (pairs), each a
-  // fixed part and a part per K block.  The constants are microseconds measured with everything in flight (148 SMs):
-  // stream kernel, two CTAs an SM, 0.36 / 0.43 / 0.50 a K block for 16 / 32 / 64 tokens, 0.75 / 0.90 for 16 / 32 in the
-  // SwiGLU form, about 0.6 of that with one CTA an SM, and 3.0; tile kernel 0.42 a K block and 2.5 a tile.  Both sides at N = 4096,
-  // K = 14336 (stream 16 / 32 / 64 tokens, tiles): M = 64 26 / 18 / 16 / 35 us, 256 - / 47 / 35 / 35 us, 512 - / - / 58 /
-  // 37 us; SwiGLU, N = 1408, K = 2048, 64 experts (16 / 32 tokens, tiles): 512 rows 52 / 48 / 78 us, 2048 rows 85 / 75 / 96
-  // us, 8192 rows 295 / 199 / 138 us.  None is faster than W's bytes (6.2 TB/s).  Forms that are bound by them alike differ
-  // in what an uneven share costs: then the wider tile, up to 2.5 times the average share (8 experts, 74 rows, N = 4096, K =
-  // 14336: 16 tokens 69 to 87 us from routing to routing, 32 tokens 69 to 74 us).
-  int clusters[3];
-  if (int rc = p.halves == 1 ? tile_clusters<1>(device, di->sm_count, clusters) : tile_clusters<2>(device, di->sm_count, clusters))
-    return rc;
+// The kernel and its tokens per tile by what the forms are expected to take: rounds of the GPU's CTAs (pairs), each a
+// fixed part and a part per K block.  The constants are microseconds measured with everything in flight (148 SMs):
+// stream kernel, two CTAs an SM, 0.36 / 0.43 / 0.50 a K block for 16 / 32 / 64 tokens, 0.75 / 0.90 for 16 / 32 in the
+// SwiGLU form, about 0.6 of that with one CTA an SM, and 3.0; tile kernel 0.42 a K block and 2.5 a tile.  Both sides at N = 4096,
+// K = 14336 (stream 16 / 32 / 64 tokens, tiles): M = 64 26 / 18 / 16 / 35 us, 256 - / 47 / 35 / 35 us, 512 - / - / 58 /
+// 37 us; SwiGLU, N = 1408, K = 2048, 64 experts (16 / 32 tokens, tiles): 512 rows 52 / 48 / 78 us, 2048 rows 85 / 75 / 96
+// us, 8192 rows 295 / 199 / 138 us.  None is faster than W's bytes (6.2 TB/s).  Forms that are bound by them alike differ
+// in what an uneven share costs: then the wider tile, up to 2.5 times the average share (8 experts, 74 rows, N = 4096, K =
+// 14336: 16 tokens 69 to 87 us from routing to routing, 32 tokens 69 to 74 us).
+static Form choose(const Problem& p, int sm_count, const int (&clusters)[3]) {
   const double n128 = (double)((p.N + 127) / 128);
-  const double used = p.args.offsets ? (double)(p.M < p.args.E ? p.M : p.args.E) : 1.0, share = p.M / used;
+  const double used = p.routed ? (double)(p.M < p.args.E ? p.M : p.args.E) : 1.0, share = p.M / used;
   const double bytes_us = used * p.halves * p.N * p.K / 6.2e6 + 3.0;
   double best = 0;
   int tok = 0, splits = 1;
@@ -210,7 +208,7 @@ static int run(const Problem& p, int device, void* cuda_stream) {
   {
     const double rounds = rounds_of(p, expected_groups(p, Tile<2>::kRows) * n_tiles, clusters[log_splits]);
     best = 5.0 + rounds * (p.args.kb * 0.42 / (1 << log_splits) + 2.5) + (log_splits ? 3.0 : 0.0);
-    const double rounds1 = rounds_of(p, expected_groups(p, Tile<1>::kRows) * n_tiles, di->sm_count);
+    const double rounds1 = rounds_of(p, expected_groups(p, Tile<1>::kRows) * n_tiles, sm_count);
     // warps without rows skip their work: nearly empty tiles take about 0.7 of a full one's time
     const double fill = share < 64 ? share / 64 : 1.0;
     const double cost1 = 3.0 + rounds1 * (p.args.kb * 0.42 + 2.5) * (p.K % 32 ? 1.5 : 1.12) * (0.7 + 0.3 * fill);
@@ -223,21 +221,62 @@ static int run(const Problem& p, int device, void* cuda_stream) {
     if (most_groups(p, 16 << i) > 65535) continue;
     const double ctas = n128 * expected_groups(p, 16 << i);
     int z = 1;  // up to eight CTAs of a cluster share a tile's K blocks, at least four each, until there are about two CTAs an SM
-    while (z < 8 && ctas * z * 2 <= 2 * di->sm_count && p.args.kb >= z * 8) z *= 2;
-    const double rounds = rounds_of(p, ctas * z, 2 * di->sm_count);
-    double cost = 2.5 + rounds * (p.args.kb * per_block[p.halves - 1][i] / z * (ctas * z <= di->sm_count ? 0.6 : 1.0) + 3.0);
+    while (z < 8 && ctas * z * 2 <= 2 * sm_count && p.args.kb >= z * 8) z *= 2;
+    const double rounds = rounds_of(p, ctas * z, 2 * sm_count);
+    double cost = 2.5 + rounds * (p.args.kb * per_block[p.halves - 1][i] / z * (ctas * z <= sm_count ? 0.6 : 1.0) + 3.0);
     if (cost < bytes_us) cost = bytes_us;
-    if (cost < best || (cost == best && (tok == 0 || (p.args.offsets && tok < 2.5 * share)))) best = cost, tok = 16 << i, splits = z;
+    if (cost < best || (cost == best && (tok == 0 || (p.routed && tok < 2.5 * share)))) best = cost, tok = 16 << i, splits = z;
   }
+  if (tok) return Form{tok, 1, splits};
+  return single ? Form{0, 1, 1} : Form{0, 2, 1 << log_splits};
+}
+
+// The form MAGI_SWIGLU_TUNE_FP8_FORM asks for, if it can serve this call.
+static int forced(const Problem& p, int value, const int (&clusters)[3], Form* f) {
+  const int base = value & 255, z = value >> 8;
+  bool ok = false;
+  if (base == 16 || base == 32 || (base == 64 && p.halves == 1)) {
+    *f = Form{base, 1, z ? z : 1};
+    ok = (z == 0 || z == 1 || z == 2 || z == 4 || z == 8) && f->splits <= p.args.kb && most_groups(p, base) <= 65535;
+  } else if (base == 1 && z == 0) {
+    *f = Form{0, 1, 1};
+    ok = true;
+  } else if ((base == 2 || base == 4 || base == 8) && z == 0) {
+    *f = Form{0, 2, base / 2};
+    const int64_t tiles = most_groups(p, Tile<2>::kRows) * ((p.N * p.halves + 255) / 256);
+    ok = base == 2 || (f->splits <= p.args.kb && tiles <= clusters[base / 4]);
+  }
+  return ok ? 0 : fail(MAGI_SWIGLU_ERR_VARIANT, "form %d of the fp8 products cannot serve this call", value);
+}
+
+static int form_of(const Problem& p, int sm_count, const int (&clusters)[3], Form* f) {
+  if (const int value = g_fp8_form.load(std::memory_order_relaxed)) return forced(p, value, clusters, f);
+  *f = choose(p, sm_count, clusters);
+  return 0;
+}
+
+static int run(const Problem& p, int device, void* cuda_stream) {
+  const DeviceInfo* di = nullptr;
+  if (int rc = require_b200(device, &di)) return rc;
+  DeviceGuard guard;
+  cudaError_t e = guard.set(device);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  int clusters[3];
+  if (int rc = p.halves == 1 ? tile_clusters<1>(device, di->sm_count, clusters) : tile_clusters<2>(device, di->sm_count, clusters))
+    return rc;
+  Form f;
+  if (int rc = form_of(p, di->sm_count, clusters, &f)) return rc;
+  const int pairs = f.tok ? 0 : clusters[f.splits >> 1];  // workers of 1, 2 or 4 pairs
   if (p.halves == 1) {
-    if (tok == 16) return launch_stream<1, 16>(p, device, splits, stream);
-    if (tok == 32) return launch_stream<1, 32>(p, device, splits, stream);
-    if (tok == 64) return launch_stream<1, 64>(p, device, splits, stream);
-    return single ? launch_tiles<1, 1>(p, 0, di->sm_count, stream) : launch_tiles<1, 2>(p, log_splits, clusters[log_splits], stream);
+    if (f.tok == 16) return launch_stream<1, 16>(p, device, f.splits, stream);
+    if (f.tok == 32) return launch_stream<1, 32>(p, device, f.splits, stream);
+    if (f.tok == 64) return launch_stream<1, 64>(p, device, f.splits, stream);
+    return f.ctas == 1 ? launch_tiles<1, 1>(p, 1, di->sm_count, stream) : launch_tiles<1, 2>(p, f.splits, pairs, stream);
   }
-  if (tok == 16) return launch_stream<2, 16>(p, device, splits, stream);
-  if (tok == 32) return launch_stream<2, 32>(p, device, splits, stream);
-  return single ? launch_tiles<2, 1>(p, 0, di->sm_count, stream) : launch_tiles<2, 2>(p, log_splits, clusters[log_splits], stream);
+  if (f.tok == 16) return launch_stream<2, 16>(p, device, f.splits, stream);
+  if (f.tok == 32) return launch_stream<2, 32>(p, device, f.splits, stream);
+  return f.ctas == 1 ? launch_tiles<2, 1>(p, 1, di->sm_count, stream) : launch_tiles<2, 2>(p, f.splits, pairs, stream);
 }
 
 static int check(const void* a, const float* a_scale, const void* b, const float* b_scale, const int32_t* offsets,
@@ -271,6 +310,7 @@ static Problem problem(const void* a, const float* a_scale, const void* b, const
   p.N = N;
   p.K = K;
   p.halves = halves;
+  p.routed = offsets != nullptr;
   p.args.a_scale = a_scale;
   p.args.b_scale = b_scale;
   p.args.offsets = offsets;
@@ -318,6 +358,34 @@ int magi_swiglu_gemm_swiglu_fp8_block(const void* a, const float* a_scale, const
   p.args.codes = static_cast<uint8_t*>(codes);
   p.args.scales = scales;
   return fp8::run(p, device, cuda_stream);
+}
+
+int magi_swiglu_fp8_block_plan(int halves, int64_t M, int64_t N, int64_t K, int num_experts, int device, int sm_count,
+                               int32_t out[4]) {
+  g_err[0] = 0;
+  if (!out) return fail(MAGI_SWIGLU_ERR_NULL, "out is null");
+  if ((halves != 1 && halves != 2) || M < 1 || N < 1 || K < 1 || M > 0x3fffffffLL || N > 0x3fffffffLL || K > 0x3fffffffLL ||
+      N % (8 * halves) || K % 16 || num_experts < 0 || num_experts > 1024)
+    return fail(MAGI_SWIGLU_ERR_SHAPE, "halves=%d, M=%lld, N=%lld, K=%lld, num_experts=%d out of range", halves, (long long)M,
+                (long long)N, (long long)K, num_experts);
+  int clusters[3] = {sm_count / 2, sm_count / 4, sm_count / 8};
+  if (sm_count <= 0) {
+    const DeviceInfo* di = nullptr;
+    if (int rc = require_b200(device, &di)) return rc;
+    DeviceGuard guard;
+    const cudaError_t e = guard.set(device);
+    if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+    sm_count = di->sm_count;
+    if (int rc = halves == 1 ? fp8::tile_clusters<1>(device, sm_count, clusters) : fp8::tile_clusters<2>(device, sm_count, clusters))
+      return rc;
+  }
+  fp8::Problem p = fp8::problem(nullptr, nullptr, nullptr, nullptr, nullptr, num_experts ? num_experts : 1, M, N, K, K,
+                                (K + 127) / 128, 0, halves);
+  p.routed = num_experts > 0;
+  fp8::Form f;
+  if (int rc = fp8::form_of(p, sm_count, clusters, &f)) return rc;
+  out[0] = f.tok, out[1] = f.ctas, out[2] = f.splits, out[3] = 0;
+  return 0;
 }
 
 int magi_swiglu_fp8_block_watchdog_selftest(int device, void* cuda_stream, int64_t limit_cycles) {

@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -43,6 +44,8 @@ inline EncodeTiledFn tensor_map_encoder() {
   }();
   return fn;
 }
+
+inline std::atomic<int> g_fp8_form{0};  // MAGI_SWIGLU_TUNE_FP8_FORM
 
 constexpr int kMaxDevices = 64;
 struct DeviceInfo {

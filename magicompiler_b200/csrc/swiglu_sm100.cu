@@ -808,6 +808,8 @@ int magi_swiglu_tuning(int knob, int value) {
       prev = t.scatter_wide;
       t.scatter_wide = value != 0;
       return prev;
+    case MAGI_SWIGLU_TUNE_FP8_FORM:
+      return magi::g_fp8_form.exchange(value > 0 ? value : 0);
     case MAGI_SWIGLU_TUNE_STREAM_K:
       prev = t.stream_k;
       t.stream_k = value < 0 ? -1 : (value != 0);

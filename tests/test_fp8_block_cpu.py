@@ -175,6 +175,41 @@ def test_a_cast_of_the_module_leaves_codes_and_scales(cast):
     assert all(p.dtype == F32 for p in trainable.parameters())
 
 
+def plan(*args, form=0, **kw):
+    prev = _loader.set_tuning("fp8_form", form)
+    try:
+        return tuple(_loader.fp8_block_plan(*args, sm_count=148, **kw).values())
+    finally:
+        assert _loader.set_tuning("fp8_form", prev) == form
+
+
+def test_plans_of_the_sizes_that_the_kernels_are_for():
+    assert plan(8192, 4096, 14336) == plan(8192, 14336, 4096, halves=2) == (0, 2, 1)  # long prompts: CTA pairs
+    assert plan(15200, 1424, 2064, halves=2, experts=64) == (0, 2, 1)
+    assert plan(15200, 1408, 2048, halves=2, experts=64) == (0, 1, 1)  # many rows an expert, K a multiple of 32: single CTAs
+    assert plan(4096, 2048, 768, experts=128) == (0, 1, 1)
+    for tokens, ctas, splits in (plan(1, 4096, 14336), plan(16, 28672, 8192, halves=2), plan(74, 4096, 14336, experts=8)):
+        assert tokens in (16, 32, 64) and ctas == 1 and splits in (1, 2, 4, 8)
+
+
+def test_a_form_asked_for_is_the_one_planned_or_refused():
+    for form in (16, 32, 64):
+        assert plan(300, 256, 2048, form=form) == (form, 1, 1) and plan(300, 256, 2048, form=form + 1024, experts=3) == (form, 1, 4)
+    for form, ctas, splits in ((1, 1, 1), (2, 2, 1), (4, 2, 2), (8, 2, 4)):
+        for halves in (1, 2):
+            assert plan(300, 256, 2048, form=form, halves=halves) == (0, ctas, splits)
+    for form, args, kw in ((64, (300, 256, 2048), dict(halves=2)), (8, (300, 256, 384), {}), (16 + 2048, (300, 256, 896), {}),
+                           (8, (8192, 4096, 4096), {}), (4, (8192, 4096, 4096), {}), (16, (2 ** 21, 256, 256), {}),
+                           (16 + 768, (300, 256, 2048), {}), (3, (300, 256, 2048), {}), (128, (300, 256, 2048), {}),
+                           (258, (300, 256, 2048), {})):
+        with pytest.raises(ValueError, match="cannot serve"):
+            plan(*args, form=form, **kw)
+    for args, kw in (((0, 16, 16), {}), ((1, 12, 16), {}), ((1, 8, 16), dict(halves=2)), ((1, 8, 24), {}), ((1, 8, 16), dict(halves=3)),
+                     ((1, 8, 16), dict(experts=1025))):
+        with pytest.raises(ValueError, match="out of range"):
+            plan(*args, **kw)
+
+
 def test_watchdog_selftest_rejects_on_the_host():
     selftest = mb.load_library().magi_swiglu_fp8_block_watchdog_selftest
     assert selftest(0, None, 10) == -2 and selftest(0, None, 10 ** 10) == -2 and selftest(1000, None, 2000) == -5

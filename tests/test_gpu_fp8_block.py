@@ -7,6 +7,8 @@ product and the multiply-add round once each (2^-24), and the additions over the
 SwiGLU: |d(silu(g) u)| <= 1.1 |u| dg + |silu(g)| du (|silu'| < 1.1) plus 2^-20 of the value for the exponential, the
 reciprocal and the products.  A scale is 1/448 of the largest of 128 such values, a code is within half an e4m3 step
 (2^-4 of the value, or 2^-10 of the scale below the smallest normal code) of value / scale."""
+import contextlib
+
 import pytest
 import torch
 
@@ -371,6 +373,155 @@ def test_both_watchdog_records_are_reported():
     assert [mb.device_status(0)["index"] for _ in range(3)] == [42, 43, 0]
     t = case(17, 384, 256)
     check_plain(t, mb.gemm_fp8_block(t["a"], t["a_scale"], t["b"], t["b_scale"]))
+    assert mb.device_status(0)["code"] == 0
+
+
+# ------------------------------------------------------------------------------------------------ every form by itself
+# The library chooses a kernel by the sizes; here each one is asked for: the stream kernel with 16, 32 or 64 rows a tile (+ 256 z:
+# z CTAs share a tile's K blocks), single-CTA tiles (1), tiles of CTA pairs (2) and of 2 or 4 pairs that share K blocks (4, 8).
+KINDS = [(h, f) for h in (1, 2) for f in (16, 32, 64, 256 + 16, 512 + 16, 1024 + 32, 2048 + 32, 2048 + 64, 1, 2, 4, 8)
+         if not (h == 2 and f % 256 == 64)]
+
+
+@contextlib.contextmanager
+def form(value):
+    prev = _loader.set_tuning("fp8_form", value)
+    try:
+        yield
+    finally:
+        _loader.set_tuning("fp8_form", prev)
+
+
+def product(t, halves, offsets=None, out=None):
+    args = (t["a"], t["a_scale"], t["b"], t["b_scale"], t["offsets"] if offsets is None else offsets)
+    if halves == 1:
+        return [mb.gemm_fp8_block(*args) if out is None else mb.gemm_fp8_block_out(*args, out=out[0])]
+    return list(mb.gemm_swiglu_fp8_block(*args) if out is None else mb.gemm_swiglu_fp8_block_out(*args, out=tuple(out)))
+
+
+def check(t, halves, got):
+    check_plain(t, *got) if halves == 1 else check_fused(t, *got)
+
+
+def same(x, y):
+    return all(torch.equal(a.float(), b.float()) for a, b in zip(x, y))
+
+
+def runs(value, M, N, K, halves, experts=0):
+    """Whether the form serves this call, and that it is the one which runs."""
+    with form(value):
+        try:
+            plan = _loader.fp8_block_plan(M, N, K, halves=halves, experts=experts)
+        except ValueError:
+            return False
+    tok = value % 256 if value % 256 >= 16 else 0
+    want = dict(tokens=tok, ctas=1, splits=max(value >> 8, 1)) if tok else dict(tokens=0, ctas=min(value, 2), splits=max(value // 2, 1))
+    assert plan == want
+    return True
+
+
+@pytest.mark.parametrize("halves,value", KINDS)
+@pytest.mark.parametrize("M,N,K", [(1, 16, 1040), (129, 144, 1040), (300, 272, 2064), (257, 128, 1024), (2100, 2576, 400), (1300, 2576, 1296)])
+def test_every_form_dense(halves, value, M, N, K):
+    many = M > 1000  # more tiles than a persistent grid has workers; too many and too short for shared K blocks
+    assert runs(value, M, N, K, halves) or (many and value in (4, 8)) or value >> 8 > -(-K // 128)
+    if not runs(value, M, N, K, halves):
+        return
+    t = case(M, N, K, halves=halves, seed=M)
+    with form(value):
+        got = product(t, halves)
+        check(t, halves, got)
+        assert same(product(t, halves), got)
+    assert mb.device_status(0)["code"] == 0
+
+
+UNEVEN = [([300, 0, 257, 100, 1], 9, 112, 1040), ([300, 0, 257, 100, 1], 9, 272, 2064), ([0, 0, 0], 40, 112, 1040),
+          ([(i * 37) % 400 if i % 3 else 0 for i in range(40)], 300, 1040, 272)]
+
+
+@pytest.mark.parametrize("halves,value", KINDS)
+@pytest.mark.parametrize("counts,tail,N,K", UNEVEN)
+def test_every_form_over_experts(halves, value, counts, tail, N, K):
+    """Empty and partial groups, a tail without experts that comes out as zeros or stays, an expert full of NaN."""
+    n, E = sum(counts), len(counts)
+    assert runs(value, n + tail, N, K, halves, E) or value in (4, 8) and N > 112 or value >> 8 > -(-K // 128)
+    if not runs(value, n + tail, N, K, halves, E):
+        return
+    t = case(n + tail, N, K, E=E, counts=counts, halves=halves, seed=N)
+    with form(value):
+        got = product(t, halves)
+        check(t, halves, got)
+        assert (got[0][n:].float() == 0).all() and (halves == 1 or (got[1][n:] == 2.0 ** -126).all())
+        held = [torch.full((g.shape[0] + 8, g.shape[1]), 5.0, device="cuda").to(g.dtype) for g in got]
+        product(t, halves, out=[h[4:-4] for h in held])
+        for h, g in zip(held, got):
+            assert torch.equal(h[4:4 + n].float(), g[:n].float()) and (h[:4].float() == 5).all() and (h[4 + n:].float() == 5).all()
+        if n:
+            lo, hi = int(t["offsets"][2]), int(t["offsets"][3])  # the third expert
+            t["a"].view(torch.uint8)[lo:hi] = 127  # NaN in e4m3
+            again = product(t, halves)
+            keep = torch.ones(n + tail, dtype=torch.bool, device="cuda")
+            keep[lo:hi] = False
+            for x, g in zip(again, got):
+                assert torch.equal(x[keep].float(), g[keep].float()) and x[lo:hi].float().isnan().all()
+    assert mb.device_status(0)["code"] == 0
+
+
+@pytest.mark.parametrize("halves,value", KINDS)
+@pytest.mark.parametrize("M,offsets", FALLING)
+def test_every_form_with_falling_offsets(halves, value, M, offsets):
+    E, hull, K = len(offsets) - 1, fallen(offsets, M), 1040
+    t = case(M, 112, K, E=E, counts=[0] * E, halves=halves, seed=M)
+    bad, t["offsets"] = (torch.tensor(o, dtype=torch.int32, device="cuda") for o in (offsets, hull))
+    assert runs(value, M, 112, K, halves, E) or value in (4, 8) and E > 7
+    if not runs(value, M, 112, K, halves, E):
+        return
+    with form(value):
+        want = product(t, halves)
+        held = [torch.full((g.shape[0] + 8, g.shape[1]), 5.0, device="cuda").to(g.dtype) for g in want]
+        product(t, halves, offsets=bad, out=[h[4:-4] for h in held])
+        lo, hi = hull[0], hull[-1]
+        for h, g in zip(held, want):
+            assert torch.equal(h[4 + lo:4 + hi].float(), g[lo:hi].float())
+            assert (h[:4 + lo].float() == 5).all() and (h[4 + hi:].float() == 5).all()
+        if lo == 0:
+            check(t, halves, want)
+    assert mb.device_status(0)["code"] == 0
+
+
+@pytest.mark.parametrize("halves", [1, 2])
+def test_single_tiles_and_pairs_give_the_same_bits(halves):
+    t = case(900, 528, 1296, E=3, counts=[257, 0, 600], halves=halves)
+    with form(1):
+        one = product(t, halves)
+    with form(2):
+        assert same(product(t, halves), one)
+
+
+@pytest.mark.parametrize("halves,value", KINDS)
+def test_every_form_captured_beside_other_kernels(halves, value):
+    """Replayed with new rows between kernels that it overlaps; what it answers is what an eager call answers."""
+    counts = [130, 0, 64, 6]
+    t = case(200, 144, 1040, E=4, counts=counts, halves=halves, seed=3)
+    x = torch.randn(200, 1040, generator=gen(5), device="cuda").to(BF)
+
+    def step():
+        t["a"], t["a_scale"] = mb.quantize_fp8_block_out(x)
+        return product(t, halves)
+
+    with form(value):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        for seed in (6, 7):
+            x.copy_(torch.randn(200, 1040, generator=gen(seed), device="cuda"))
+            graph.replay()
+            assert same(held, step())
     assert mb.device_status(0)["code"] == 0
 
 
