@@ -329,8 +329,10 @@ int magi_swiglu_gemm_fp8_block(const void* a, const float* a_scale, const void* 
                                int64_t lda, int64_t ld_scale, int zero_tail, int device, void* cuda_stream);
 
 /* The fused SwiGLU form: y = silu(A . Wg^T) * (A . Wu^T) on the scaled fp32 sums, quantised in the epilogue to codes [M, N]
- * e4m3 and scales [M, ceil(N/128)] fp32 (scale = max(max|y| / 448, 2^-126) per row and 128 columns, code = e4m3(y / scale)):
- * what magi_swiglu_gemm_fp8_block reads next.  w_gate_up [num_experts, 2N, K], gate rows first; w_scale [num_experts,
+ * e4m3 and scales [M, ceil(N/128)] fp32 (scale = max(max|y| / 448, 2^-126) per row and 128 columns, code = e4m3(y / scale),
+ * the fp32 values' own quotients, as magi_swiglu_quantize_fp8_block takes them; y is off by at most |y| * (2^-21 + |g| *
+ * 2^-23) from silu(g) * u of its two fp32 sums, the exponential and the reciprocal being approximations, and 0 for g below
+ * -87.3): what magi_swiglu_gemm_fp8_block reads next.  w_gate_up [num_experts, 2N, K], gate rows first; w_scale [num_experts,
  * 2 * ceil(N/128), ceil(K/128)], the blocks of the gate half, then those of the up half (each half is blocked from its own
  * first row).  N % 16 == 0.
  * Replaces: gate = F.silu(gate_proj(x)); up = up_proj(x); gate * up (tests/model_definition.py:337-339) in 8 bits, with

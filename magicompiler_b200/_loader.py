@@ -17,7 +17,7 @@ CSRC = _PKG / "csrc"
 INCLUDE = _PKG.parent / "include"
 LIB_PATH = _PKG / "_lib" / "libmagi_swiglu.so"
 SOURCES = [CSRC / "swiglu_sm100.cu", CSRC / "routed_sm100.cu", CSRC / "fp8_block_sm100.cu"]
-HEADERS = [CSRC / "ptx_sm100.cuh", CSRC / "swiglu_kernels.cuh", CSRC / "swiglu_plan.hpp", CSRC / "host_common.hpp",
+HEADERS = [CSRC / "ptx_sm100.cuh", CSRC / "swiglu_kernels.cuh", CSRC / "swiglu_plan.hpp", CSRC / "host_common.hpp", CSRC / "fp8_format.cuh",
            CSRC / "routed_kernels.cuh", CSRC / "fp8_block_kernels.cuh", INCLUDE / "magi_swiglu.h"]
 
 NVCC_FLAGS = [

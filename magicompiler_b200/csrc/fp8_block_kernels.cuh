@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "fp8_format.cuh"
 #include "ptx_sm100.cuh"
 
 namespace magi {
@@ -28,8 +29,6 @@ constexpr int kRowsW = 128;               // rows of W per tile = tensor-memory 
 constexpr int kWTile = kRowsW * kBlk;     // bytes
 constexpr int kMaxStages = 8;
 constexpr long long kWaitLimit = 6000000000LL;  // three to four seconds of SM cycles
-constexpr float kCodeMax = 448.0f;
-constexpr float kScaleFloor = 1.17549435e-38f;  // 2^-126
 
 __device__ unsigned int g_fp8_watchdog[4];  // {role that gave up, block, stage/buffer, parity}
 
@@ -176,12 +175,6 @@ __device__ __forceinline__ float warp_max_nan(float v) {  // maximum of non-nega
 #pragma unroll
   for (int o = 16; o; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
   return __uint_as_float(b);
-}
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-  uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-  return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
@@ -429,15 +422,16 @@ fp8_block_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_c
         }
       } else {
         // columns beyond N hold zeros (W's rows there are zero-filled), which no maximum notices
-        const float y0 = silu_mul(v[0].x, v[1].x), y1 = silu_mul(v[0].y, v[1].y), y2 = silu_mul(v[0].z, v[1].z),
-                    y3 = silu_mul(v[0].w, v[1].w);
+        float y0 = silu_mul(v[0].x, v[1].x), y1 = silu_mul(v[0].y, v[1].y), y2 = silu_mul(v[0].z, v[1].z),
+              y3 = silu_mul(v[0].w, v[1].w);
         unsigned top = max(max(__float_as_uint(fabsf(y0)), __float_as_uint(fabsf(y1))),
                            max(__float_as_uint(fabsf(y2)), __float_as_uint(fabsf(y3))));
-        float s = __fdiv_rn(warp_max_nan(__uint_as_float(top)), kCodeMax);
-        s = s < kScaleFloor ? kScaleFloor : s;
-        // one reciprocal per row: a product with it is off by at most 2^-23 before the rounding to 4 bits
-        const float r = __frcp_rn(s);
-        if (n < a.N) *reinterpret_cast<uint32_t*>(a.codes + row * a.N + n) = pack4(y0 * r, y1 * r, y2 * r, y3 * r);
+        const float s = block_scale(warp_max_nan(__uint_as_float(top))), lift = lift_of(s);
+        y0 *= lift, y1 *= lift, y2 *= lift, y3 *= lift;
+        const Divisor d(s * lift);
+        d.divide(y0, y1);
+        d.divide(y2, y3);
+        if (n < a.N) *reinterpret_cast<uint32_t*>(a.codes + row * a.N + n) = pack4_e4m3(y0, y1, y2, y3);
         if (lane == 0) a.scales[row * a.nb + n0 / kBlk] = s;
       }
     }
@@ -819,9 +813,12 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
         top_half[part][32 * q + lane] = top;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
         top = max(top, top_half[part ^ 1][32 * q + lane]);
-        float s = __fdiv_rn(__uint_as_float(top), kCodeMax);
-        s = s < kScaleFloor ? kScaleFloor : s;
-        const float r = __frcp_rn(s);  // see the stream kernel
+        const float s = block_scale(__uint_as_float(top)), lift = lift_of(s);
+        if (__any_sync(0xffffffffu, lift != 1.0f)) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) acc[j] *= lift;
+        }
+        const Divisor d(s * lift);
         const int n = at.n0 + 64 * part;
         if (here) {
           uint8_t* dst = a.codes + row * a.N + n;
@@ -829,8 +826,12 @@ fp8_block_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
           for (int j = 0; j < 64; j += 16) {
             uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              o[i] = pack4(acc[j + 4 * i] * r, acc[j + 4 * i + 1] * r, acc[j + 4 * i + 2] * r, acc[j + 4 * i + 3] * r);
+            for (int i = 0; i < 4; ++i) {
+              float* y = acc + j + 4 * i;
+              d.divide(y[0], y[1]);
+              d.divide(y[2], y[3]);
+              o[i] = pack4_e4m3(y[0], y[1], y[2], y[3]);
+            }
             if (n + j < a.N) *reinterpret_cast<uint4*>(dst + j) = make_uint4(o[0], o[1], o[2], o[3]);
           }
           if (part == 0) a.scales[row * a.nb + at.n0 / kBlk] = s;

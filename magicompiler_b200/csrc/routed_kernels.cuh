@@ -17,14 +17,13 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "fp8_format.cuh"
 #include "ptx_sm100.cuh"
 
 namespace magi {
 
 constexpr int kMaxExperts = 1024;   // one 32-warp histogram of 1025 counters is 131 KB of shared memory
 constexpr int kSlotBatch = 4;       // expert rows of one token in flight per thread of the combine's backward
-constexpr float kFp8Max = 448.0f;   // largest e4m3 value
-constexpr float kScaleFloor = 1.17549435e-38f;  // 2^-126: a block of zeros (or of subnormals) keeps a normal scale
 
 // ---------------------------------------------------------------- sort
 // Stable counting sort of the slots by expert, slots without an expert last.  One thread-block cluster does it in one
@@ -372,28 +371,11 @@ expert_combine_backward_kernel(const uint4* dout, long long lddout, const uint4*
 // Per row and 128 columns: s = max(max|x| / 448, 2^-126), q = e4m3(x / s).  Eight lanes hold a block (16 columns each).
 // The maximum is taken on the bf16 bit patterns without their sign, which order like the values and put infinities and
 // NaN on top: a block with an infinity gets s = inf (its finite elements become 0, the infinity NaN), one with a NaN is
-// all NaN.  Codes and scales equal the formula evaluated in fp32 with IEEE divisions bit for bit: x / s is x * r with
-// r = 1 / s rounded, corrected by its own remainder (Markstein 1990: q + r * (x - q * s) with fused multiply-adds), which
-// the tests compare with IEEE division for every pair of bf16 mantissas of x and of the block's maximum; powers of two
-// change nothing as long as the remainder stays normal, so blocks with an extreme or non-finite scale divide.  8192 x 4096:
+// all NaN.  Codes and scales equal the formula evaluated in fp32 with IEEE divisions bit for bit (the tests compare them for
+// every pair of bf16 mantissas of x and of the block's maximum): the quotient is a corrected product (fp8_format.cuh), and
+// blocks with an extreme or non-finite scale, where the correction is not exact, divide.  8192 x 4096:
 // the bytes take 15.5 us; with sixteen divisions a thread 26.6 us, with the correction 18.9 us, with two values an
 // instruction 17.7 us.
-__device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
-  uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-  return (uint32_t)lo | ((uint32_t)hi << 16);
-}
-__device__ __forceinline__ float block_scale(float amax) {
-  const float s = __fdiv_rn(amax, kFp8Max);
-  return s < kScaleFloor ? kScaleFloor : s;  // a NaN stays
-}
-
-__device__ __forceinline__ void quotients(float& x0, float& x1, uint64_t minus_s, uint64_t r) {
-  const uint64_t x = pack_f32x2(x0, x1), q = mul_f32x2(x, r);
-  unpack_f32x2(fma_f32x2(r, fma_f32x2(q, minus_s, x), q), x0, x1);
-}
-
 // slot_row null: codes[t], scales[t] from x[t].  Else the quantised gather: token t goes to rows slot_row[t, j] and row
 // t * k + j gets zero codes and the floor scale when it holds no slot.
 __global__ void __launch_bounds__(256)
@@ -419,13 +401,12 @@ quantize_fp8_block_kernel(const uint4* x, long long ldx, const int* row_slot, co
   float f[8], g[8];
   bf16x8_to_f32(a, f);
   bf16x8_to_f32(b, g);
-  if (s > 7.9e-31f && s < 1.3e36f) {  // 2^-100, 2^120
-    const float inv = __frcp_rn(s);
-    const uint64_t r = pack_f32x2(inv, inv), minus_s = pack_f32x2(-s, -s);
+  if (s > kScaleSmall && s < kScaleLarge) {
+    const Divisor d(s);
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      quotients(f[i], f[i + 1], minus_s, r);
-      quotients(g[i], g[i + 1], minus_s, r);
+      d.divide(f[i], f[i + 1]);
+      d.divide(g[i], g[i + 1]);
     }
   } else {
 #pragma unroll

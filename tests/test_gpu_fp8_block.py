@@ -525,6 +525,78 @@ def test_every_form_captured_beside_other_kernels(halves, value):
     assert mb.device_status(0)["code"] == 0
 
 
+@pytest.mark.parametrize("value", [16, 32, 512 + 16, 1, 2, 4])
+@pytest.mark.parametrize("exponent", [0, -40, 40])
+def test_fused_codes_are_the_quotients_rounded_once(value, exponent):
+    """Values whose quotients lie at, or one fp32 step beside, the middle between two codes: a product with the reciprocal of the
+    scale would put many on the wrong side.  Every gate is 64 or more, where silu(g) = g in fp32, and every sum has one or two
+    terms of few bits, so the values to quantise are known bit for bit."""
+    M, N, K = 300, 128, 2048
+    grid = torch.arange(0, 127, dtype=torch.uint8, device="cuda").view(F8)  # 0 .. 448
+    step = torch.cat([grid.float()[1:] - grid.float()[:-1], torch.zeros(1, device="cuda")])
+    t = dict(offsets=None, a=torch.zeros(M, K, device="cuda"), b=torch.zeros(2 * N, K, device="cuda"))
+    t["a"][:, :2] = 1
+    t["b"][:N, 0] = 1  # gates: the row's scale
+    up = torch.cat([grid.float(), torch.zeros(1, device="cuda")])
+    t["b"][N:, 0], t["b"][N:N + 127, 1] = up, torch.where(step / 2 >= 2.0 ** -9, step / 2, 0.0)
+    t["a"], t["b"] = t["a"].to(F8), t["b"].to(F8)
+    t["a_scale"] = 64 + 64 * torch.rand(M, K // 128, generator=gen(1), device="cuda")  # 24 random bits
+    t["b_scale"] = torch.ones(2, K // 128, device="cuda")
+    t["b_scale"][1] = 2.0 ** exponent
+    with form(value):
+        codes, scales = product(t, 2)
+    g = t["a_scale"][:, :1]
+    u = (g * 2.0 ** exponent) * (up + t["b"][N:, 1].float())  # fp32: one rounding
+    y = g * u
+    s = y.amax(1, keepdim=True)
+    s = s / torch.full_like(s, 448.0)
+    assert torch.equal(scales, s)
+    assert torch.equal(codes.float(), (y / s).to(F8).float())
+    assert not torch.equal((y * (1 / s)).to(F8).float(), codes.float())  # the values do tell the two apart
+
+
+@pytest.mark.parametrize("value", [16, 32, 1, 2])
+@pytest.mark.parametrize("exponent", [-142, -140, -127, -120, -113, -111, 90, 103])
+def test_fused_codes_of_extreme_scales(value, exponent):
+    """The same quotients when the block's scale is near the ends of fp32 (K one block: the up half's scale carries it)."""
+    M, N, K = 200, 128, 128
+    t = dict(offsets=None, a=torch.zeros(M, K, device="cuda"), b=torch.zeros(2 * N, K, device="cuda"))
+    t["a"][:, 0] = 1
+    t["b"][:N, 0] = 1
+    t["b"][N:, 0] = torch.cat([torch.arange(0, 127, dtype=torch.uint8, device="cuda").view(F8).float(), torch.zeros(1, device="cuda")])
+    t["a"], t["b"] = t["a"].to(F8), t["b"].to(F8)
+    t["a_scale"] = 64 + 64 * torch.rand(M, 1, generator=gen(2), device="cuda")
+    t["b_scale"] = torch.tensor([[1.0], [2.0 ** exponent]], device="cuda")
+    with form(value):
+        codes, scales = product(t, 2)
+    g = t["a_scale"]
+    y = g * ((g * 2.0 ** exponent) * t["b"][N:, 0].float())
+    s = y.amax(1, keepdim=True)
+    s = (s / torch.full_like(s, 448.0)).clamp_min(2.0 ** -126)
+    assert torch.equal(scales, s) and torch.equal(codes.float(), (y / s).to(F8).float())
+
+
+@pytest.mark.parametrize("value", [16, 1, 2])
+def test_silu_of_one_gate_a_row(value):
+    """Gates from -80 to 80 against 64 bits: with one column a row's scale is its value over 448.  ex2 is off by 2^-22, its
+    argument -g * log2(e) by |g| * 2^-23 after two roundings, the reciprocal by 2^-23, sum and products by 2^-24 each; the scale's
+    division by 2^-24."""
+    M, K, N = 4001, 128, 16
+    g = torch.linspace(-80, 80, M, device="cuda")[:, None]
+    t = dict(offsets=None, a=torch.zeros(M, K, device="cuda"), b=torch.zeros(2 * N, K, device="cuda"))
+    t["a"][:, 0] = torch.where(g[:, 0] < 0, -1.0, 1.0)
+    t["b"][0, 0], t["b"][N, 0] = 1, 1
+    t["a"], t["b"] = t["a"].to(F8), t["b"].to(F8)
+    t["a_scale"], t["b_scale"] = g.abs(), torch.ones(2, 1, device="cuda")
+    with form(value):
+        codes, scales = product(t, 2)
+    g = g.double()
+    y = g * torch.sigmoid(g) * g  # the up sum is the gate's
+    err = (scales.double() * 448 - y.abs()).abs()
+    assert (err <= y.abs() * (2.0 ** -21 + g.abs() * 2.0 ** -23 + 2.0 ** -24) * (1 + 2.0 ** -20) + 448 * 2.0 ** -126).all()
+    assert (codes[:, 1:].float() == 0).all()
+
+
 def routed_block(s):
     row_slot, slot_row, offsets = mb.expert_sort_out(s["ids"], s["w2"].shape[0])
     a, sc = mb.expert_gather_fp8_out(s["x"], row_slot, slot_row)
