@@ -304,6 +304,21 @@ def test_quantiser_of_every_bf16_value():
         assert torch.equal(scales, ws) and torch.equal(codes.float(), wc.float())
 
 
+def test_quantiser_of_every_bf16_value_with_a_maximum_near_it():
+    """Each positive finite bf16 value in a block whose maximum is a multiple of it: powers of two, odd ones, and those that put
+    the quotient at the middle between two codes (448 / c for c = 17, 19, .. 31 sixteenths)."""
+    vals = torch.arange(0x0001, 0x7f80, dtype=torch.int32).to(torch.int16).view(BF).cuda()
+    factors = [1, 2, 4, 64, 2 ** 9, 2 ** 17, 2 ** 19, 3, 5, 7, 28, 251, 448] + [448 * 16 / c for c in range(17, 32, 2)]
+    tops = (vals.float()[:, None] * torch.tensor(factors, device="cuda")).to(BF)
+    for sign in (1, -1):
+        x = torch.zeros(vals.numel(), len(factors), 128, dtype=BF, device="cuda")
+        x[:, :, 5], x[:, :, 127] = sign * vals[:, None], tops
+        x = x.view(vals.numel(), -1)
+        codes, scales = mb.quantize_fp8_block(x)
+        wc, ws = plain_quantise(x)
+        assert torch.equal(scales, ws) and same_codes(codes, wc)
+
+
 def test_quantiser_of_every_pair_of_mantissas():
     """The quotient x / s takes one correction step instead of a division: each of the 128 bf16 mantissas of x against each
     of the 128 of the block's maximum, at every distance of exponents that gives a code other than zero, at scales near
