@@ -184,7 +184,7 @@ int magi_swiglu_expert_combine_backward_bf16(const void* dout, const void* y, co
   DeviceGuard guard;
   cudaError_t e = guard.set(device);
   if (e != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
-  // One warp walks a whole token when there are enough tokens to fill the GPU (8 warps a block, 8 blocks an SM); few
+  // One warp walks a whole token when there are enough tokens to fill the GPU (8 warps a block, 4 blocks an SM); few
   // tokens get up to eight warps each, as far as the row has pieces for them.
   int token_warps = 1;
   while (token_warps < 8 && T * token_warps < (int64_t)di->sm_count * 32 && H / 8 > token_warps * 32) token_warps *= 2;
