@@ -4,8 +4,8 @@ Importing the package registers the custom op ``magi_swiglu::gemm_swiglu`` (proc
 before a model is decorated with ``magi_compile`` so the op is a graph split point for that model, and
 before ahead-of-time artifacts that mention the op are deserialised.
 """
-from ._loader import (MagiSwigluLibraryError, build_library, device_status, kernel_clock, load_library,  # noqa: F401
-                      plan, workspace_bytes)
+from ._loader import (MagiSwigluLibraryError, build_library, device_status, fp8_block_plan, kernel_clock,  # noqa: F401
+                      load_library, plan, workspace_bytes)
 from .fp8_block import (gemm_fp8_block, gemm_fp8_block_out, gemm_swiglu_fp8_block, gemm_swiglu_fp8_block_out,  # noqa: F401
                         quantize_fp8_gate_up, quantize_fp8_weight)
 from .ops import (OP_NAME, fold_rmsnorm_weight, gemm_bf16, gemm_nt, gemm_nt_out, gemm_swiglu, gemm_swiglu_fp8, gemm_swiglu_out,  # noqa: F401
@@ -35,5 +35,5 @@ __all__ = [
     "expert_combine_backward", "expert_gather_fp8", "expert_gather_fp8_out", "quantize_fp8_block", "quantize_fp8_block_out",
     "gemm_fp8_block", "gemm_fp8_block_out", "gemm_swiglu_fp8_block", "gemm_swiglu_fp8_block_out", "quantize_fp8_weight",
     "quantize_fp8_gate_up", "RoutedSwiGLUMLP",
-    "COMPUTE_SENSITIVE_OPS", "build_library", "load_library", "plan", "workspace_bytes", "device_status", "kernel_clock", "MagiSwigluLibraryError",
+    "COMPUTE_SENSITIVE_OPS", "build_library", "load_library", "plan", "fp8_block_plan", "workspace_bytes", "device_status", "kernel_clock", "MagiSwigluLibraryError",
 ]

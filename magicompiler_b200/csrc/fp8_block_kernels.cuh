@@ -7,8 +7,8 @@
 // being written in a wider type.  With `offsets`, rows [offsets[e], offsets[e+1]) of A meet expert e's W.
 //
 // The inner sums run on the tensor cores (tcgen05 kind::f8f6f4, fp32 in tensor memory); the scales are not powers of two,
-// so every K block of 128 is finished in tensor memory, read back, scaled and added to fp32 registers.  Two accumulator
-// buffers in tensor memory let the MMAs of the next block run meanwhile.
+// so every K block of 128 is finished in tensor memory, read back, scaled and added to fp32 registers.  Several accumulator
+// buffers in tensor memory (four in the stream kernel, two in the tile kernel) let the MMAs of the next blocks run meanwhile.
 //
 // fp8_block_stream_kernel: W's rows are the MMA's 128 rows ("M") and the tokens are its columns ("N", 16..64), so few
 // tokens cost few MMA columns and few additions, and the kernel is a stream over W.  A CTA owns 128 output columns (128

@@ -198,12 +198,14 @@ static Form choose(const Problem& p, int sm_count, const int (&clusters)[3]) {
   const int64_t n_tiles = (p.N * p.halves + 255) / 256;
   const int log_splits = tile_log_splits(most_groups(p, Tile<2>::kRows) * n_tiles, p.args.kb, clusters);
   // CTA pairs (256 rows) or single CTAs (128): half as much of a small expert's last group is padding, but a CTA fetches
-  // 48 KB a K block and not 32, more yet when rows of K bytes start inside a 32-byte sector.  Pairs / singles: SwiGLU, 64
-  // experts, 15200 rows, N = 1408: K = 2048 156 / 139 us, 2064 170 / 188, 2112 178 / 155; 6000 rows, K = 2048 128 / 91; 128
-  // experts, 32768 rows, plain, N = 2048, K = 768 125 / 105; dense SwiGLU, N = 14336, K = 4096: 384 rows 79 / 64, 8192 rows
-  // 1002 / 1052.  Both add in the same order.  Short K and few rows of many experts suit single CTAs better than the stream
-  // kernel, whose CTAs are set up anew for every tile: plain, 128 experts, N = 2048, K = 768, singles / 32 tokens: 1024 rows
-  // 35 / 48 us, 4096 rows 45 / 81.
+  // 48 KB a K block and not 32, more yet when rows of K bytes start inside a 32-byte sector.  Pairs / singles, us: SwiGLU, 64
+  // experts, 16040 rows, N = 1424: K = 1024 107 / 86, 2048 172 / 149, 4096 360 / 303, but 1040 117 / 123, 2064 191 / 217, 4112
+  // 354 / 460; dense, 8192 rows, N = 4096: 1024 92 / 90, 2048 141 / 148, but 1040 101 / 130, 2064 161 / 226, 4112 293 / 437.  A
+  // short K of this kind pays less than the rule expects (K = 528, the 64 experts: 87 / 78).  Other sizes: 64 experts, 6000
+  // rows, N = 1408, K = 2048 128 / 91; 128 experts, 32768 rows, plain, N = 2048, K = 768 125 / 105; dense SwiGLU, N = 14336, K =
+  // 4096: 384 rows 79 / 64, 8192 rows 1002 / 1052.  Both add in the same order.  Short K and few rows of many experts suit
+  // single CTAs better than the stream kernel, whose CTAs are set up anew for every tile: plain, 128 experts, N = 2048, K = 768,
+  // singles / 32 tokens: 1024 rows 35 / 48 us, 4096 rows 45 / 81.
   bool single = false;
   {
     const double rounds = rounds_of(p, expected_groups(p, Tile<2>::kRows) * n_tiles, clusters[log_splits]);

@@ -6,7 +6,8 @@ projection with SwiGLU, whose result leaves in the same format), dense or over r
 ``a`` is float8_e4m3fn ``[M, K]`` with fp32 ``a_scale [M, ceil(K/128)]`` (``quantize_fp8_block`` / ``expert_gather_fp8``),
 ``b`` float8_e4m3fn ``[N, K]`` with one fp32 scale per 128 x 128 block, ``[ceil(N/128), ceil(K/128)]``
 (``quantize_fp8_weight``, once at load).  With ``offsets`` (``expert_sort``) ``b`` is ``[E, N, K]`` and rows
-``offsets[e]:offsets[e+1]`` of ``a`` meet ``b[e]``; nothing is read on the host.  Inference only: no autograd.
+``offsets[e]:offsets[e+1]`` of ``a`` meet ``b[e]`` (they start at 0 and do not fall; one that does counts as the largest
+before it); nothing is read on the host.  Inference only: no autograd.
 
 A SwiGLU block in 8 bits, routed (dense: leave out the routing and ``offsets``):
 
