@@ -23,8 +23,9 @@ __device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float 
 }
 
 // Pairs of fp32 values divided by s: x * r with r = 1 / s rounded, corrected by its own remainder (Markstein 1990: q + r * (x -
-// q * s) with fused multiply-adds), which gives the IEEE quotient as long as the remainder is exact.  It is for quotients that
-// matter to an e4m3 code (above 2^-11) and s above kScaleSmall.  s infinite: 0, of an infinity NaN.
+// q * s) with fused multiply-adds).  The remainder is exact and r off by 2^-24, so what the last step rounds is within 2^-22 of a
+// unit in the last place of x / s: the IEEE quotient but for a chance in millions.  It is for quotients that matter to an e4m3
+// code (above 2^-11) and s above kScaleSmall.  s infinite: 0, of an infinity NaN.
 struct Divisor {
   uint64_t r, minus_s;
   __device__ __forceinline__ explicit Divisor(float s) {
