@@ -9,7 +9,7 @@ namespace magi {
 
 constexpr float kFp8Max = 448.0f;               // largest e4m3 value
 constexpr float kScaleFloor = 1.17549435e-38f;  // 2^-126: a block of zeros (or of subnormals) keeps a normal scale
-constexpr float kScaleSmall = 0x1p-100f, kScaleLarge = 0x1p120f;  // see Divisor; no finite block has a larger scale
+constexpr float kScaleSmall = 0x1p-80f, kScaleLarge = 0x1p120f;  // see Divisor; no finite block has a larger scale
 
 __device__ __forceinline__ float block_scale(float amax) {
   const float s = __fdiv_rn(amax, kFp8Max);
@@ -24,8 +24,9 @@ __device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float 
 
 // Pairs of fp32 values divided by s: x * r with r = 1 / s rounded, corrected by its own remainder (Markstein 1990: q + r * (x -
 // q * s) with fused multiply-adds).  The remainder is exact and r off by 2^-24, so what the last step rounds is within 2^-22 of a
-// unit in the last place of x / s: the IEEE quotient but for a chance in millions.  It is for quotients that matter to an e4m3
-// code (above 2^-11) and s above kScaleSmall.  s infinite: 0, of an infinity NaN.
+// unit in the last place of x / s: the IEEE quotient but for a chance in millions.  That holds for quotients that matter to an
+// e4m3 code (above 2^-11) and s above kScaleSmall (the remainder's last bit is then above 2^-149).  s infinite: 0, of an infinity
+// NaN.
 struct Divisor {
   uint64_t r, minus_s;
   __device__ __forceinline__ explicit Divisor(float s) {

@@ -335,6 +335,20 @@ def test_quantiser_of_every_pair_of_mantissas():
             assert torch.equal(scales, ws) and torch.equal(codes.float(), wc.float()), (power, down)
 
 
+@pytest.mark.parametrize("power", [-73, -72, -71, -70])
+def test_quantiser_where_corrected_products_take_over_from_divisions(power):
+    """Blocks whose scale lies on either side of 2^-80: every pair of mantissas again."""
+    mant = (1.0 + torch.arange(128) / 128.0).cuda()
+    for down in range(1, 20):
+        x = torch.zeros(128, 128, device="cuda")
+        x[:, :] = mant * 2.0 ** (power - down)
+        x[:, 0] = mant * 2.0 ** power
+        x = x.to(BF)
+        codes, scales = mb.quantize_fp8_block(x)
+        wc, ws = plain_quantise(x)
+        assert torch.equal(scales, ws) and torch.equal(codes.float(), wc.float())
+
+
 def test_quantiser_of_special_values():
     x = rows_of(8, 256, 1)
     x[0, 3], x[1, 200], x[2, 5], x[3], x[4, :128] = float("nan"), float("inf"), float("-inf"), 0, 1e-40
