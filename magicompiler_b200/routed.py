@@ -20,6 +20,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.utils._device import DeviceContext
 
 from . import _loader
 from .ops import _raw_stream, _rows_view
@@ -167,7 +168,14 @@ def _plain(*operands: torch.Tensor | None) -> bool:
         if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter and t is not None:
             return False
     return not torch.compiler.is_compiling() and not torch._C._is_tracing() and torch._C._len_torch_dispatch_stack() == 0 \
-        and torch._C._len_torch_function_stack() == 0 and torch._C._functorch.peek_interpreter_stack() is None
+        and (torch._C._len_torch_function_stack() == 0 or _only_a_default_device()) \
+        and torch._C._functorch.peek_interpreter_stack() is None
+
+
+def _only_a_default_device() -> bool:
+    """Whether every torch-function mode is one of ``torch.set_default_device`` / ``with torch.device(..)``, which touch
+    nothing but factory functions."""
+    return all(type(m) is DeviceContext for m in torch.overrides._get_current_function_mode_stack())
 
 
 def _ld(t2: torch.Tensor) -> int:

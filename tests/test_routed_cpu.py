@@ -216,6 +216,20 @@ def test_a_torch_function_mode_sees_the_operators(without_kernels):
         assert {f"magi_swiglu.{op}", f"magi_swiglu.{op}.default"} & set(watch.seen), op
 
 
+def test_a_default_device_does_not_send_calls_through_the_dispatcher(without_kernels):
+    from magicompiler_b200 import routed
+
+    x = torch.zeros(3, 16, dtype=BF)
+    with torch.device("cpu"):
+        assert routed._plain(x) and routed._plain(x, None, x)
+        mb.expert_gather(x, *maps())
+        with _Watch():
+            assert not routed._plain(x)
+    with _Watch(), torch.device("cpu"):
+        assert not routed._plain(x)
+    assert routed._plain(x) and not routed._plain(x, _Wrapped(x))
+
+
 def test_the_row_movements_split_graphs():
     for op in ("expert_sort", "expert_gather", "expert_combine", "expert_gather_fp8"):
         assert f"magi_swiglu::{op}" in mb.SPLITTING_OPS
